@@ -13,7 +13,7 @@ Definitions.
                lengths[b] tokens, token p in page table[b, p // block]. A write
                of n_b tokens fills the last n_b positions: per block and head
                amax = the largest finite |new value|, s = max(old scale (none
-               for a block whose first token is written), max(amax, 2^-100) *
+               for a block whose first token is written), max(amax, 2^-80) *
                f32(1/127)); where the scale grew the block's earlier codes q
                become rint(f32(q * s_old) * f32(1 / s)); new codes are
                rint(x * f32(1 / s)), within +-127. A code stands for q * s.
@@ -332,7 +332,7 @@ def _cache_plain(s, case):
     amax = torch.where(fresh, x.abs(), 0.0).amax(dim=(3, 4))
     held = (begin[:, 0] > p * block)[:, None, None]  # the block holds earlier tokens
     old = torch.where(held, s["scales"][pages], 0.0)
-    scale = torch.maximum(old, amax.clamp(min=2.0 ** -100) * _INV127)
+    scale = torch.maximum(old, amax.clamp(min=2.0 ** -80) * _INV127)
     inverse = (1.0 / scale)[..., None, None]
     q = s["codes"][pages].float()
     moved = torch.round(q * old[..., None, None] * inverse)
@@ -504,7 +504,7 @@ def _cache_exact(s, case):
                     hi = min(length, (page0 + i + 1) * block)
                     part = x[:, lo - first:hi - first]
                     at, end = lo - (page0 + i) * block, hi - (page0 + i) * block
-                    want = f32(part.abs().amax(dim=(1, 2)).clamp(min=2.0 ** -100) * inv127)
+                    want = f32(part.abs().amax(dim=(1, 2)).clamp(min=2.0 ** -80) * inv127)
                     t = torch.maximum(scale[i], want) if at else want
                     inv = f32(1.0 / t)[:, None, None]
                     held = q[i, :, :at]
