@@ -335,6 +335,8 @@ int cim22_cuda_model_invoke(cim22_cuda_model *model, void **buffers, const int64
 #define CIM22_STATUS_CHIP_NOT_FINITE 0x80   /* Legacy: a chip output to compensate is not finite */
 #define CIM22_STATUS_LEGACY_SCALING 0x100   /* Legacy group scaling changed prealigned mantissas */
 #define CIM22_STATUS_LEGACY_I21 0x200       /* Legacy: all -128 input group and weight lane */
+#define CIM22_STATUS_CACHE_INDEX 0x400      /* key/value cache: page, length or start out of range */
+#define CIM22_STATUS_CACHE_NOT_FINITE 0x800 /* NaN/Inf written to the 8-bit key/value cache */
 
 /* Message of the lowest set status bit ("" for 0). */
 const char *cim22_cuda_status_message(int32_t status);
@@ -755,6 +757,138 @@ int cim22_cuda_channel_affine_nchw(const float *x, const float *scale,
                                    const float *shift, float *y, int32_t n,
                                    int32_t c, int64_t hw, int32_t activation,
                                    void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* Glue of decoder blocks (no counterpart in the reference): the norms around
+ * a block with its gate and residual, an 8-bit key/value cache, attention over
+ * it. Activations are f32 (what the CIM layers read and write), bf16 or f16;
+ * all arithmetic is f32. Every launch goes to the current device, which must
+ * be the one that holds the memory. */
+#define CIM22_FLOAT32 0
+#define CIM22_BFLOAT16 1
+#define CIM22_FLOAT16 2
+
+#define CIM22_NORM_NONE 0
+#define CIM22_NORM_RMS 1   /* v / sqrt(mean(v^2) + eps) * weight (+ bias) */
+#define CIM22_NORM_LAYER 2 /* the same of v - mean(v) */
+typedef struct cim22_norm {
+  int32_t kind;       /* CIM22_NORM_RMS or CIM22_NORM_LAYER */
+  float eps;
+  const void *weight; /* device [dim], or NULL for ones */
+  const void *bias;   /* device [dim], or NULL */
+  int32_t type;       /* of weight and bias: CIM22_FLOAT32 or the activations' */
+} cim22_norm;
+
+#define CIM22_GATE_NONE 0
+#define CIM22_GATE_SIGMOID 1
+#define CIM22_GATE_TANH 2
+#define CIM22_BLOCK_NORM_MAX_DIM 16384
+/* h = residual_scale * residual + act(gate) * post(x), y = pre(h): a block's
+ * output x normed, gated and added to the residual stream, and the stream
+ * normed for the next block, in one pass. y is computed from h before h is
+ * rounded to the activations' type. Rows are contiguous; strides count
+ * elements. x or residual may be h or y of the same call (same stride). */
+typedef struct cim22_block_norm {
+  int32_t type;           /* of x, residual, h and y */
+  int64_t rows, dim;      /* 1 <= dim <= CIM22_BLOCK_NORM_MAX_DIM */
+  const void *x;
+  int64_t x_stride;
+  const void *residual;   /* or NULL */
+  int64_t residual_stride;
+  float residual_scale;
+  const void *gate;       /* or NULL (a gate of one) */
+  int64_t gate_stride;    /* between gate rows */
+  int64_t gate_rows;      /* consecutive rows that share a gate row; 0: all rows */
+  int64_t gate_columns;   /* dim, or 1: one value for a whole row */
+  int32_t gate_type;      /* CIM22_FLOAT32 or the activations' */
+  int32_t gate_activation; /* CIM22_GATE_* */
+  const cim22_norm *post; /* or NULL */
+  const cim22_norm *pre;  /* or NULL: y = h */
+  void *h;                /* or NULL */
+  int64_t h_stride;
+  void *y;                /* or NULL */
+  int64_t y_stride;
+} cim22_block_norm;
+int cim22_cuda_block_norm(const cim22_block_norm *description, void *stream);
+
+/* A paged key/value cache in 8 bits: int8 codes [pages][kv_heads][2][block]
+ * [head_dim] (0 = key, 1 = value) and one f32 scale [pages][kv_heads][2] for
+ * each block of tokens, head and side; a code q stands for q * scale. Token p
+ * of sequence b lies in page table[b * table_stride + p / block]. Pages may
+ * be shared by sequences that only read them.
+ *
+ * The same sequence description serves the write, the read and the attention:
+ * lengths[b] counts the tokens that sequence b holds with this call's tokens,
+ * which are its last n_b; their rows are packed, sequence b's from starts[b]
+ * to starts[b + 1] - 1 (starts NULL: one row for every sequence). A token at
+ * a negative position (lengths[b] < n_b, such as an empty slot's) is neither
+ * written nor read. Rows from starts[batch] on are left alone. Offsets,
+ * lengths or page numbers out of range are not followed: they set
+ * CIM22_STATUS_CACHE_INDEX and the tokens in question are skipped. */
+typedef struct cim22_kv_cache {
+  int8_t *codes;   /* 16-byte aligned */
+  float *scales;   /* 8-byte aligned */
+  int64_t pages;
+  int32_t kv_heads;
+  int32_t block;   /* tokens a page: 16, 32, 64 or 128 */
+  int32_t head_dim; /* a multiple of 16, at most 128 */
+} cim22_kv_cache;
+typedef struct cim22_kv_sequences {
+  int32_t batch;
+  const int32_t *table;   /* device, page numbers */
+  int64_t table_stride;
+  int32_t table_width;    /* pages a row of the table can hold */
+  const int32_t *lengths; /* device [batch] */
+  const int32_t *starts;  /* device [batch + 1] or NULL */
+  int64_t rows;           /* packed rows that the row arrays hold */
+  int32_t most;           /* host bound of n_b: more is an index error */
+} cim22_kv_sequences;
+
+/* Writes packed rows of keys and values, [rows][kv_heads][head_dim] with the
+ * given row and head strides in elements (last axis contiguous). Each touched
+ * block's scale becomes max(its old one, max(amax, 2^-80) * f32(1/127)), amax
+ * the largest finite magnitude among the block's new values (the old scale
+ * counts only when the block holds earlier tokens); where it grew, the
+ * earlier codes q become rint(f32(q * old) * f32(1 / scale)). New codes are
+ * rint(f32(x * f32(1 / scale))) within +-127; infinities become +-127, NaN 0,
+ * and both set CIM22_STATUS_CACHE_NOT_FINITE. Two sequences of one call must
+ * not write the same page. */
+int cim22_cuda_kv_write(const cim22_kv_cache *cache, const cim22_kv_sequences *sequences,
+                        int32_t type, const void *k, int64_t k_row_stride, int64_t k_head_stride,
+                        const void *v, int64_t v_row_stride, int64_t v_head_stride,
+                        int32_t *status, void *stream);
+/* Reads each sequence's last n_b tokens back as values f32(q * scale), rounded
+ * to `type`, into contiguous packed rows [rows][kv_heads][head_dim]; k or v
+ * may be NULL. */
+int cim22_cuda_kv_read(const cim22_kv_cache *cache, const cim22_kv_sequences *sequences,
+                       int32_t type, void *k, void *v, int32_t *status, void *stream);
+
+/* out = softmax(scale * q k^T) v over the values that the cache's codes stand
+ * for. q is [rows][q_heads][head_dim] (strides in elements, last axis
+ * contiguous), q head h reads kv head h / (q_heads / kv_heads). Query i of n_b
+ * sits at position lengths[b] - n_b + i; causal: it sees positions up to its
+ * own, otherwise all lengths[b]; window > 0: only positions above its own
+ * minus window. A query that sees nothing gives zeros and lse = -inf. out is
+ * contiguous [rows][q_heads][head_dim] of q's type; lse (or NULL) is f32
+ * [rows][q_heads], the natural logarithm of the sum of exp(score). */
+typedef struct cim22_kv_attention {
+  int32_t type;
+  int32_t q_heads;
+  const void *q;
+  int64_t q_row_stride, q_head_stride;
+  void *out;
+  float *lse;
+  float scale;
+  int32_t causal;
+  int32_t window;
+  int64_t longest; /* host bound of lengths[b] that the split is planned for (any value is right) */
+} cim22_kv_attention;
+size_t cim22_cuda_kv_attend_workspace(const cim22_kv_cache *cache,
+                                      const cim22_kv_sequences *sequences,
+                                      const cim22_kv_attention *attention);
+int cim22_cuda_kv_attend(const cim22_kv_cache *cache, const cim22_kv_sequences *sequences,
+                         const cim22_kv_attention *attention, void *workspace,
+                         size_t workspace_bytes, int32_t *status, void *stream);
 
 #ifdef __cplusplus
 }

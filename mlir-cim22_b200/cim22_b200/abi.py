@@ -236,6 +236,92 @@ class PeerFlags(ctypes.Structure):
     ]
 
 
+# Activation types of the decoder-block glue (include/cim22_cuda.h).
+FLOAT32, BFLOAT16, FLOAT16 = range(3)
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
+GATE_NONE, GATE_SIGMOID, GATE_TANH = range(3)
+
+
+class Norm(ctypes.Structure):
+    """cim22_norm: one RMS or layer norm over the last axis."""
+    _fields_ = [
+        ("kind", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("type", ctypes.c_int32),
+    ]
+
+
+class BlockNorm(ctypes.Structure):
+    """cim22_block_norm: post norm, gate, residual and pre norm of one call."""
+    _fields_ = [
+        ("type", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("dim", ctypes.c_int64),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("residual_scale", ctypes.c_float),
+        ("gate", ctypes.c_void_p),
+        ("gate_stride", ctypes.c_int64),
+        ("gate_rows", ctypes.c_int64),
+        ("gate_columns", ctypes.c_int64),
+        ("gate_type", ctypes.c_int32),
+        ("gate_activation", ctypes.c_int32),
+        ("post", ctypes.POINTER(Norm)),
+        ("pre", ctypes.POINTER(Norm)),
+        ("h", ctypes.c_void_p),
+        ("h_stride", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    """cim22_kv_cache: int8 pages and their scales."""
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int32),
+        ("block", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+    ]
+
+
+class KvSequences(ctypes.Structure):
+    """cim22_kv_sequences: page table, lengths and packed rows of one call."""
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("table_width", ctypes.c_int32),
+        ("lengths", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("most", ctypes.c_int32),
+    ]
+
+
+class KvAttention(ctypes.Structure):
+    """cim22_kv_attention: queries, outputs and mask of one call."""
+    _fields_ = [
+        ("type", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("longest", ctypes.c_int64),
+    ]
+
+
 ABI_STRUCTS = (
     FramePacket,
     StaticWeight,
@@ -250,6 +336,11 @@ ABI_STRUCTS = (
     ChainLayer,
     PeerOutputs,
     PeerFlags,
+    Norm,
+    BlockNorm,
+    KvCache,
+    KvSequences,
+    KvAttention,
 )
 
 

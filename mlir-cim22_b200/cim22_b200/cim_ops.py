@@ -6,7 +6,9 @@ kernel of libcim22_cuda.so. Tensors must be contiguous CUDA tensors.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+from dataclasses import dataclass
 
 import numpy as np
 import torch
@@ -30,15 +32,32 @@ def _require(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
         raise TypeError(f"{name} must be a contiguous CUDA {dtype} tensor")
 
 
+FLOAT_TYPES = {torch.float32: abi.FLOAT32, torch.bfloat16: abi.BFLOAT16,
+               torch.float16: abi.FLOAT16}
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which launches go to a tensor's device."""
+    if device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
+
+
 class Workspace:
-    """Grow-only scratch buffer shared by the layers of one program."""
+    """Grow-only scratch buffer shared by the layers of one program, which run
+    one after another. Buffers it has outgrown are kept, since a captured graph
+    may still use them (each is at least twice the one before)."""
 
     def __init__(self, device: torch.device) -> None:
         self.device = device
         self.buffer = torch.empty(0, dtype=torch.uint8, device=device)
+        self.outgrown: list[torch.Tensor] = []
 
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buffer.numel() < nbytes:
+            if self.buffer.numel():
+                self.outgrown.append(self.buffer)
             self.buffer = torch.empty(max(nbytes, 2 * self.buffer.numel()), dtype=torch.uint8,
                                       device=self.device)
         return self.buffer
@@ -403,6 +422,129 @@ def softmax(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     check(lib().cim22_cuda_softmax(_ptr(x), _ptr(out), x.numel() // cols, cols,
                                    _stream(x.device)), "softmax")
     return out
+
+
+@dataclass(frozen=True)
+class Norm:
+    """An RMS ("rms") or layer ("layer") norm over the last axis: v /
+    sqrt(mean(v^2) + eps) * weight + bias of v, or of v - mean(v). Weight and
+    bias are [dim], of one type: f32 or the activations'; None for ones and
+    zeros."""
+
+    kind: str
+    weight: torch.Tensor | None = None
+    bias: torch.Tensor | None = None
+    eps: float = 1e-6
+
+
+_NORM_KIND = {"rms": abi.NORM_RMS, "layer": abi.NORM_LAYER}
+_GATE_ACT = {None: abi.GATE_NONE, "none": abi.GATE_NONE, "sigmoid": abi.GATE_SIGMOID,
+             "tanh": abi.GATE_TANH}
+
+
+def _as_rows(t: torch.Tensor, like: torch.Tensor, name: str) -> int:
+    """The row stride of a tensor taken as rows of its last axis: any 2-D tensor
+    whose last axis is contiguous, or a contiguous one."""
+    if t.device != like.device or t.dtype != like.dtype or t.shape != like.shape:
+        raise TypeError(f"{name} must have x's shape, type and device")
+    dim = t.shape[-1]
+    if t.dim() == 2 and (t.stride(1) == 1 or dim == 1) and (t.shape[0] <= 1
+                                                            or t.stride(0) >= dim):
+        return t.stride(0)
+    if not t.is_contiguous():
+        raise TypeError(f"{name} must be contiguous, or rows with a contiguous last axis")
+    return dim
+
+
+def _norm_arg(norm: Norm | None, x: torch.Tensor, name: str) -> abi.Norm | None:
+    if norm is None:
+        return None
+    if norm.kind not in _NORM_KIND:
+        raise ValueError(f"{name} norm must be \"rms\" or \"layer\"")
+    arg = abi.Norm(kind=_NORM_KIND[norm.kind], eps=norm.eps, type=FLOAT_TYPES[x.dtype])
+    kinds = set()
+    for field, t in (("weight", norm.weight), ("bias", norm.bias)):
+        if t is None:
+            continue
+        if t.device != x.device or t.dtype not in (torch.float32, x.dtype) \
+                or t.shape != x.shape[-1:] or not t.is_contiguous():
+            raise TypeError(f"{name} {field} must be a contiguous [dim] tensor on x's device, "
+                            "f32 or of x's type")
+        kinds.add(t.dtype)
+        arg.type = FLOAT_TYPES[t.dtype]
+        setattr(arg, field, t.data_ptr())
+    if len(kinds) > 1:
+        raise TypeError(f"{name} weight and bias must have one type")
+    return arg
+
+
+def block_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
+               post: Norm | None = None, pre: Norm | None = None,
+               gate: torch.Tensor | None = None, gate_activation: str | None = None,
+               residual_scale: float = 1.0, out: torch.Tensor | None = None,
+               normed: torch.Tensor | None = None
+               ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """The norms before and after a decoder block with its gate and residual
+    between them, in one pass:
+
+        h = residual_scale * residual + act(gate) * post(x),   y = pre(h)
+
+    x is the block's output, [..., dim] f32, bf16 or f16; returns (h, y), h
+    None when there is nothing to combine (no residual, post or gate) and y
+    None without pre. gate is [dim]; [rows, dim] or [rows, 1]; or, for a batch
+    of equally long sequences, [groups, dim] or [groups, 1] with groups
+    dividing the rows (consecutive rows share a gate row); f32 or x's type;
+    gate_activation None, "sigmoid" or "tanh". Arithmetic is f32, and y is
+    computed from h before h is rounded. out and normed receive h and y; they
+    may be x or residual themselves (the same view), but not overlap them in
+    any other way."""
+    if not x.is_cuda or x.dtype not in FLOAT_TYPES or x.dim() < 1:
+        raise TypeError("x must be a CUDA f32, bf16 or f16 tensor")
+    dim = x.shape[-1]
+    if not 1 <= dim <= 16384:
+        raise ValueError("x's last axis must have 1 to 16384 elements")
+    rows = x.numel() // dim
+    if gate_activation not in _GATE_ACT:
+        raise ValueError("gate activation must be None, sigmoid or tanh")
+    d = abi.BlockNorm(type=FLOAT_TYPES[x.dtype], rows=rows, dim=dim, x=x.data_ptr(),
+                      x_stride=_as_rows(x, x, "x"), residual_scale=residual_scale)
+    if residual is not None:
+        d.residual, d.residual_stride = residual.data_ptr(), _as_rows(residual, x, "residual")
+    if gate is not None:
+        if gate.device != x.device or gate.dtype not in (torch.float32, x.dtype) \
+                or not gate.is_contiguous():
+            raise TypeError("gate must be a contiguous tensor on x's device, f32 or of x's type")
+        lead = gate.numel() // max(1, gate.shape[-1]) if gate.dim() else 0
+        if gate.dim() == 1 and gate.shape[0] == dim:
+            lead = 1
+        elif gate.dim() < 2 or gate.shape[-1] not in (1, dim) \
+                or lead < 1 and rows or lead and rows % lead:
+            raise ValueError("gate must be [dim], or [groups, dim] or [groups, 1] with groups "
+                             "dividing the rows")
+        d.gate, d.gate_type = gate.data_ptr(), FLOAT_TYPES[gate.dtype]
+        d.gate_columns = d.gate_stride = gate.shape[-1]
+        d.gate_rows = rows // lead if lead > 1 else 0
+        d.gate_activation = _GATE_ACT[gate_activation]
+    combined = residual is not None or post is not None or gate is not None
+    post_arg, pre_arg = _norm_arg(post, x, "post"), _norm_arg(pre, x, "pre")
+    h = y = None
+    if combined or out is not None:
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+        d.h, d.h_stride = h.data_ptr(), _as_rows(h, x, "out")
+    if pre is not None:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if normed is None else normed
+        d.y, d.y_stride = y.data_ptr(), _as_rows(y, x, "normed")
+    elif normed is not None:
+        raise ValueError("normed is an output of pre: it needs one")
+    if h is None and y is None:
+        raise ValueError("nothing to compute: give a residual, post, gate or pre")
+    if post_arg is not None:
+        d.post = ctypes.pointer(post_arg)
+    if pre_arg is not None:
+        d.pre = ctypes.pointer(pre_arg)
+    with on_device(x.device):
+        check(lib().cim22_cuda_block_norm(ctypes.byref(d), _stream(x.device)), "block_norm")
+    return h, y
 
 
 def nhwc_to_nchw(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -114,6 +114,11 @@ _SIGNATURES = {
     "cim22_cuda_avgpool2d_nchw": (c.c_int, [P, P, I32, I32, I32, I32, I32, I32, P]),
     "cim22_cuda_global_avgpool_nchw": (c.c_int, [P, P, I32, I32, I32, I32, P]),
     "cim22_cuda_channel_affine_nchw": (c.c_int, [P, P, P, P, I32, I32, I64, I32, P]),
+    "cim22_cuda_block_norm": (c.c_int, [P, P]),
+    "cim22_cuda_kv_write": (c.c_int, [P, P, I32, P, I64, I64, P, I64, I64, P, P]),
+    "cim22_cuda_kv_read": (c.c_int, [P, P, I32, P, P, P, P]),
+    "cim22_cuda_kv_attend_workspace": (SZ, [P, P, P]),
+    "cim22_cuda_kv_attend": (c.c_int, [P, P, P, P, SZ, P, P]),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -138,8 +143,8 @@ def lib() -> ctypes.CDLL:
 
 
 def abi_sizes() -> list[int]:
-    sizes = (ctypes.c_int64 * 16)()
-    n = lib().cim22_cuda_abi_sizes(sizes, 16)
+    sizes = (ctypes.c_int64 * 32)()
+    n = lib().cim22_cuda_abi_sizes(sizes, 32)
     return list(sizes[:n])
 
 

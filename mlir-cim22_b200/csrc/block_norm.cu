@@ -1,0 +1,343 @@
+// block_norm.cu - the norms before and after a decoder block with the block's
+// gate and residual add between them, one pass over the data:
+//
+//   h = residual_scale * residual + act(gate) * post(x)      (stored as T)
+//   y = pre(h)                                               (stored as T)
+//
+// post / pre: RMS norm v / sqrt(mean(v^2) + eps) * w (+ b) or layer norm
+// (v - mean) / sqrt(mean((v - mean)^2) + eps) * w (+ b), over the row. All
+// arithmetic is f32; pre reads h before it is rounded to T, so y carries one
+// rounding only.
+//
+// Bound by HBM (x and residual read once, h and y written once): a row stays
+// in registers between the reductions, kPer 16-byte vectors a thread, W warps
+// a row.
+#include "decoder_util.cuh"
+
+#include <algorithm>
+
+namespace cim {
+namespace {
+
+struct NormArg {
+  int kind; // CIM22_NORM_*
+  float eps;
+  const void *weight, *bias;
+  int type; // of weight and bias
+};
+
+struct BlockNormArgs {
+  const void *x, *residual, *gate;
+  void *h, *y;
+  int64_t rows, dim, x_stride, residual_stride, gate_stride, h_stride, y_stride;
+  int64_t gate_rows; // consecutive rows that share a gate row
+  int gate_type, gate_columns, gate_act;
+  float residual_scale;
+  NormArg post, pre;
+  int warps_log2; // warps a row, log2
+};
+
+// kVec parameter values at element e as f32 (`fill` outside the row).
+template <int N>
+__device__ __forceinline__ void load_params(const void *base, int type, int64_t e, int64_t count,
+                                            float (&out)[N]) {
+  if (type == CIM22_FLOAT32) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4) {
+      const Pack<float> p = load_pack(static_cast<const float *>(base), e + c, count);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        out[c + i] = p.at[i];
+    }
+  } else if constexpr (N == 8) {
+    if (type == CIM22_BFLOAT16) {
+      const Pack<__nv_bfloat16> p = load_pack(static_cast<const __nv_bfloat16 *>(base), e, count);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        out[i] = to_f32(p.at[i]);
+    } else {
+      const Pack<__half> p = load_pack(static_cast<const __half *>(base), e, count);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        out[i] = to_f32(p.at[i]);
+    }
+  }
+}
+
+__device__ __forceinline__ float gate_fn(float g, int act) {
+  if (act == CIM22_GATE_SIGMOID)
+    return 1.0f / (1.0f + expf(-g));
+  if (act == CIM22_GATE_TANH)
+    return tanhf(g);
+  return g;
+}
+
+// Sum over the W warps of a row; `slot` alternates so that one barrier a
+// reduction is enough.
+__device__ __forceinline__ float row_sum(float v, int warps_log2, float *buffer, int &slot) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (warps_log2 == 0)
+    return v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float *part = buffer + 32 * slot;
+  slot ^= 1;
+  if (lane == 0)
+    part[warp] = v;
+  __syncthreads();
+  const int w = 1 << warps_log2;
+  v = lane < w ? part[(warp & ~(w - 1)) + lane] : 0.0f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T, int kPer, int kMax>
+__global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a) {
+  constexpr int V = kVec<T>;
+  __shared__ float buffer[64];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int w = 1 << a.warps_log2;
+  const int64_t row_at = static_cast<int64_t>(blockIdx.x) * ((blockDim.x >> 5) >> a.warps_log2) +
+                         (warp >> a.warps_log2);
+  const bool live = row_at < a.rows;
+  const int64_t row = live ? row_at : a.rows - 1; // every thread reaches the barriers
+  const int thread = ((warp & (w - 1)) << 5) | lane;
+  const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+  const T *residual = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
+  // Vectors are aligned to x's 16-byte boundaries: the first starts `phase`
+  // elements before the row.
+  const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const float inverse = 1.0f / static_cast<float>(a.dim);
+  int slot = 0;
+
+  Pack<T> raw[kPer], res[kPer];
+  float v[kPer][V];
+#pragma unroll
+  for (int p = 0; p < kPer; ++p)
+    raw[p] = load_pack(x, static_cast<int64_t>(p * (w << 5) + thread) * V - phase, a.dim);
+  if (residual) {
+#pragma unroll
+    for (int p = 0; p < kPer; ++p)
+      res[p] = load_pack(residual, static_cast<int64_t>(p * (w << 5) + thread) * V - phase, a.dim);
+  }
+#pragma unroll
+  for (int p = 0; p < kPer; ++p)
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      v[p][i] = to_f32(raw[p].at[i]);
+
+  auto normalise = [&](const NormArg &n) {
+    float mean = 0.0f;
+    if (n.kind == CIM22_NORM_LAYER) {
+      float s = 0.0f;
+#pragma unroll
+      for (int p = 0; p < kPer; ++p)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          s += v[p][i]; // zero outside the row
+      mean = row_sum(s, a.warps_log2, buffer, slot) * inverse;
+    }
+    float s = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      const int64_t e = static_cast<int64_t>(p * (w << 5) + thread) * V - phase;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[p][i] = (e + i >= 0 && e + i < a.dim) ? v[p][i] - mean : 0.0f;
+        s = fmaf(v[p][i], v[p][i], s);
+      }
+    }
+    const float power = row_sum(s, a.warps_log2, buffer, slot) * inverse;
+    const float scale = 1.0f / sqrtf(power + n.eps);
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      const int64_t e = static_cast<int64_t>(p * (w << 5) + thread) * V - phase;
+      float g[V];
+      if (n.weight) {
+        load_params<V>(n.weight, n.type, e, a.dim, g);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          v[p][i] *= scale * g[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          v[p][i] *= scale;
+      }
+      if (n.bias) {
+        load_params<V>(n.bias, n.type, e, a.dim, g);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          v[p][i] += g[i];
+      }
+    }
+  };
+
+  if (a.post.kind != CIM22_NORM_NONE)
+    normalise(a.post);
+  if (a.gate) {
+    const int64_t at = a.gate_rows ? row / a.gate_rows * a.gate_stride : 0;
+    const char *gate = static_cast<const char *>(a.gate) + at * (a.gate_type == CIM22_FLOAT32 ? 4 : 2);
+    if (a.gate_columns == 1) {
+      float g;
+      if (a.gate_type == CIM22_FLOAT32)
+        g = *reinterpret_cast<const float *>(gate);
+      else if (a.gate_type == CIM22_BFLOAT16)
+        g = to_f32(*reinterpret_cast<const __nv_bfloat16 *>(gate));
+      else
+        g = to_f32(*reinterpret_cast<const __half *>(gate));
+      g = gate_fn(g, a.gate_act);
+#pragma unroll
+      for (int p = 0; p < kPer; ++p)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          v[p][i] *= g;
+    } else {
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        float g[V];
+        load_params<V>(gate, a.gate_type, static_cast<int64_t>(p * (w << 5) + thread) * V - phase,
+                       a.dim, g);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          v[p][i] *= gate_fn(g[i], a.gate_act);
+      }
+    }
+  }
+  if (residual) {
+#pragma unroll
+    for (int p = 0; p < kPer; ++p)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        v[p][i] = fmaf(a.residual_scale, to_f32(res[p].at[i]), v[p][i]);
+  }
+  auto put = [&](void *out, int64_t stride) {
+    if (!live)
+      return;
+    T *to = static_cast<T *>(out) + row * stride;
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      Pack<T> o;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        o.at[i] = from_f32<T>(v[p][i]);
+      store_pack(to, static_cast<int64_t>(p * (w << 5) + thread) * V - phase, a.dim, o);
+    }
+  };
+  if (a.h)
+    put(a.h, a.h_stride);
+  if (a.y) {
+    if (a.pre.kind != CIM22_NORM_NONE)
+      normalise(a.pre);
+    put(a.y, a.y_stride);
+  }
+}
+
+template <typename T>
+cudaError_t launch_block_norm(BlockNormArgs a, cudaStream_t stream) {
+  constexpr int V = kVec<T>;
+  const bool aligned = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.x_stride % V == 0;
+  const int64_t vectors = (a.dim + (aligned ? 0 : V - 1) + V - 1) / V;
+  // Vectors a thread and warps a row: the fewest warps that hold the row.
+  int per = 1, log2w = 0;
+  while (per < 4 && (int64_t{32} * per) < vectors)
+    per *= 2;
+  while ((int64_t{32} * per << log2w) < vectors)
+    ++log2w;
+  if (log2w > 5) { // the widest rows, off a vector boundary: one vector too many
+    per = 8;
+    log2w = 5;
+  }
+  a.warps_log2 = log2w;
+  const int warps = std::max(8, 1 << log2w);
+  const int64_t rows_per = warps >> log2w;
+  const int64_t grid = (a.rows + rows_per - 1) / rows_per;
+  const auto kernel = per == 1       ? block_norm_kernel<T, 1, 256>
+                      : per == 2     ? block_norm_kernel<T, 2, 256>
+                      : per == 8     ? block_norm_kernel<T, 8, 1024>
+                      : warps <= 8   ? block_norm_kernel<T, 4, 256>
+                      : warps <= 16  ? block_norm_kernel<T, 4, 512>
+                                     : block_norm_kernel<T, 4, 1024>;
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(warps * 32), 0, stream, a);
+}
+
+bool refuse(const char *why) {
+  set_last_error(std::string("cim22_cuda_block_norm: ") + why);
+  return false;
+}
+
+bool norm_arg(const cim22_norm *n, int32_t type, NormArg &out) {
+  out = NormArg{CIM22_NORM_NONE, 0.0f, nullptr, nullptr, type};
+  if (!n)
+    return true;
+  if (n->kind != CIM22_NORM_RMS && n->kind != CIM22_NORM_LAYER)
+    return refuse("norm kind must be CIM22_NORM_RMS or CIM22_NORM_LAYER");
+  if (n->type != CIM22_FLOAT32 && n->type != type)
+    return refuse("norm weights must be f32 or the activations' type");
+  if (!(n->eps >= 0.0f))
+    return refuse("norm eps must not be negative");
+  out = NormArg{n->kind, n->eps, n->weight, n->bias, n->type};
+  return true;
+}
+
+} // namespace
+} // namespace cim
+
+extern "C" int cim22_cuda_block_norm(const cim22_block_norm *d, void *stream) {
+  using namespace cim;
+  const int bad = CIM22_STATUS_BAD_ARGUMENT;
+  if (!d)
+    return refuse("null description"), bad;
+  if (!float_type(d->type))
+    return refuse("unknown activation type"), bad;
+  if (d->rows < 0 || d->dim < 1 || d->dim > CIM22_BLOCK_NORM_MAX_DIM || d->rows > 0x7fffffff)
+    return refuse("rows or dim out of range"), bad;
+  if (d->rows > 0 && (!d->x || (!d->h && !d->y)))
+    return refuse("null x, or neither h nor y"), bad;
+  if ((d->rows > 1) && (d->x_stride < d->dim || (d->residual && d->residual_stride < d->dim) ||
+                        (d->h && d->h_stride < d->dim) || (d->y && d->y_stride < d->dim)))
+    return refuse("row strides must be at least dim"), bad;
+  if (d->gate) {
+    if (d->gate_type != CIM22_FLOAT32 && d->gate_type != d->type)
+      return refuse("gate must be f32 or the activations' type"), bad;
+    if (d->gate_columns != 1 && d->gate_columns != d->dim)
+      return refuse("gate must have 1 or dim columns"), bad;
+    if (d->gate_rows < 0 || d->gate_activation < 0 || d->gate_activation > CIM22_GATE_TANH)
+      return refuse("gate rows or activation out of range"), bad;
+  }
+  BlockNormArgs a{};
+  if (!norm_arg(d->post, d->type, a.post) || !norm_arg(d->pre, d->type, a.pre))
+    return bad;
+  if (d->rows == 0)
+    return 0;
+  a.x = d->x;
+  a.residual = d->residual;
+  a.gate = d->gate;
+  a.h = d->h;
+  a.y = d->y;
+  a.rows = d->rows;
+  a.dim = d->dim;
+  a.x_stride = d->x_stride;
+  a.residual_stride = d->residual_stride;
+  a.gate_stride = d->gate_stride;
+  a.h_stride = d->h_stride;
+  a.y_stride = d->y_stride;
+  a.gate_rows = d->gate_rows;
+  a.gate_type = d->gate_type;
+  a.gate_columns = static_cast<int>(d->gate_columns == d->dim ? 0 : 1);
+  a.gate_act = d->gate_activation;
+  a.residual_scale = d->residual_scale;
+  const auto s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (d->type == CIM22_FLOAT32)
+    e = launch_block_norm<float>(a, s);
+  else if (d->type == CIM22_BFLOAT16)
+    e = launch_block_norm<__nv_bfloat16>(a, s);
+  else
+    e = launch_block_norm<__half>(a, s);
+  return cuda_ok(e, "block_norm") ? 0 : bad;
+}

@@ -46,6 +46,10 @@ const char *cim22_cuda_status_message(int32_t status) {
     return "CIM BF16 result exceeds signed i21 range";
   if (status & CIM22_STATUS_CHIP_NOT_FINITE)
     return "CIM BF16 chip output is not finite";
+  if (status & CIM22_STATUS_CACHE_INDEX)
+    return "key/value cache page, length or start out of range";
+  if (status & CIM22_STATUS_CACHE_NOT_FINITE)
+    return "key/value cache does not support NaN or infinity";
   return "";
 }
 
@@ -59,7 +63,9 @@ int cim22_cuda_abi_sizes(int64_t *sizes, int capacity) {
       sizeof(cim22_transaction),   sizeof(cim22_trace_event),
       sizeof(cim22_memref2d),      sizeof(cim22_gather),
       sizeof(cim22_chain_layer),   sizeof(cim22_peer_outputs),
-      sizeof(cim22_peer_flags)};
+      sizeof(cim22_peer_flags),    sizeof(cim22_norm),
+      sizeof(cim22_block_norm),    sizeof(cim22_kv_cache),
+      sizeof(cim22_kv_sequences),  sizeof(cim22_kv_attention)};
   const int n = static_cast<int>(sizeof(all) / sizeof(all[0]));
   if (sizes)
     for (int i = 0; i < std::min(n, capacity); ++i)

@@ -1,0 +1,117 @@
+// kv_attention.h - what the attention kernels over the 8-bit cache share.
+#pragma once
+
+#include "kv_util.cuh"
+
+#include <atomic>
+
+namespace cim {
+
+struct KvAttendArgs {
+  KvView v;
+  const void *q;
+  int64_t q_row_stride, q_head_stride;
+  void *out;
+  float *lse;
+  float scale_log2; // softmax scale * log2(e)
+  int q_heads, group, causal, window;
+  int splits;     // parts of the key axis
+  float *part_o;  // [splits][rows * q_heads][dim], relative to 2^m, when splits > 1
+  float4 *part_ml; // [splits][rows * q_heads] (m, l, unrounded l, -)
+  int32_t *status;
+};
+
+// Allows a kernel its dynamic shared memory, once for each device.
+class DynamicSmem {
+public:
+  template <typename K> cudaError_t allow(K kernel, size_t bytes) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && done_.load() >> device & 1))
+      return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(bytes));
+    if (e == cudaSuccess && device < 64)
+      done_.fetch_or(uint64_t{1} << device);
+    return e;
+  }
+
+private:
+  std::atomic<uint64_t> done_{0};
+};
+
+#if defined(__CUDACC__)
+namespace {
+
+// Softmax over values held as codes with a scale for each block. With
+// t = score * log2(e) + log2(value scale of the key's block), m a running
+// reference near max t, p = 2^(t - m):
+//   out = sum_j p_j * code_j / l,   l = sum_j p_j / value_scale_j,
+// so the products take the codes alone (exact in f16), p needs no range
+// beyond its own maximum, and one multiply a block scales l.
+// Value scales below kKvLeastScale count as it (the writer's least one).
+constexpr float kKvLeastScale = 0x1p-87f;
+// p is kept at most 2^kTop when the reference is set and may grow to
+// 2^kGrowth before it is set again. f16 (largest 65504, steps of 2^-24) then
+// holds every p to within 2^-11 of itself or 2^-31 of the largest; with two
+// parts (f32 queries), which set it again sooner, to within 2^-22 or 2^-38.
+template <int kParts> constexpr float kTop = kParts == 2 ? 13.0f : 6.0f;
+template <int kParts> constexpr float kGrowth = kParts == 2 ? 15.0f : 14.0f;
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float nan_max(float a, float b) { // a NaN stays
+  return b > a || b != b ? b : a;
+}
+
+// The range of keys [lo, hi) that rows at positions p0 .. p1 can see.
+__device__ __forceinline__ void key_range(const KvAttendArgs &a, int length, int p0, int p1,
+                                          int &lo, int &hi) {
+  hi = a.causal ? min(length, p1 + 1) : length;
+  lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+  if (hi < lo)
+    hi = lo;
+}
+
+__device__ __forceinline__ bool sees(const KvAttendArgs &a, int length, int p, int key) {
+  return key < length && (!a.causal || key <= p) && (a.window <= 0 || key > p - a.window);
+}
+
+// Power-of-two factor 2^(141 - E) that brings a row whose largest magnitude
+// has biased exponent E to [2^14, 2^15), so that its f16 parts keep every
+// element to within 2^-39 of the largest, and the factor's inverse.
+__device__ __forceinline__ void row_factor(float amax, float &factor, float &inverse) {
+  const int e = min(max((__float_as_int(amax) >> 23) & 255, 15), 254);
+  factor = amax == 0.0f ? 1.0f : __int_as_float((268 - e) << 23);
+  inverse = amax == 0.0f ? 1.0f : __int_as_float((e - 14) << 23);
+}
+
+// Four int8 codes as two f16 pairs, exactly: code + 128 as the low byte of
+// 1024 + u, less 1152.
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  w ^= 0x80808080u;
+  const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), bias);
+  const __half2 y = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
+  lo = *reinterpret_cast<const uint32_t *>(&x);
+  hi = *reinterpret_cast<const uint32_t *>(&y);
+}
+
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ float2 unpack_half(uint32_t h) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&h));
+}
+
+} // namespace
+#endif
+
+} // namespace cim

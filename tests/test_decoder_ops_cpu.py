@@ -1,0 +1,142 @@
+"""Host-side checks of the decoder-block entry points, on CPU: descriptions
+that the C interface refuses before any launch (the pointers are never
+followed), and what the Python side refuses without a device."""
+
+import ctypes
+
+import pytest
+import torch
+
+from cim22_b200 import abi, cim_ops, native
+from cim22_b200.kv_cache import Int8KVCache
+
+HERE = 4096  # an address that is never read
+
+
+def cache(**kw):
+    d = dict(codes=HERE, scales=HERE, pages=4, kv_heads=2, block=16, head_dim=32)
+    return abi.KvCache(**{**d, **kw})
+
+
+def sequences(**kw):
+    d = dict(batch=2, table=HERE, table_stride=3, table_width=3, lengths=HERE, starts=HERE, rows=9,
+             most=9)
+    return abi.KvSequences(**{**d, **kw})
+
+
+def attention(**kw):
+    d = dict(type=abi.FLOAT32, q_heads=4, q=HERE, q_row_stride=128, q_head_stride=32, out=HERE,
+             lse=None, scale=1.0, causal=1, window=0, longest=48)
+    return abi.KvAttention(**{**d, **kw})
+
+
+CACHES = [dict(block=8), dict(block=24), dict(head_dim=8), dict(head_dim=40), dict(head_dim=144),
+          dict(kv_heads=0), dict(kv_heads=40000), dict(pages=-1), dict(pages=2 ** 31),
+          dict(codes=None), dict(scales=None), dict(codes=HERE + 8), dict(scales=HERE + 4)]
+SEQUENCES = [dict(batch=-1), dict(batch=65536), dict(lengths=None), dict(table=None),
+             dict(table_width=-1), dict(table_stride=2), dict(rows=-1), dict(most=-1),
+             dict(starts=None, rows=1)]
+ATTENTIONS = [dict(type=7), dict(q_heads=0), dict(q_heads=3), dict(window=-1), dict(longest=-1),
+              dict(q_row_stride=-1), dict(q_head_stride=-1), dict(scale=float("nan")),
+              dict(scale=float("inf")), dict(q=None), dict(out=None)]
+
+
+@pytest.mark.parametrize("c,s,a", [(c, {}, {}) for c in CACHES] + [({}, s, {}) for s in SEQUENCES]
+                         + [({}, {}, a) for a in ATTENTIONS])
+def test_attend_refuses(c, s, a):
+    lib = native.lib()
+    args = (ctypes.byref(cache(**c)), ctypes.byref(sequences(**s)), ctypes.byref(attention(**a)))
+    assert lib.cim22_cuda_kv_attend(*args, HERE, 1 << 40, HERE, None) != 0
+    assert native.last_error().startswith("cim22_cuda_kv_attend: ")
+
+
+@pytest.mark.parametrize("c,s", [(c, {}) for c in CACHES] + [({}, s) for s in SEQUENCES])
+def test_write_and_read_refuse(c, s):
+    lib = native.lib()
+    args = (ctypes.byref(cache(**c)), ctypes.byref(sequences(**s)))
+    assert lib.cim22_cuda_kv_write(*args, abi.FLOAT32, HERE, 64, 32, HERE, 64, 32, HERE, None) != 0
+    assert native.last_error().startswith("cim22_cuda_kv_write: ")
+    assert lib.cim22_cuda_kv_read(*args, abi.FLOAT32, HERE, HERE, HERE, None) != 0
+    assert native.last_error().startswith("cim22_cuda_kv_read: ")
+
+
+def test_null_and_unknown_arguments_are_refused():
+    lib = native.lib()
+    c, s, a = cache(), sequences(), attention()
+    assert lib.cim22_cuda_kv_attend(None, ctypes.byref(s), ctypes.byref(a), HERE, 64, HERE, None)
+    assert lib.cim22_cuda_kv_attend(ctypes.byref(c), None, ctypes.byref(a), HERE, 64, HERE, None)
+    assert lib.cim22_cuda_kv_attend(ctypes.byref(c), ctypes.byref(s), None, HERE, 64, HERE, None)
+    assert lib.cim22_cuda_kv_attend(ctypes.byref(c), ctypes.byref(s), ctypes.byref(a), HERE,
+                                    1 << 40, None, None)
+    for kind, k, row, status in ((7, HERE, 64, HERE), (0, None, 64, HERE), (0, HERE, -1, HERE),
+                                 (0, HERE, 64, None)):
+        assert lib.cim22_cuda_kv_write(ctypes.byref(c), ctypes.byref(s), kind, k, row, 32, HERE,
+                                       64, 32, status, None) != 0
+    assert lib.cim22_cuda_kv_read(ctypes.byref(c), ctypes.byref(s), 7, HERE, HERE, HERE, None)
+    assert lib.cim22_cuda_kv_read(ctypes.byref(c), ctypes.byref(s), 0, HERE, HERE, None, None)
+
+
+def test_workspace_too_small_is_refused():
+    lib = native.lib()
+    c = cache(pages=4096, block=64, head_dim=128)
+    s = sequences(batch=1, table_width=4096, starts=None, rows=1)
+    a = attention(longest=200000)
+    need = lib.cim22_cuda_kv_attend_workspace(ctypes.byref(c), ctypes.byref(s), ctypes.byref(a))
+    assert need > 0
+    for ws, size in ((HERE, need - 1), (None, need), (HERE + 4, need)):
+        assert lib.cim22_cuda_kv_attend(ctypes.byref(c), ctypes.byref(s), ctypes.byref(a), ws,
+                                        size, HERE, None) != 0
+        assert "workspace" in native.last_error()
+
+
+def block_norm(post=None, pre=None, **kw):
+    d = dict(type=abi.FLOAT32, rows=4, dim=32, x=HERE, x_stride=32, residual=HERE,
+             residual_stride=32, residual_scale=1.0, gate=HERE, gate_stride=32, gate_rows=0,
+             gate_columns=32, gate_type=abi.FLOAT32, gate_activation=0, h=HERE, h_stride=32,
+             y=HERE, y_stride=32)
+    call = abi.BlockNorm(**{**d, **kw})
+    if post:
+        call.post = ctypes.pointer(post)
+    if pre:
+        call.pre = ctypes.pointer(pre)
+    return call
+
+
+@pytest.mark.parametrize("call", [
+    dict(type=5), dict(rows=-1), dict(rows=2 ** 31), dict(dim=0), dict(dim=16385), dict(x=None),
+    dict(h=None, y=None), dict(x_stride=31), dict(residual_stride=31), dict(h_stride=31),
+    dict(y_stride=31), dict(gate_type=abi.BFLOAT16), dict(gate_columns=2), dict(gate_rows=-1),
+    dict(gate_activation=3), dict(post=abi.Norm(kind=3)), dict(pre=abi.Norm(kind=0)),
+    dict(pre=abi.Norm(kind=1, eps=-1.0)), dict(pre=abi.Norm(kind=1, eps=float("nan"))),
+    dict(post=abi.Norm(kind=1, type=abi.FLOAT16))])
+def test_block_norm_refuses(call):
+    assert native.lib().cim22_cuda_block_norm(ctypes.byref(block_norm(**call)), None) != 0
+    assert native.last_error().startswith("cim22_cuda_block_norm: ")
+    assert native.lib().cim22_cuda_block_norm(None, None) != 0
+
+
+def test_empty_calls_do_nothing():
+    lib = native.lib()
+    assert lib.cim22_cuda_block_norm(ctypes.byref(block_norm(rows=0)), None) == 0
+    c, a = ctypes.byref(cache()), ctypes.byref(attention())
+    for kw in (dict(rows=0), dict(batch=0, rows=0)):
+        s = ctypes.byref(sequences(**kw))
+        assert lib.cim22_cuda_kv_attend(c, s, a, None, 0, HERE, None) == 0
+        assert lib.cim22_cuda_kv_write(c, s, 0, HERE, 64, 32, HERE, 64, 32, HERE, None) == 0
+        assert lib.cim22_cuda_kv_read(c, s, 0, HERE, HERE, HERE, None) == 0
+
+
+def test_cpu_tensors_and_shapes_are_refused():
+    x = torch.zeros(4, 8)
+    with pytest.raises(TypeError, match="CUDA"):
+        cim_ops.block_norm(x, pre=cim_ops.Norm("rms"))
+    with pytest.raises(TypeError, match="CUDA"):
+        Int8KVCache.over(torch.zeros(2, 1, 2, 16, 16, dtype=torch.int8), torch.zeros(2, 1, 2))
+    for shape in ((2, 1, 24, 16), (2, 1, 144, 16), (2, 0, 16, 16), (2, 1, 16, 48), (-1, 1, 16, 16)):
+        with pytest.raises(ValueError):
+            Int8KVCache(*shape)
+
+
+def test_status_messages():
+    assert native.status_message(0x400) == "key/value cache page, length or start out of range"
+    assert native.status_message(0x800) == "key/value cache does not support NaN or infinity"

@@ -1,0 +1,515 @@
+"""The 8-bit key/value cache and attention over it against their definitions in
+64 bits (tests/decoder_reference.py)."""
+
+import math
+
+import pytest
+import torch
+
+import decoder_reference as ref
+from cim22_b200.cim_ops import CimLayer, Norm, StatusWord, Workspace, block_norm
+from cim22_b200.kv_cache import Int8KVCache
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+class Setup:
+    """A device cache and its host twin, with a shuffled page table."""
+
+    def __init__(self, lengths, heads, dim, block, seed=0, spare=2, width=None):
+        self.g = torch.Generator().manual_seed(seed)
+        self.block, self.heads, self.dim = block, heads, dim
+        used = [(n + block - 1) // block for n in lengths]
+        total = sum(used) + spare
+        order = torch.randperm(total, generator=self.g)
+        self.table = torch.full((len(lengths), width or max(1, max(used))), -1,
+                                dtype=torch.int32)
+        at = 0
+        for b, u in enumerate(used):
+            self.table[b, :u] = order[at:at + u]
+            at += u
+        self.cache = Int8KVCache(total, heads, dim, block)
+        self.host = ref.Cache(total, heads, dim, block)
+        # What a page held before it was given to a sequence must not matter.
+        self.cache.codes.fill_(93)
+        self.cache.scales.fill_(1e30)
+        self.lengths = list(lengths)
+        self.status = StatusWord(torch.device("cuda", 0))
+
+    def rows(self, n, heads, dtype, scale=1.0):
+        return (torch.randn(n, heads, self.dim, generator=self.g) * scale).to(dtype)
+
+    def device(self, lengths, starts=None):
+        return (self.table.cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+                None if starts is None else torch.tensor(starts, dtype=torch.int32,
+                                                         device="cuda"))
+
+    def write(self, new, lengths, dtype=torch.float32, scale=1.0, **kw):
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        k, v = (self.rows(starts[-1], self.heads, dtype, scale) for _ in range(2))
+        self.host.write(k, v, self.table, lengths, starts)
+        table, at, first = self.device(lengths, starts)
+        self.cache.write(k.cuda(), v.cuda(), table, at, first, status=self.status, **kw)
+        return k, v
+
+    def fill(self, dtype=torch.float32, scale=1.0):
+        """Writes every sequence whole."""
+        self.write(self.lengths, self.lengths, dtype, scale)
+
+    def check_read(self, dtype=torch.float32):
+        starts = [0]
+        for n in self.lengths:
+            starts.append(starts[-1] + n)
+        table, at, first = self.device(self.lengths, starts)
+        got = self.cache.read(table, at, first, tokens=starts[-1], dtype=dtype,
+                              status=self.status)
+        self.status.raise_if_set()
+        for side in range(2):
+            want = torch.cat([self.host.values(self.table[b], n, side)
+                              for b, n in enumerate(self.lengths)])
+            # Codes and scales are defined to the bit, and so are values.
+            assert torch.equal(got[side].cpu(), want.float().to(dtype))
+
+    def check_attend(self, new, dtype, causal=True, window=0, group=2, scale=None, starts="rows",
+                     q=None, **kw):
+        heads = self.heads * group
+        total = sum(new)
+        q = self.rows(total, heads, dtype) if q is None else q
+        first = [0]
+        for n in new:
+            first.append(first[-1] + n)
+        table, at, dev_starts = self.device(self.lengths, first if starts == "rows" else None)
+        out, lse = self.cache.attend(q.cuda(), table, at, dev_starts, causal=causal,
+                                     window=window, scale=scale, return_lse=True,
+                                     status=self.status, **kw)
+        self.status.raise_if_set()
+        parts = 2 if dtype == torch.float32 else 1
+        step = 2.0 ** -22  # one product or sum of the tensor cores, truncation allowed for
+        # A probability is off by half a step of f16 (one part) or of its two
+        # parts' 22 bits; weights and their sum both carry it.
+        p_err = torch.finfo(torch.float16).eps / 2 if parts == 1 else step
+        # Far below the largest, a probability (times its block's value scale)
+        # is off by half a step of f16's subnormals, 2^-25, where the largest is
+        # at least 2^6 (one part) or 2^13; it multiplies a code of at most 127.
+        floor = 127 * 2.0 ** (-31 if parts == 1 else -38)
+        for b, n in enumerate(new):
+            keys = self.lengths[b]
+            k, v = (self.host.values(self.table[b], keys, side) for side in range(2))
+            s = self.dim ** -0.5 if scale is None else scale
+            want, want_lse, size, reach, peak = ref.attend(
+                q[first[b]:first[b + 1]], k, v, keys - n, s, causal, window,
+                self.host.value_scales(self.table[b], keys))
+            got = out[first[b]:first[b + 1]].double().cpu()
+            got_lse = lse[first[b]:first[b + 1]].double().cpu()
+            # Score error: the contraction's steps, the queries' parts and the
+            # exponent's own rounding (arguments below 128).
+            delta = (parts * (self.dim / 16) + 6) * step * reach + 130 * 2.0 ** -24
+            steps = (keys / 16 + 70) * step
+            tol = torch.finfo(dtype).eps / 2 * want.abs() + size * (
+                2 * p_err + 2 * delta + steps)[..., None] + floor * peak[..., None]
+            if dtype == torch.float16:
+                tol = tol + 2.0 ** -25
+            off = (got - want).abs()
+            assert bool((off <= tol).all()), (b, float((off / tol.clamp(min=1e-300)).max()))
+            seen = torch.isfinite(want_lse)
+            assert torch.equal(seen, torch.isfinite(got_lse))
+            assert bool((got_lse[~seen] == -math.inf).all())
+            lse_tol = delta + steps + 2.0 ** -23 * want_lse.abs()
+            assert bool(((got_lse - want_lse).abs() <= lse_tol)[seen].all())
+        return out
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("block,dim,heads", [(16, 16, 1), (32, 80, 3), (64, 128, 2), (128, 48, 2)])
+def test_write_and_read_back(dtype, block, dim, heads):
+    s = Setup([1, block - 1, block, block + 1, 3 * block + 5, 0, 2], heads, dim, block)
+    s.fill(dtype)
+    s.check_read(dtype)
+    s.check_read()
+
+
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_token_by_token_equals_the_definition(block, dtype):
+    """Scales grow and earlier codes are rounded again as tokens arrive."""
+    s = Setup([block + 3, 0, 2 * block], 2, 32, block)
+    for t in range(2 * block):
+        lengths = [min(t + 1, s.lengths[0]), 0, t + 1]
+        new = [1 if t < s.lengths[0] else 0, 0, 1]
+        s.write(new, lengths, dtype, scale=1.0 + t % 7)
+    s.check_read()
+
+
+def test_decode_rows_without_starts_and_an_empty_slot():
+    s = Setup([5, 0, 40], 1, 16, 16)
+    s.write([4, 0, 39], [4, 0, 39])
+    k, v = s.rows(3, 1, torch.float32), s.rows(3, 1, torch.float32)
+    s.host.write(k, v, s.table, s.lengths, [0, 1, 2, 3])
+    table, at, _ = s.device(s.lengths)
+    before = s.cache.codes.clone()
+    s.cache.write(k.cuda(), v.cuda(), table, at, status=s.status)
+    changed = (s.cache.codes != before).flatten(1).any(1).nonzero().flatten().tolist()
+    assert set(changed) <= {int(s.table[0, 0]), int(s.table[2, 2])}
+    s.check_read()
+
+
+def test_chunked_prompt_writes_join():
+    s = Setup([150, 70], 2, 64, 32)
+    s.write([40, 70], [40, 70], torch.bfloat16)
+    s.write([61, 0], [101, 70], torch.bfloat16)
+    s.write([49, 0], [150, 70], torch.bfloat16)
+    s.check_read(torch.bfloat16)
+
+
+def test_values_of_all_sizes_and_not_finite():
+    s = Setup([64], 1, 16, 16)
+    k = torch.zeros(64, 1, 16)
+    k[0:16] = torch.linspace(-3e38, 3e38, 256).view(16, 1, 16)  # the largest
+    k[16:32] = torch.linspace(-1e-38, 1e-38, 256).view(16, 1, 16)  # below the floor
+    k[40, 0, 3], k[41, 0, 4], k[42, 0, 5], k[43] = math.nan, math.inf, -math.inf, 2.5
+    v = torch.zeros(64, 1, 16)  # all zero: codes zero
+    s.host.write(k, v, s.table, [64], [0, 64])
+    table, at, first = s.device([64], [0, 64])
+    s.cache.write(k.cuda(), v.cuda(), table, at, first, status=s.status)
+    with pytest.raises(RuntimeError, match="does not support NaN or infinity"):
+        s.status.raise_if_set()
+    s.status.reset()
+    s.check_read()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_a_fused_projection(dtype):
+    """Strided views, rows off a 16-byte boundary too."""
+    s = Setup([37, 20], 2, 32, 16)
+    for base, pad in ((0, 0), (3, 1)):
+        flat = torch.randn(57 * (6 * 32 + pad) + 8, generator=s.g).to(dtype)
+        fused = flat.as_strided((57, 6, 32), (6 * 32 + pad, 32, 1), base)
+        k, v = fused[:, 2:4], fused[:, 4:6]
+        s.host.write(k, v, s.table, s.lengths, [0, 37, 57])
+        dev = flat.cuda().as_strided((57, 6, 32), (6 * 32 + pad, 32, 1), base)
+        table, at, first = s.device(s.lengths, [0, 37, 57])
+        s.cache.write(dev[:, 2:4], dev[:, 4:6], table, at, first, status=s.status)
+        s.check_read(dtype)
+        want = s.cache.attend(dev[:, 0:2].contiguous(), table, at, first, status=s.status)
+        got = s.cache.attend(dev[:, 0:2], table, at, first, status=s.status)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,block", [(16, 16), (64, 32), (80, 16), (128, 64), (112, 128)])
+def test_decode(dtype, dim, block):
+    s = Setup([1, 2, 15, 16, 17, 0, 63, 64, 200], 2, dim, block)
+    s.fill()
+    s.check_attend([1] * 9, dtype, group=4, starts=None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [1, 3, 8])
+def test_chunks_and_prompts(dtype, group):
+    s = Setup([5, 33, 130, 260, 0], 1, 64, 32)
+    s.fill()
+    s.check_attend([5, 2, 130, 17, 0], dtype, group=group)
+    s.check_attend([1, 33, 64, 129, 0], dtype, group=group)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [1, 5, 16, 100])
+def test_windows(causal, window):
+    s = Setup([7, 90, 300], 1, 128, 16)
+    s.fill()
+    s.check_attend([7, 30, 140], torch.bfloat16, causal=causal, window=window)
+    s.check_attend([1, 1, 1], torch.float32, causal=causal, window=window, starts=None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_queries_than_tokens_leaves_empty_rows(dtype):
+    s = Setup([3, 0, 20], 2, 32, 16)
+    s.fill()
+    out = s.check_attend([5, 4, 20], dtype)
+    assert bool((out[:2] == 0).all()) and bool((out[5:9] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_axis_is_split_and_joined(dtype):
+    s = Setup([3000], 1, 64, 64)
+    s.fill()
+    s.check_attend([1], dtype, group=2, starts=None)
+    s.check_attend([1], dtype, group=2, starts=None, longest=64)
+    s.check_attend([1], dtype, group=2, starts=None, window=700)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scales_that_differ_by_blocks(dtype):
+    """Value scales 1e-6 to 1e6 and key scales apart: probabilities carry the
+    value scale in their exponent."""
+    s = Setup([128], 1, 32, 16)
+    k = s.rows(128, 1, torch.float32)
+    v = s.rows(128, 1, torch.float32)
+    for i in range(8):
+        v[16 * i:16 * i + 16] *= 10.0 ** (3 - i if i % 2 else i - 6)
+        k[16 * i:16 * i + 16] *= 2.0 ** (i - 4)
+    s.host.write(k, v, s.table, [128], [0, 128])
+    table, at, first = s.device([128], [0, 128])
+    s.cache.write(k.cuda(), v.cuda(), table, at, first, status=s.status)
+    s.check_attend([128], dtype, group=1)
+    s.check_attend([1], dtype, group=1, starts=None)
+    s.check_attend([3], dtype, group=1, scale=-0.3)
+    s.check_attend([3], dtype, group=1, scale=0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_queries_of_all_sizes(dtype):
+    s = Setup([40], 1, 48, 16)
+    s.fill()
+    q = s.rows(40, 2, dtype)
+    q[0] = 0
+    q[1] *= 1e-6
+    q[2] *= 100
+    q[3, 0, 0] = 300
+    s.check_attend([40], dtype, q=q)
+
+
+def test_not_finite_queries_stay_in_their_rows():
+    s = Setup([40], 1, 32, 16)
+    s.fill()
+    q = s.rows(20, 2, torch.float32)
+    clean = q.clone()
+    q[3, 0, 5], q[7, 1, 0] = math.nan, math.inf
+    table, at, first = s.device([40], [0, 20])
+    got = s.cache.attend(q.cuda(), table, at, first, status=s.status)
+    want = s.cache.attend(clean.cuda(), table, at, first, status=s.status)
+    assert bool(torch.isnan(got[3, 0]).all()) and bool(torch.isnan(got[7, 1]).all())
+    keep = torch.ones(20, 2, dtype=torch.bool)
+    keep[3, 0] = keep[7, 1] = False
+    assert torch.equal(got.cpu()[keep], want.cpu()[keep])
+
+
+def test_rows_behind_the_last_sequence_are_left():
+    s = Setup([20, 9], 1, 16, 16)
+    s.fill()
+    q = s.rows(15, 2, torch.float32).cuda()
+    table, at, first = s.device(s.lengths, [0, 6, 9])
+    out = torch.full((15, 2, 16), 5.0, device="cuda")
+    s.cache.attend(q, table, at, first, out=out, status=s.status)
+    assert bool((out[9:] == 5).all()) and not bool((out[:9] == 5).any())
+    k = torch.full((15, 1, 16), 5.0, device="cuda")
+    v = k.clone()
+    s.cache.read(table, at, first, out=(k, v), status=s.status)
+    assert bool((k[9:] == 5).all()) and bool((v[9:] == 5).all())
+    s.status.raise_if_set()
+
+
+def bad_descriptions(s):
+    table, at, first = s.device(s.lengths, [0, 6, 9])
+    high = table.clone()
+    high[0, 0] = s.cache.pages
+    low = table.clone()
+    low[0, 0] = -5
+    long = at.clone()
+    long[0] = 16 * table.shape[1] + 1
+    negative = at.clone()
+    negative[0] = -1
+    back = first.clone()
+    back[1] = -3
+    past = first.clone()
+    past[2] = 10
+    return {"page past the cache": (high, at, first), "negative page": (low, at, first),
+            "length past the table": (table, long, first), "negative length": (table, negative, first),
+            "starts run backwards": (table, at, back), "starts past the rows": (table, at, past)}
+
+
+@pytest.mark.parametrize("which", ["page past the cache", "negative page", "length past the table",
+                                   "negative length", "starts run backwards",
+                                   "starts past the rows"])
+def test_bad_descriptions_are_reported_not_followed(which):
+    s = Setup([12, 9], 1, 16, 16)
+    s.fill()
+    s.status.raise_if_set()
+    table, at, first = bad_descriptions(s)[which]
+    q = s.rows(9, 2, torch.float32).cuda()
+    k = s.rows(9, 1, torch.float32).cuda()
+    calls = [lambda: s.cache.attend(q, table, at, first, status=s.status),
+             lambda: s.cache.read(table, at, first, tokens=9, status=s.status),
+             lambda: s.cache.write(k, k, table, at, first, status=s.status)]
+    for call in calls:
+        s.status.reset()
+        call()
+        with pytest.raises(RuntimeError, match="page, length or start out of range"):
+            s.status.raise_if_set()
+    # More rows in a sequence than the host said.
+    table, at, first = s.device(s.lengths, [0, 6, 9])
+    s.status.reset()
+    s.cache.attend(q, table, at, first, most=5, status=s.status)
+    with pytest.raises(RuntimeError, match="page, length or start out of range"):
+        s.status.raise_if_set()
+
+
+def test_offsets_past_32_bits():
+    """A cache of more than 2^31 codes: its last pages."""
+    block, heads, dim = 128, 8, 128
+    pages = 2 ** 31 // (heads * 2 * block * dim) + 3
+    cache = Int8KVCache(pages, heads, dim, block)
+    table = torch.tensor([[pages - 1, 0], [pages - 2, 1]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([200, 130], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 200, 330], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(330, heads, dim, generator=g, device="cuda") for _ in range(2))
+    cache.write(k, v, table, lengths, starts)
+    got = cache.read(table, lengths, starts, tokens=330)
+    small = Int8KVCache(4, heads, dim, block)
+    near = torch.tensor([[3, 0], [2, 1]], dtype=torch.int32, device="cuda")
+    small.write(k, v, near, lengths, starts)
+    want = small.read(near, lengths, starts, tokens=330)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q = torch.randn(330, 16, dim, generator=g, device="cuda")
+    assert torch.equal(cache.attend(q, table, lengths, starts),
+                       small.attend(q, near, lengths, starts))
+
+
+def test_captured_step_takes_new_contents():
+    """Write and attention of a decoding step in one graph, replayed as the
+    sequences grow; two graphs with one workspace, one after the other."""
+    s = Setup([600, 300], 2, 64, 32, width=30)
+    s.lengths = [600, 300]
+    s.fill()
+    table, at, _ = s.device(s.lengths)
+    workspace = Workspace(torch.device("cuda", 0))
+    q = torch.zeros(2, 4, 64, device="cuda")
+    kv = torch.zeros(2, 4, 64, device="cuda")
+
+    def step():
+        s.cache.write(kv[:, :2], kv[:, 2:], table, at, status=s.status)
+        return s.cache.attend(q, table, at, workspace=workspace, status=s.status)
+
+    # New tokens go to pages of their own: the table has room for 30 pages a row.
+    spare = Int8KVCache(s.cache.pages + 40, 2, 64, 32)
+    spare.codes[:s.cache.pages] = s.cache.codes
+    spare.scales[:s.cache.pages] = s.cache.scales
+    old = s.cache.pages
+    s.cache = spare
+    for b, used in enumerate((19, 10)):
+        for i in range(used, 30):
+            table[b, i] = old + 11 * b + i - used
+    at += 1
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for i in range(40):
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+        kv.copy_(torch.randn(kv.shape, generator=g, device="cuda"))
+        at += 1
+        graph, out = graphs[i % 2]
+        graph.replay()
+        want = s.cache.attend(q, table, at, status=s.status)
+        assert torch.equal(out, want)
+    s.status.raise_if_set()
+
+
+def test_results_repeat_and_do_not_hang_on_streams():
+    s = Setup([900, 40, 300], 2, 128, 64)
+    s.fill()
+    q = s.rows(1240, 8, torch.bfloat16).cuda()
+    table, at, first = s.device(s.lengths, [0, 900, 940, 1240])
+    want = s.cache.attend(q, table, at, first, status=s.status)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for st in streams:
+        with torch.cuda.stream(st):
+            outs.append(s.cache.attend(q, table, at, first, status=s.status))
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@pytest.mark.parametrize("call", [
+    lambda s, q, k, t, n, st: s.cache.attend(q.double(), t, n, st),
+    lambda s, q, k, t, n, st: s.cache.attend(q[..., :8], t, n, st),
+    lambda s, q, k, t, n, st: s.cache.attend(q[:, :1].repeat(1, 3, 1), t, n, st),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st, window=-1),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st, scale=math.inf),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st, longest=-1),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st, most=-1),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t.long(), n, st),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t.t(), n, st),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n.cpu(), st),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st[:2]),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st, out=q.half()),
+    lambda s, q, k, t, n, st: s.cache.attend(q.cpu(), t, n, st),
+    lambda s, q, k, t, n, st: s.cache.write(k, k.half(), t, n, st),
+    lambda s, q, k, t, n, st: s.cache.write(k, k[:8], t, n, st),
+    lambda s, q, k, t, n, st: s.cache.write(q, q, t, n, st),
+    lambda s, q, k, t, n, st: s.cache.read(t, n, st),
+    lambda s, q, k, t, n, st: s.cache.read(t, n, st, tokens=9, dtype=torch.int8),
+    lambda s, q, k, t, n, st: Int8KVCache(4, 2, 24),
+    lambda s, q, k, t, n, st: Int8KVCache(4, 2, 144),
+    lambda s, q, k, t, n, st: Int8KVCache(4, 2, 64, 48),
+    lambda s, q, k, t, n, st: Int8KVCache(4, 0, 64),
+    lambda s, q, k, t, n, st: Int8KVCache.over(s.cache.codes[:, :, :1], s.cache.scales),
+    lambda s, q, k, t, n, st: Int8KVCache.over(s.cache.codes.float(), s.cache.scales),
+    lambda s, q, k, t, n, st: Int8KVCache.over(s.cache.codes, s.cache.scales.half()),
+    lambda s, q, k, t, n, st: Int8KVCache.over(s.cache.codes, s.cache.scales[:1]),
+])
+def test_refusals(call):
+    s = Setup([20, 9], 2, 16, 16)
+    q, k = s.rows(9, 4, torch.float32).cuda(), s.rows(9, 2, torch.float32).cuda()
+    table, at, first = s.device(s.lengths, [0, 6, 9])
+    with pytest.raises((TypeError, ValueError)):
+        call(s, q, k, table, at, first)
+
+
+def test_a_decoder_block_of_cim_layers():
+    """Norm, CIM projections, cache, attention and the gated residual as one
+    block, prompt then single tokens, against the same block in 64 bits around
+    the same CIM layers."""
+    dev = torch.device("cuda", 0)
+    g = torch.Generator().manual_seed(0)
+    width, heads, kv_heads, dim, block = 96, 4, 2, 32, 16
+    wq = (torch.randn((heads + 2 * kv_heads) * dim, width, generator=g) * 0.1).numpy()
+    wo = (torch.randn(width, heads * dim, generator=g) * 0.1).numpy()
+    qkv_layer, out_layer = CimLayer(wq, device=dev), CimLayer(wo, device=dev)
+    pre, post = (Norm("rms", 1 + 0.1 * torch.randn(width, generator=g).to(dev)) for _ in range(2))
+    gate = torch.randn(width, generator=g).to(dev)
+    cache, host = Int8KVCache(8, kv_heads, dim, block), ref.Cache(8, kv_heads, dim, block)
+    table = torch.arange(8, dtype=torch.int32).view(2, 4).to(dev)
+    status, workspace = StatusWord(dev), Workspace(dev)
+    lengths = [0, 0]
+    for new in ([21, 9], [1, 1], [1, 1], [4, 2]):
+        total = sum(new)
+        starts = [0, new[0], total]
+        lengths = [n + a for n, a in zip(lengths, new)]
+        x = torch.randn(total, width, generator=g).to(dev)
+        at = torch.tensor(lengths, dtype=torch.int32, device=dev)
+        first = torch.tensor(starts, dtype=torch.int32, device=dev)
+        _, y = block_norm(x, pre=pre)
+        qkv = qkv_layer.linear_bf16(y, status=status).view(total, -1, dim)
+        q, k, v = qkv.split([heads, kv_heads, kv_heads], dim=1)
+        cache.write(k, v, table, at, first, status=status)
+        o = cache.attend(q, table, at, first, workspace=workspace, status=status)
+        f = out_layer.linear_bf16(o.view(total, -1), status=status)
+        h, y2 = block_norm(f, x, post=post, pre=pre, gate=gate, gate_activation="sigmoid")
+        status.raise_if_set()
+
+        # Each stage against 64 bits on its own inputs: the f32 stages differ
+        # from it by roundings of 2^-24 of their terms (at most a few hundred).
+        near = dict(rtol=2.0 ** -16, atol=2.0 ** -16)
+        assert torch.allclose(y.double(), ref.norm(x.double(), "rms", pre.weight), **near)
+        host.write(k.cpu(), v.cpu(), table.cpu(), lengths, starts)
+        for b in range(2):
+            held = [host.values(table.cpu()[b], lengths[b], side) for side in range(2)]
+            want = ref.attend(q[starts[b]:starts[b + 1]].cpu(), *held, lengths[b] - new[b],
+                              dim ** -0.5, True, 0)[0]
+            assert torch.allclose(o[starts[b]:starts[b + 1]].cpu().double(), want, **near)
+        stream = x.double() + torch.sigmoid(gate.double()) * ref.norm(f.double(), "rms", post.weight)
+        assert torch.allclose(h.double(), stream, **near)
+        assert torch.allclose(y2.double(), ref.norm(stream, "rms", pre.weight), **near)
