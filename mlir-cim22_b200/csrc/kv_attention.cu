@@ -22,7 +22,6 @@
 #include <algorithm>
 
 namespace cim {
-
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 6;
@@ -497,17 +496,32 @@ int decode_splits(const KvView &v, int64_t tiles, int64_t longest) {
 }
 
 struct Plan {
+  bool prompt; // by the tensor-memory kernel
+  bool share;  // with one query tile a CTA
   int splits;
   int64_t tiles;
   size_t bytes; // of the partial results
 };
 
-Plan decode_plan(const KvView &v, const cim22_kv_attention &t) {
+// Up to kDecodeRows query rows a sequence and kv head go to the decode kernel.
+constexpr int64_t kDecodeRows = 32;
+
+Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   Plan p;
   const int64_t group = t.q_heads / v.heads;
-  p.tiles = (std::min<int64_t>(v.most, v.rows) * group + 15) / 16;
+  const int64_t rows = std::min<int64_t>(v.most, v.rows) * group;
   const int64_t held = static_cast<int64_t>(v.table_width) << v.block_log2;
-  p.splits = decode_splits(v, p.tiles, std::max<int64_t>(1, std::min(t.longest, held)));
+  const int64_t longest = std::max<int64_t>(1, std::min(t.longest, held));
+  p.prompt = rows > kDecodeRows;
+  p.share = p.prompt && (t.type == CIM22_FLOAT32 || rows <= 128);
+  if (!p.prompt) {
+    p.tiles = (rows + 15) / 16;
+    p.splits = decode_splits(v, p.tiles, longest);
+  } else {
+    p.tiles = (rows + (p.share ? 127 : 255)) / (p.share ? 128 : 256);
+    const int64_t items = p.tiles * v.heads * v.batch;
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min({148 / std::max<int64_t>(1, items), (longest + 1023) / 1024, int64_t{64}})));
+  }
   p.bytes = p.splits == 1 ? 0
                           : static_cast<size_t>(p.splits) * v.rows * t.q_heads *
                                 (static_cast<size_t>(v.dim) * 4 + 16);
@@ -548,9 +562,10 @@ cudaError_t launch_decode(const KvAttendArgs &a, int64_t tiles, cudaStream_t str
 }
 
 template <typename T, int kParts>
-cudaError_t launch_attend(const KvAttendArgs &a, int64_t tiles, cudaStream_t stream) {
-  cudaError_t e = a.v.dim > 64 ? launch_decode<T, 2, kParts>(a, tiles, stream)
-                               : launch_decode<T, 1, kParts>(a, tiles, stream);
+cudaError_t launch_attend(const KvAttendArgs &a, int type, const Plan &plan, cudaStream_t stream) {
+  cudaError_t e = plan.prompt ? kv_prompt_launch(a, type, plan.share, static_cast<int>(plan.tiles), stream)
+                  : a.v.dim > 64 ? launch_decode<T, 2, kParts>(a, plan.tiles, stream)
+                                 : launch_decode<T, 1, kParts>(a, plan.tiles, stream);
   if (e == cudaSuccess && a.splits > 1) {
     const int64_t rows = std::min<int64_t>(a.v.most, a.v.rows) * a.q_heads;
     e = launch_pdl(kv_join_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4), 1, a.v.batch),
@@ -573,7 +588,7 @@ size_t cim22_cuda_kv_attend_workspace(const cim22_kv_cache *cache,
   if (!kv_view("cim22_cuda_kv_attend_workspace", cache, sequences, v) ||
       !attend_args("cim22_cuda_kv_attend_workspace", v, attention))
     return 0;
-  return decode_plan(v, *attention).bytes;
+  return attend_plan(v, *attention).bytes;
 }
 
 int cim22_cuda_kv_attend(const cim22_kv_cache *cache, const cim22_kv_sequences *sequences,
@@ -590,7 +605,7 @@ int cim22_cuda_kv_attend(const cim22_kv_cache *cache, const cim22_kv_sequences *
   }
   if (v.batch == 0 || v.rows == 0)
     return 0;
-  const Plan plan = decode_plan(v, *attention);
+  const Plan plan = attend_plan(v, *attention);
   if (plan.bytes > workspace_bytes || (plan.bytes && !workspace) ||
       (reinterpret_cast<uintptr_t>(workspace) & 15)) {
     set_last_error("cim22_cuda_kv_attend: workspace too small or not 16-byte aligned");
@@ -619,9 +634,9 @@ int cim22_cuda_kv_attend(const cim22_kv_cache *cache, const cim22_kv_sequences *
   a.status = status;
   const auto s = static_cast<cudaStream_t>(stream);
   const cudaError_t e =
-      attention->type == CIM22_FLOAT32    ? launch_attend<float, 2>(a, plan.tiles, s)
-      : attention->type == CIM22_BFLOAT16 ? launch_attend<__nv_bfloat16, 1>(a, plan.tiles, s)
-                                          : launch_attend<__half, 1>(a, plan.tiles, s);
+      attention->type == CIM22_FLOAT32    ? launch_attend<float, 2>(a, attention->type, plan, s)
+      : attention->type == CIM22_BFLOAT16 ? launch_attend<__nv_bfloat16, 1>(a, attention->type, plan, s)
+                                          : launch_attend<__half, 1>(a, attention->type, plan, s);
   return cuda_ok(e, "kv_attend") ? 0 : bad;
 }
 

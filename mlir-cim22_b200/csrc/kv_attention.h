@@ -21,6 +21,10 @@ struct KvAttendArgs {
   int32_t *status;
 };
 
+// The tensor-memory kernel for prompts (kv_attention_tc.cu).
+cudaError_t kv_prompt_launch(const KvAttendArgs &a, int type, bool share, int tiles,
+                             cudaStream_t stream);
+
 // Allows a kernel its dynamic shared memory, once for each device.
 class DynamicSmem {
 public:

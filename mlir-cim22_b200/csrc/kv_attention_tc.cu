@@ -1,0 +1,725 @@
+// kv_attention_tc.cu - attention of prompts and chunks over the 8-bit cache on
+// the tensor cores (tcgen05, operands and accumulators in TMEM).
+//
+// Bound by the tensor cores and, about as much, by the exponentials: a 128 x
+// 128 tile of scores takes 2 x 512 cycles of f16 products (head_dim 128) and
+// 1,024 of the special-function units. A CTA therefore runs two streams of
+// 128 query rows, so that one's products cover the other's softmax:
+//   warps 0-3, 4-7  softmax of stream 0 and 1: a thread a row, scores from
+//                   TMEM, probabilities back over them as the f16 A operand
+//   warps 8-11      converters: 128-token tiles of keys and values, int8 codes
+//                   (16 bytes a load, exact in f16) into 128-byte-swizzled
+//                   shared-memory tiles, alternately into a ring of four
+//   warp 12         issues the products: S = Q K^T, then O += P V
+// Query rows are the tokens of a sequence times the heads that share a kv
+// head, so a tile of keys is converted once for up to 256 rows. The codes'
+// scales stay out of the products: a group of 16 tokens lies in one page, and
+// its key scale multiplies the scores, its value scale goes into the exponent
+// (kv_attention.h).
+// kShare: both streams take the same 128 rows and alternate tiles of keys, and
+// their results are joined at the end. It serves few rows, and f32 queries,
+// whose rows are two f16 parts and need the second tile's shared memory.
+#include "kv_attention.h"
+
+#include <algorithm>
+
+namespace cim {
+namespace {
+
+constexpr int kThreads = 512, kTile = 128;
+constexpr int kPanel = kTile * 128; // bytes: 128 rows of 64 f16
+constexpr uint64_t kWaitLimit = 2000000000ull; // ns
+
+template <int kCh> struct alignas(1024) PromptSmem {
+  uint8_t q[2][kCh * kPanel];    // query tiles, or the two parts of one
+  uint8_t kv[4][kCh * kPanel];   // keys of tile j at 2 (j % 2), values after
+  float4 scale[4][8];            // of tile j % 4: key scale, log2 and inverse of the value scale
+  float coef[2 * kTile];         // what turns a row's product into an exponent
+  float join[3][kTile];
+  uint64_t kv_full[4], kv_empty[4], scale_full[4];
+  uint64_t s_full[2], p_full[2], o_full[2], done;
+  uint32_t tmem;
+  int failed;
+};
+
+__device__ __forceinline__ uint32_t smem_at(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ void bar_init(uint64_t *bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_at(bar)), "r"(count));
+}
+
+__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(bar)) : "memory");
+}
+
+// Waits for the phase of the given parity, for at most kWaitLimit of the
+// global timer; gives up sooner when another role has.
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *failed) {
+  const uint32_t at = smem_at(bar);
+  uint64_t start = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+                 " selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done)
+                 : "r"(at), "r"(parity)
+                 : "memory");
+    if (done)
+      return true;
+    if ((i & 31) == 0) {
+      uint64_t now;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+      if (start == 0)
+        start = now;
+      if (now - start > kWaitLimit || *reinterpret_cast<volatile int *>(failed)) {
+        *reinterpret_cast<volatile int *>(failed) = 1;
+        return false;
+      }
+    }
+  }
+}
+
+// Matrix descriptors, 128-byte swizzle. K-major (queries, keys): rows of 128
+// bytes in 1024-byte atoms. MN-major (values): a row holds 64 elements of one
+// token; 64-element panels kPanel apart, 8-token atoms 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t at) {
+  return ((at & 0x3ffffull) >> 4) | (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 46) |
+         (uint64_t{2} << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t at) {
+  return desc_k_major(at) | (uint64_t{kPanel >> 4} << 16);
+}
+
+// kind::f16 with f16 A and B and f32 accumulators (format 1 at bit 4); B is
+// MN-major with bit 16.
+constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) {
+  return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+               "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+               "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_at(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, "
+               "%9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+               "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+               "tcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+                 "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                 "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+                 "=r"(r[30]), "=r"(r[31])
+               : "r"(at)
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, "
+               "%9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+               "%24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+               "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+               "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+               "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+               "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, "
+               "%9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+               "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+               "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_stored() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// kCount neighbouring elements of a query row as f32, zero from `dim` on.
+template <typename T, int kCount>
+__device__ __forceinline__ void load_few(const T *row, int d, int dim, float (&x)[kCount]) {
+  constexpr int kBytes = kCount * static_cast<int>(sizeof(T));
+  union {
+    uint32_t raw[kBytes / 4];
+    T at[kCount];
+  } p;
+  const T *at = row + d;
+  if (d >= dim) { // head_dim is a multiple of 16: all or nothing
+#pragma unroll
+    for (int i = 0; i < kBytes / 4; ++i)
+      p.raw[i] = 0;
+  } else if ((reinterpret_cast<uintptr_t>(at) & (kBytes - 1)) == 0) {
+    if constexpr (kBytes == 16)
+      *reinterpret_cast<uint4 *>(p.raw) = *reinterpret_cast<const uint4 *>(at);
+    else if constexpr (kBytes == 8)
+      *reinterpret_cast<uint2 *>(p.raw) = *reinterpret_cast<const uint2 *>(at);
+    else
+      p.raw[0] = *reinterpret_cast<const uint32_t *>(at);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i)
+      p.at[i] = at[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kCount; ++i)
+    x[i] = to_f32(p.at[i]);
+}
+
+template <typename T, int kCh, int kParts, bool kShare>
+__global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendArgs a, int tiles) {
+  static_assert(kParts == 1 || kShare, "two query tiles of two parts do not fit");
+  extern __shared__ uint8_t raw[];
+  PromptSmem<kCh> &sm =
+      *reinterpret_cast<PromptSmem<kCh> *>(raw + ((1024u - (smem_at(raw) & 1023u)) & 1023u));
+  const KvView &v = a.v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kRows = kShare ? kTile : 2 * kTile; // query rows of this CTA
+  constexpr int kD = 64 * kCh;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) {
+      bar_init(&sm.kv_full[i], 128);
+      bar_init(&sm.kv_empty[i], 1);
+      bar_init(&sm.scale_full[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sm.s_full[i], 1);
+      bar_init(&sm.p_full[i], 128);
+      bar_init(&sm.o_full[i], 1);
+    }
+    bar_init(&sm.done, 1);
+    sm.failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.z, split = blockIdx.x;
+  const int head = blockIdx.y % v.heads;
+  // The last tiles of a causal prompt see the most keys: they start first.
+  const int f0 = (tiles - 1 - static_cast<int>(blockIdx.y) / v.heads) * kRows;
+  const KvSequence s = kv_sequence(v, b);
+  if (!s.ok) {
+    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0)
+      atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
+    return;
+  }
+  const int rows = s.n * a.group;
+  if (f0 >= rows)
+    return;
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_at(&sm.tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  const int offset = s.length - s.n;
+  const int last = min(f0 + kRows, rows) - 1;
+  int lo, hi;
+  key_range(a, s.length, offset + f0 / a.group, offset + last / a.group, lo, hi);
+  const int first16 = lo >> 4;
+  const int all = (((hi + 15) >> 4) - first16 + 7) / 8; // tiles of 128 keys
+  const int each = (all + a.splits - 1) / a.splits;
+  const int tile0 = min(all, split * each), count = min(all, tile0 + each) - tile0;
+  const int key_base = (first16 << 4) + tile0 * kTile; // of this CTA's tile 0
+
+  // Queries: a warp takes every 16th row, a lane 2 * kCh neighbouring elements.
+  const bool negative = a.scale_log2 < 0.0f; // the products then take -q
+#pragma unroll 4
+  for (int r = warp; r < kRows; r += kThreads / 32) {
+    constexpr int kE = 2 * kCh;
+    const int f = f0 + r;
+    const int d = kE * lane;
+    float x[kE];
+#pragma unroll
+    for (int i = 0; i < kE; ++i)
+      x[i] = 0.0f;
+    if (f < rows) {
+      const int i = f / a.group;
+      load_few<T, kE>(static_cast<const T *>(a.q) + (s.row0 + i) * a.q_row_stride +
+                          (head * a.group + f - i * a.group) * a.q_head_stride,
+                      d, v.dim, x);
+    }
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kE; ++i)
+      amax = nan_max(amax, fabsf(x[i]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      amax = nan_max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    // A row with NaN or infinity gives NaN wherever it sees a key.
+    const bool wild = !(amax < INFINITY);
+    float factor, inverse;
+    row_factor(wild ? 0.0f : amax, factor, inverse);
+    if (lane == 0)
+      sm.coef[r] = wild ? NAN : inverse * fabsf(a.scale_log2);
+    if (negative)
+      factor = -factor;
+    uint32_t h[kE / 2], l[kE / 2];
+#pragma unroll
+    for (int i = 0; i < kE; i += 2) {
+      const float y0 = wild ? 0.0f : x[i] * factor, y1 = wild ? 0.0f : x[i + 1] * factor;
+      h[i / 2] = pack_half(y0, y1);
+      const float2 back = unpack_half(h[i / 2]);
+      l[i / 2] = pack_half(y0 - back.x, y1 - back.y);
+    }
+    uint8_t *to = sm.q[kShare ? 0 : r / kTile] + (d / 64) * kPanel + (r % kTile) * 128 +
+                  ((((d % 64) / 8) ^ (r & 7)) << 4) + (d % 8) * 2;
+    if constexpr (kCh == 2) {
+      *reinterpret_cast<uint2 *>(to) = make_uint2(h[0], h[1]);
+      if constexpr (kParts == 2)
+        *reinterpret_cast<uint2 *>(to + kCh * kPanel) = make_uint2(l[0], l[1]);
+    } else {
+      *reinterpret_cast<uint32_t *>(to) = h[0];
+      if constexpr (kParts == 2)
+        *reinterpret_cast<uint32_t *>(to + kCh * kPanel) = l[0];
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = sm.tmem;
+  int *failed = &sm.failed;
+
+  if (warp == 12) {
+    // ----------------------------------------------------------- products
+    if (lane == 0) {
+      constexpr uint32_t kS = idesc_f16(kTile, kTile, false), kO = idesc_f16(kTile, kD, true);
+      const uint32_t q_at = smem_at(sm.q), kv_at = smem_at(sm.kv);
+      auto scores = [&](int st, int tile) { // S of stream st
+        const uint32_t qt = q_at + (kShare ? 0 : st) * kCh * kPanel;
+        const uint32_t kt = kv_at + 2 * (tile & 1) * kCh * kPanel;
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) // the small part first
+#pragma unroll
+          for (int i = 0; i < 4 * kCh; ++i) {
+            const uint32_t step = (i / 4) * kPanel + (i % 4) * 32;
+            mma_ss(tmem + st * kTile, desc_k_major(qt + (kParts - 1 - part) * kCh * kPanel + step),
+                   desc_k_major(kt + step), kS, part + i > 0);
+          }
+        commit(&sm.s_full[st]);
+      };
+      auto outputs = [&](int st, int tile, bool fresh) { // O of stream st
+        const uint32_t vt = kv_at + (2 * (tile & 1) + 1) * kCh * kPanel;
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            mma_ts(tmem + 2 * kTile + st * kD,
+                   tmem + st * kTile + (i / 2) * 32 + (i % 2) * 8 + (kParts - 1 - part) * 16,
+                   desc_mn_major(vt + i * 2048), kO, !fresh || part + i > 0);
+        commit(&sm.o_full[st]);
+      };
+      bool ok = true;
+      auto wait = [&](uint64_t *bar, uint32_t parity) {
+        ok = ok && bar_wait(bar, parity, failed);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        return ok;
+      };
+      if constexpr (kShare) {
+        for (int j = 0; j < 2 && j < count; ++j)
+          if (wait(&sm.kv_full[2 * (j & 1)], (j >> 1) & 1)) {
+            scores(j & 1, j);
+            commit(&sm.kv_empty[2 * (j & 1)]);
+          }
+        for (int j = 0; j < count && ok; ++j) {
+          const int st = j & 1, slot = 2 * (j & 1);
+          if (!wait(&sm.kv_full[slot + 1], (j >> 1) & 1) || !wait(&sm.p_full[st], (j >> 1) & 1))
+            break;
+          outputs(st, j, j < 2);
+          commit(&sm.kv_empty[slot + 1]);
+          if (j + 2 < count) {
+            if (!wait(&sm.kv_full[slot], ((j + 2) >> 1) & 1))
+              break;
+            scores(st, j + 2);
+            commit(&sm.kv_empty[slot]);
+          }
+        }
+      } else if (count > 0) {
+        if (wait(&sm.kv_full[0], 0)) {
+          scores(0, 0);
+          scores(1, 0);
+          commit(&sm.kv_empty[0]);
+        }
+        for (int j = 0; j < count && ok; ++j) {
+          const int slot = 2 * (j & 1), next = 2 * ((j + 1) & 1);
+          if (!wait(&sm.kv_full[slot + 1], (j >> 1) & 1))
+            break;
+          for (int st = 0; st < 2 && ok; ++st) {
+            if (!wait(&sm.p_full[st], j & 1))
+              break;
+            outputs(st, j, j == 0);
+            if (st == 1)
+              commit(&sm.kv_empty[slot + 1]);
+            if (j + 1 < count) {
+              if (st == 0 && !wait(&sm.kv_full[next], ((j + 1) >> 1) & 1))
+                break;
+              scores(st, j + 1);
+              if (st == 1)
+                commit(&sm.kv_empty[next]);
+            }
+          }
+        }
+      }
+      // Nothing of this CTA may be in flight when its TMEM is freed.
+      commit(&sm.done);
+      int unused = 0;
+      bar_wait(&sm.done, 0, &unused);
+    }
+  } else if (warp >= 8 && warp < 12) {
+    // ---------------------------------------------------------- converters
+    // A thread loads 16 codes (one token's sixteenth part p of 64 or 128) a
+    // step; eight neighbouring lanes hold two tokens of one panel, so that
+    // their 16-byte stores fall in different banks.
+    constexpr int kSteps = 4 * kCh;          // steps of kTile tokens
+    constexpr int kTokens = kTile / kSteps;  // tokens a step
+    const int t = threadIdx.x - 256, quarter = t >> 3, r = t & 7;
+    const int token = kCh == 2 ? (quarter >> 1) * 2 + (r >> 2) : quarter * 2 + (r >> 2);
+    const int part = kCh == 2 ? (quarter & 1) * 4 + (r & 3) : (r & 3);
+    const bool inside = part * 16 < v.dim;
+    const int64_t per_page = static_cast<int64_t>(v.heads) * 2 << v.block_log2;
+    const int in_page = (1 << v.block_log2) - 1;
+
+    // Lane i (mod 8) holds the page of the tile's i-th group of 16 tokens.
+    auto pages_of = [&](int tile) {
+      int page = -1;
+      const int key = key_base + tile * kTile + (lane & 7) * 16;
+      if (tile < count && key < s.length) {
+        page = kv_page(v, b, key >> v.block_log2);
+        if (page < 0 && t < 8)
+          atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
+      }
+      return page;
+    };
+    uint4 hold[2][kSteps];
+    auto load = [&](int tile, int side, int pages, uint4 (&to)[kSteps]) {
+      const int key0 = key_base + tile * kTile;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int at = i * kTokens + token;
+        const int page = __shfl_sync(0xffffffffu, pages, at >> 4);
+        to[i] = make_uint4(0, 0, 0, 0);
+        if (page >= 0 && inside) {
+          const int64_t row = page * per_page + (static_cast<int64_t>(head * 2 + side) << v.block_log2) +
+                              ((key0 + at) & in_page);
+          to[i] = __ldg(reinterpret_cast<const uint4 *>(v.codes + row * v.dim + part * 16));
+        }
+      }
+    };
+    auto store = [&](int slot, const uint4 (&from)[kSteps]) {
+      uint8_t *base = sm.kv[slot] + (part / 4) * kPanel;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int at = i * kTokens + token;
+        uint4 x, y;
+        codes_to_half(from[i].x, x.x, x.y);
+        codes_to_half(from[i].y, x.z, x.w);
+        codes_to_half(from[i].z, y.x, y.y);
+        codes_to_half(from[i].w, y.z, y.w);
+        uint8_t *row = base + at * 128;
+        const int chunk = (part & 3) * 2;
+        *reinterpret_cast<uint4 *>(row + ((chunk ^ (at & 7)) << 4)) = x;
+        *reinterpret_cast<uint4 *>(row + (((chunk + 1) ^ (at & 7)) << 4)) = y;
+      }
+    };
+    int pages = pages_of(0), next = pages_of(1);
+    load(0, 0, pages, hold[0]);
+    for (int j = 0; j < count; ++j) {
+      const int slot = 2 * (j & 1), round = j >> 1;
+      load(j, 1, pages, hold[1]);
+      if (t < 8) { // scales of the tile's groups
+        float4 sc = make_float4(0.0f, -INFINITY, 0.0f, 0.0f); // hidden
+        if (pages >= 0) {
+          const float2 two = *reinterpret_cast<const float2 *>(
+              v.scales + (static_cast<int64_t>(pages) * v.heads + head) * 2);
+          const float sv = fmaxf(two.y, kKvLeastScale);
+          sc = make_float4(two.x, log2f(sv), 1.0f / sv, 0.0f);
+        }
+        sm.scale[j & 3][t] = sc;
+      }
+      if (t < 32) {
+        __syncwarp();
+        if (t == 0)
+          bar_arrive(&sm.scale_full[j & 3]);
+      }
+      if (round > 0 && !bar_wait(&sm.kv_empty[slot], (round - 1) & 1, failed))
+        break;
+      store(slot, hold[0]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(&sm.kv_full[slot]);
+      const int after = pages_of(j + 2);
+      if (j + 1 < count)
+        load(j + 1, 0, next, hold[0]);
+      if (round > 0 && !bar_wait(&sm.kv_empty[slot + 1], (round - 1) & 1, failed))
+        break;
+      store(slot + 1, hold[1]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(&sm.kv_full[slot + 1]);
+      pages = next;
+      next = after;
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------- softmax
+    const int st = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + st * kTile + lanes, o_at = tmem + 2 * kTile + st * kD + lanes;
+    const int f = f0 + (kShare ? 0 : st * kTile) + row;
+    const bool live = f < rows;
+    const int pos = offset + (live ? f / a.group : 0);
+    const int row_hi = !live ? 0 : a.causal ? min(s.length, pos + 1) : s.length;
+    const int row_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const float coef = sm.coef[kShare ? row : st * kTile + row];
+    float m = -INFINITY, l = 0.0f;
+    const int mine = kShare ? (count - st + 1) / 2 : count;
+    bool ok = true;
+#pragma unroll 1
+    for (int n = 0; n < mine; ++n) {
+      const int tile = kShare ? 2 * n + st : n;
+      const int key0 = key_base + tile * kTile;
+      const int from = min(max(row_lo - key0, 0), kTile), to = min(max(row_hi - key0, 0), kTile);
+      const bool whole = __all_sync(0xffffffffu, from == 0 && to == kTile);
+      auto visible = [&](int c) -> uint32_t { // of scores 32 c .. 32 c + 31
+        const int x = min(max(from - 32 * c, 0), 32), y = min(max(to - 32 * c, 0), 32);
+        return y > x ? (0xffffffffu >> (32 - (y - x))) << x : 0u;
+      };
+      ok = bar_wait(&sm.scale_full[tile & 3], (tile >> 2) & 1, failed) &&
+           bar_wait(&sm.s_full[st], n & 1, failed);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok)
+        break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const float4 *scale = sm.scale[tile & 3];
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[32];
+        tmem_load(s_at + 32 * c, x);
+        const uint32_t seen = whole ? 0xffffffffu : visible(c);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float best = -INFINITY;
+#pragma unroll
+          for (int i = 16 * g; i < 16 * g + 16; ++i)
+            best = fmaxf(best, whole || (seen >> i & 1) ? __uint_as_float(x[i]) : -INFINITY);
+          const float4 sc = scale[2 * c + g];
+          if (best != -INFINITY)
+            top = nan_max(top, fmaf(best, coef * sc.x, sc.y));
+        }
+      }
+      // Set the row's reference again when its probabilities outgrow f16.
+      const bool set = top != -INFINITY &&
+                       (m == -INFINITY || !(top - m <= kGrowth<kParts>));
+      if (__any_sync(0xffffffffu, set)) {
+        const float m_new = set ? top - kTop<kParts> : m;
+        const float shrink = set ? exp2_approx(m - m_new) : 1.0f; // 0 for the first
+        m = m_new;
+        l *= shrink;
+        if (n > 0) {
+          ok = __all_sync(0xffffffffu, bar_wait(&sm.o_full[st], (n - 1) & 1, failed));
+          if (!ok)
+            break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+          for (int c = 0; c < 2 * kCh; ++c) {
+            uint32_t x[32];
+            tmem_load(o_at + 32 * c, x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              x[i] = __float_as_uint(__uint_as_float(x[i]) * shrink);
+            tmem_store32(o_at + 32 * c, x);
+          }
+        }
+      }
+      const float origin = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[32];
+        tmem_load(s_at + 32 * c, x);
+        const uint32_t seen = whole ? 0xffffffffu : visible(c);
+        uint32_t high[16], low[16];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const float4 sc = scale[2 * c + g];
+          const float slope = coef * sc.x, shift = sc.y - origin;
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 16 * g; i < 16 * g + 16; i += 2) {
+            float e0 = fmaf(__uint_as_float(x[i]), slope, shift);
+            float e1 = fmaf(__uint_as_float(x[i + 1]), slope, shift);
+            if (!whole) {
+              e0 = seen >> i & 1 ? e0 : -INFINITY;
+              e1 = seen >> (i + 1) & 1 ? e1 : -INFINITY;
+            }
+            const float p0 = exp2_approx(e0), p1 = exp2_approx(e1);
+            sum += p0 + p1;
+            high[i / 2] = pack_half(p0, p1);
+            if constexpr (kParts == 2) {
+              const float2 back = unpack_half(high[i / 2]);
+              low[i / 2] = pack_half(p0 - back.x, p1 - back.y);
+            }
+          }
+          l = fmaf(sum, sc.z, l);
+        }
+        // Over the scores just read.
+        tmem_store16(s_at + 32 * c, high);
+        if constexpr (kParts == 2)
+          tmem_store16(s_at + 32 * c + 16, low);
+      }
+      tmem_stored();
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      bar_arrive(&sm.p_full[st]);
+    }
+    if (ok && mine > 0)
+      ok = bar_wait(&sm.o_full[st], (mine - 1) & 1, failed);
+    ok = __all_sync(0xffffffffu, ok);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    float share = 1.0f, other = 0.0f;
+    float *joined = reinterpret_cast<float *>(sm.kv[0]); // [element][row]
+    if constexpr (kShare) {
+      // Every product has completed (both streams have waited for theirs).
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (st == 1) {
+        sm.join[0][row] = mine > 0 ? m : -INFINITY;
+        sm.join[1][row] = l;
+        if (mine > 0) {
+#pragma unroll 1
+          for (int c = 0; c < 2 * kCh; ++c) {
+            uint32_t x[32];
+            tmem_load(o_at + 32 * c, x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              joined[(32 * c + i) * kTile + row] = __uint_as_float(x[i]);
+          }
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (st == 0) {
+        const float m1 = sm.join[0][row];
+        const float most = nan_max(m, m1);
+        share = m == -INFINITY ? 0.0f : exp2_approx(m - most);
+        other = m1 == -INFINITY ? 0.0f : exp2_approx(m1 - most);
+        l = l * share + (m1 == -INFINITY ? 0.0f : sm.join[1][row] * other);
+        m = most;
+      }
+    }
+    const bool some = m != -INFINITY;
+    if (!kShare || st == 0) {
+      const bool apart = a.splits > 1;
+      const float scale = !some ? 0.0f : apart ? 1.0f : 1.0f / l;
+      const int i = live ? f / a.group : 0;
+      const int64_t at = (s.row0 + i) * a.q_heads + head * a.group + (live ? f - i * a.group : 0);
+      const int64_t slot = static_cast<int64_t>(split) * v.rows * a.q_heads + at;
+#pragma unroll 1
+      for (int c = 0; c < 2 * kCh; ++c) {
+        uint32_t x[32];
+        tmem_load(o_at + 32 * c, x);
+        float y[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          // Where a stream had no keys its accumulators hold nothing.
+          float o = share == 0.0f ? 0.0f : __uint_as_float(x[k]) * share;
+          if constexpr (kShare)
+            if (other != 0.0f)
+              o = fmaf(joined[(32 * c + k) * kTile + row], other, o);
+          y[k] = some ? o * scale : 0.0f;
+        }
+        if (live && ok) {
+          if (apart) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              Pack<float> p;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                p.at[e] = y[k + e];
+              store_pack(a.part_o + slot * v.dim, 32 * c + k, v.dim, p);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; k += kVec<T>) {
+              Pack<T> p;
+#pragma unroll
+              for (int e = 0; e < kVec<T>; ++e)
+                p.at[e] = from_f32<T>(y[k + e]);
+              store_pack(static_cast<T *>(a.out) + at * v.dim, 32 * c + k, v.dim, p);
+            }
+          }
+        }
+      }
+      if (live && ok) {
+        if (apart)
+          a.part_ml[slot] = make_float4(some ? m : -INFINITY, l, l, 0.0f);
+        else if (a.lse)
+          a.lse[at] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(failed))
+    atomicOr(a.status, CIM22_STATUS_TIMEOUT);
+  if (warp == 12) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+template <typename T, int kCh, int kParts, bool kShare>
+cudaError_t launch_prompt(const KvAttendArgs &a, int tiles, cudaStream_t stream) {
+  constexpr size_t bytes = sizeof(PromptSmem<kCh>) + 1024;
+  const auto kernel = kv_prompt_kernel<T, kCh, kParts, kShare>;
+  static DynamicSmem allowed;
+  if (const cudaError_t e = allowed.allow(kernel, bytes); e != cudaSuccess)
+    return e;
+  return launch_pdl(kernel, dim3(a.splits, static_cast<unsigned>(tiles * a.v.heads), a.v.batch),
+                    dim3(kThreads), bytes, stream, a, tiles);
+}
+
+} // namespace
+
+cudaError_t kv_prompt_launch(const KvAttendArgs &a, int type, bool share, int tiles,
+                             cudaStream_t stream) {
+  const bool wide = a.v.dim > 64;
+  if (type == CIM22_FLOAT32)
+    return wide ? launch_prompt<float, 2, 2, true>(a, tiles, stream)
+                : launch_prompt<float, 1, 2, true>(a, tiles, stream);
+  if (type == CIM22_BFLOAT16) {
+    if (share)
+      return wide ? launch_prompt<__nv_bfloat16, 2, 1, true>(a, tiles, stream)
+                  : launch_prompt<__nv_bfloat16, 1, 1, true>(a, tiles, stream);
+    return wide ? launch_prompt<__nv_bfloat16, 2, 1, false>(a, tiles, stream)
+                : launch_prompt<__nv_bfloat16, 1, 1, false>(a, tiles, stream);
+  }
+  if (share)
+    return wide ? launch_prompt<__half, 2, 1, true>(a, tiles, stream)
+                : launch_prompt<__half, 1, 1, true>(a, tiles, stream);
+  return wide ? launch_prompt<__half, 2, 1, false>(a, tiles, stream)
+              : launch_prompt<__half, 1, 1, false>(a, tiles, stream);
+}
+
+} // namespace cim
