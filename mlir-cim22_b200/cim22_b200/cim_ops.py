@@ -6,7 +6,6 @@ kernel of libcim22_cuda.so. Tensors must be contiguous CUDA tensors.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -24,7 +23,10 @@ def _ptr(t: torch.Tensor | None):
 
 
 def _stream(device: torch.device | None = None):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    index = device.index if device is not None else None
+    if index is None:
+        index = torch.cuda.current_device()
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
 
 
 def _require(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
@@ -34,14 +36,18 @@ def _require(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
 
 FLOAT_TYPES = {torch.float32: abi.FLOAT32, torch.bfloat16: abi.BFLOAT16,
                torch.float16: abi.FLOAT16}
-_SAME_DEVICE = contextlib.nullcontext()
 
 
-def on_device(device: torch.device):
-    """Context in which launches go to a tensor's device."""
-    if device.index == torch.cuda.current_device():
-        return _SAME_DEVICE
-    return torch.cuda.device(device)
+def launch(what: str, index: int, fn, *args) -> None:
+    """fn(*args, stream) with launches going to device `index` and its current
+    stream."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    check(rc, what)
 
 
 class Workspace:
@@ -445,37 +451,49 @@ _GATE_ACT = {None: abi.GATE_NONE, "none": abi.GATE_NONE, "sigmoid": abi.GATE_SIG
 def _as_rows(t: torch.Tensor, like: torch.Tensor, name: str) -> int:
     """The row stride of a tensor taken as rows of its last axis: any 2-D tensor
     whose last axis is contiguous, or a contiguous one."""
-    if t.device != like.device or t.dtype != like.dtype or t.shape != like.shape:
+    if t.get_device() != like.get_device() or t.dtype != like.dtype or t.shape != like.shape:
         raise TypeError(f"{name} must have x's shape, type and device")
-    dim = t.shape[-1]
-    if t.dim() == 2 and (t.stride(1) == 1 or dim == 1) and (t.shape[0] <= 1
-                                                            or t.stride(0) >= dim):
+    if t.is_contiguous():
+        return t.shape[-1]
+    if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1]:
         return t.stride(0)
-    if not t.is_contiguous():
-        raise TypeError(f"{name} must be contiguous, or rows with a contiguous last axis")
-    return dim
+    raise TypeError(f"{name} must be contiguous, or rows with a contiguous last axis")
 
 
-def _norm_arg(norm: Norm | None, x: torch.Tensor, name: str) -> abi.Norm | None:
-    if norm is None:
-        return None
+def _norm_arg(norm: Norm, x: torch.Tensor, dim: int, name: str):
     if norm.kind not in _NORM_KIND:
         raise ValueError(f"{name} norm must be \"rms\" or \"layer\"")
-    arg = abi.Norm(kind=_NORM_KIND[norm.kind], eps=norm.eps, type=FLOAT_TYPES[x.dtype])
-    kinds = set()
-    for field, t in (("weight", norm.weight), ("bias", norm.bias)):
+    weight, bias = norm.weight, norm.bias
+    dtype = x.dtype
+    for field, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
-        if t.device != x.device or t.dtype not in (torch.float32, x.dtype) \
-                or t.shape != x.shape[-1:] or not t.is_contiguous():
+        if t.get_device() != x.get_device() or t.dtype not in (torch.float32, x.dtype) \
+                or t.dim() != 1 or t.shape[0] != dim or not t.is_contiguous():
             raise TypeError(f"{name} {field} must be a contiguous [dim] tensor on x's device, "
                             "f32 or of x's type")
-        kinds.add(t.dtype)
-        arg.type = FLOAT_TYPES[t.dtype]
-        setattr(arg, field, t.data_ptr())
-    if len(kinds) > 1:
+        dtype = t.dtype
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"{name} weight and bias must have one type")
-    return arg
+    return ctypes.pointer(abi.Norm(_NORM_KIND[norm.kind], norm.eps,
+                                   None if weight is None else weight.data_ptr(),
+                                   None if bias is None else bias.data_ptr(),
+                                   FLOAT_TYPES[dtype]))
+
+
+def _gate_rows(gate: torch.Tensor, x: torch.Tensor, rows: int, dim: int) -> int:
+    """Consecutive rows that share a gate row; 0 for a single gate row."""
+    if gate.get_device() != x.get_device() or gate.dtype not in (torch.float32, x.dtype) \
+            or not gate.is_contiguous():
+        raise TypeError("gate must be a contiguous tensor on x's device, f32 or of x's type")
+    if gate.dim() == 1 and gate.shape[0] == dim:
+        return 0
+    if gate.dim() >= 2 and gate.shape[-1] in (1, dim):
+        lead = gate.numel() // gate.shape[-1]
+        if rows == 0 or lead and rows % lead == 0:
+            return rows // lead if lead > 1 else 0
+    raise ValueError("gate must be [dim], or [groups, dim] or [groups, 1] with groups dividing "
+                     "the rows")
 
 
 def block_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
@@ -506,44 +524,29 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     rows = x.numel() // dim
     if gate_activation not in _GATE_ACT:
         raise ValueError("gate activation must be None, sigmoid or tanh")
-    d = abi.BlockNorm(type=FLOAT_TYPES[x.dtype], rows=rows, dim=dim, x=x.data_ptr(),
-                      x_stride=_as_rows(x, x, "x"), residual_scale=residual_scale)
-    if residual is not None:
-        d.residual, d.residual_stride = residual.data_ptr(), _as_rows(residual, x, "residual")
-    if gate is not None:
-        if gate.device != x.device or gate.dtype not in (torch.float32, x.dtype) \
-                or not gate.is_contiguous():
-            raise TypeError("gate must be a contiguous tensor on x's device, f32 or of x's type")
-        lead = gate.numel() // max(1, gate.shape[-1]) if gate.dim() else 0
-        if gate.dim() == 1 and gate.shape[0] == dim:
-            lead = 1
-        elif gate.dim() < 2 or gate.shape[-1] not in (1, dim) \
-                or lead < 1 and rows or lead and rows % lead:
-            raise ValueError("gate must be [dim], or [groups, dim] or [groups, 1] with groups "
-                             "dividing the rows")
-        d.gate, d.gate_type = gate.data_ptr(), FLOAT_TYPES[gate.dtype]
-        d.gate_columns = d.gate_stride = gate.shape[-1]
-        d.gate_rows = rows // lead if lead > 1 else 0
-        d.gate_activation = _GATE_ACT[gate_activation]
-    combined = residual is not None or post is not None or gate is not None
-    post_arg, pre_arg = _norm_arg(post, x, "post"), _norm_arg(pre, x, "pre")
+    gate_rows = 0 if gate is None else _gate_rows(gate, x, rows, dim)
     h = y = None
-    if combined or out is not None:
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-        d.h, d.h_stride = h.data_ptr(), _as_rows(h, x, "out")
+    if out is not None or residual is not None or post is not None or gate is not None:
+        h = torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else out
     if pre is not None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if normed is None else normed
-        d.y, d.y_stride = y.data_ptr(), _as_rows(y, x, "normed")
+        y = torch.empty_like(x, memory_format=torch.contiguous_format) if normed is None \
+            else normed
     elif normed is not None:
         raise ValueError("normed is an output of pre: it needs one")
     if h is None and y is None:
         raise ValueError("nothing to compute: give a residual, post, gate or pre")
-    if post_arg is not None:
-        d.post = ctypes.pointer(post_arg)
-    if pre_arg is not None:
-        d.pre = ctypes.pointer(pre_arg)
-    with on_device(x.device):
-        check(lib().cim22_cuda_block_norm(ctypes.byref(d), _stream(x.device)), "block_norm")
+    call = abi.BlockNorm(
+        FLOAT_TYPES[x.dtype], rows, dim, x.data_ptr(), _as_rows(x, x, "x"),
+        None if residual is None else residual.data_ptr(),
+        0 if residual is None else _as_rows(residual, x, "residual"), residual_scale,
+        None if gate is None else gate.data_ptr(), 0 if gate is None else gate.shape[-1],
+        gate_rows, 0 if gate is None else gate.shape[-1],
+        0 if gate is None else FLOAT_TYPES[gate.dtype], _GATE_ACT[gate_activation],
+        None if post is None else _norm_arg(post, x, dim, "post"),
+        None if pre is None else _norm_arg(pre, x, dim, "pre"),
+        None if h is None else h.data_ptr(), 0 if h is None else _as_rows(h, x, "out"),
+        None if y is None else y.data_ptr(), 0 if y is None else _as_rows(y, x, "normed"))
+    launch("block_norm", x.get_device(), lib().cim22_cuda_block_norm, ctypes.byref(call))
     return h, y
 
 

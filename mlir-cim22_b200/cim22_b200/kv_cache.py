@@ -25,8 +25,8 @@ import math
 import torch
 
 from . import abi
-from .cim_ops import FLOAT_TYPES, StatusWord, Workspace, _ptr, _stream, on_device
-from .native import check, lib
+from .cim_ops import FLOAT_TYPES, StatusWord, Workspace, launch
+from .native import lib
 
 BLOCKS = (16, 32, 64, 128)
 
@@ -74,26 +74,29 @@ class Int8KVCache:
     def _init(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
         self.codes, self.scales = codes, scales
         self.pages, self.kv_heads, _, self.block, self.head_dim = codes.shape
-        self.device = codes.device
+        self.device, self._index = codes.device, codes.get_device()
         self._view = abi.KvCache(codes=codes.data_ptr(), scales=scales.data_ptr(),
                                  pages=self.pages, kv_heads=self.kv_heads, block=self.block,
                                  head_dim=self.head_dim)
 
     # ------------------------------------------------------------- descriptions
 
-    def _int32(self, t: torch.Tensor, shape: tuple, name: str) -> None:
-        if t.device != self.device or t.dtype != torch.int32 or tuple(t.shape) != shape:
-            raise TypeError(f"{name} must be an int32 tensor {list(shape)} on the cache's device")
+    def _int32(self, t: torch.Tensor, count: int, name: str) -> None:
+        if t.get_device() != self._index or t.dtype != torch.int32 or t.dim() != 1 \
+                or t.shape[0] != count or not t.is_contiguous():
+            raise TypeError(f"{name} must be a contiguous int32 tensor [{count}] on the cache's "
+                            "device")
 
     def _sequences(self, table: torch.Tensor, lengths: torch.Tensor,
                    starts: torch.Tensor | None, rows: int, most: int | None) -> abi.KvSequences:
-        if table.dim() != 2:
-            raise TypeError("table must be an int32 tensor [batch, pages a sequence]")
+        if table.get_device() != self._index or table.dtype != torch.int32 or table.dim() != 2:
+            raise TypeError("table must be an int32 tensor [batch, pages a sequence] on the "
+                            "cache's device")
         batch, width = table.shape
-        self._int32(table, (batch, width), "table")
-        if width > 1 and table.stride(1) != 1 or batch > 1 and table.stride(0) < width:
+        if not table.is_contiguous() and (width > 1 and table.stride(1) != 1
+                                          or batch > 1 and table.stride(0) < width):
             raise TypeError("table rows must be contiguous and must not overlap")
-        self._int32(lengths, (batch,), "lengths")
+        self._int32(lengths, batch, "lengths")
         if batch > 65535:
             raise ValueError("at most 65535 sequences a call")
         if starts is None:
@@ -101,26 +104,22 @@ class Int8KVCache:
                 raise ValueError("without starts there must be one row for every sequence")
             most = 1
         else:
-            self._int32(starts, (batch + 1,), "starts")
-            if not starts.is_contiguous():
-                raise TypeError("starts must be contiguous")
+            self._int32(starts, batch + 1, "starts")
             most = rows if most is None else most
             if not 0 <= most <= 0x7fffffff:
                 raise ValueError("most out of range")
-        if not lengths.is_contiguous():
-            raise TypeError("lengths must be contiguous")
-        return abi.KvSequences(batch=batch, table=table.data_ptr(), table_stride=table.stride(0),
-                               table_width=width, lengths=lengths.data_ptr(),
-                               starts=None if starts is None else starts.data_ptr(), rows=rows,
-                               most=most)
+        return abi.KvSequences(batch, table.data_ptr(), table.stride(0), width,
+                               lengths.data_ptr(), None if starts is None else starts.data_ptr(),
+                               rows, most)
 
     def _rows(self, t: torch.Tensor, heads: int, name: str) -> None:
-        if t.device != self.device or t.dtype not in FLOAT_TYPES or t.dim() != 3:
+        if t.get_device() != self._index or t.dtype not in FLOAT_TYPES or t.dim() != 3:
             raise TypeError(f"{name} must be an f32, bf16 or f16 tensor [rows, heads, head_dim] "
                             "on the cache's device")
-        if t.shape[1] != heads or t.shape[2] != self.head_dim:
+        _, has, dim = t.shape
+        if has != heads or dim != self.head_dim:
             raise ValueError(f"{name} must have {heads} heads of {self.head_dim}")
-        if t.stride(2) != 1 or min(t.stride()) < 0:
+        if t.stride(2) != 1:
             raise TypeError(f"{name}'s last axis must be contiguous")
 
     # -------------------------------------------------------------------- calls
@@ -144,11 +143,10 @@ class Int8KVCache:
         seqs = self._sequences(table, lengths, starts, k.shape[0], most)
         own_status = status is None
         status = status or StatusWord(self.device)
-        with on_device(self.device):
-            check(lib().cim22_cuda_kv_write(
-                ctypes.byref(self._view), ctypes.byref(seqs), FLOAT_TYPES[k.dtype], _ptr(k),
-                k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1),
-                _ptr(status.tensor), _stream(self.device)), "cim22_cuda_kv_write")
+        launch("cim22_cuda_kv_write", self._index, lib().cim22_cuda_kv_write,
+               ctypes.byref(self._view), ctypes.byref(seqs), FLOAT_TYPES[k.dtype], k.data_ptr(),
+               k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+               status.tensor.data_ptr())
         if own_status:
             status.raise_if_set()
 
@@ -167,8 +165,8 @@ class Int8KVCache:
                 if starts is not None:
                     raise ValueError("tokens (the number of packed rows) is needed with starts")
                 tokens = lengths.shape[0]
-            out = tuple(torch.empty(tokens, self.kv_heads, self.head_dim, dtype=dtype,
-                                    device=self.device) for _ in range(2))
+            k = torch.empty(tokens, self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
+            out = k, torch.empty_like(k)
         k, v = out
         for t, name in ((k, "k"), (v, "v")):
             self._rows(t, self.kv_heads, name)
@@ -179,10 +177,9 @@ class Int8KVCache:
         seqs = self._sequences(table, lengths, starts, k.shape[0], most)
         own_status = status is None
         status = status or StatusWord(self.device)
-        with on_device(self.device):
-            check(lib().cim22_cuda_kv_read(
-                ctypes.byref(self._view), ctypes.byref(seqs), FLOAT_TYPES[k.dtype], _ptr(k),
-                _ptr(v), _ptr(status.tensor), _stream(self.device)), "cim22_cuda_kv_read")
+        launch("cim22_cuda_kv_read", self._index, lib().cim22_cuda_kv_read,
+               ctypes.byref(self._view), ctypes.byref(seqs), FLOAT_TYPES[k.dtype], k.data_ptr(),
+               v.data_ptr(), status.tensor.data_ptr())
         if own_status:
             status.raise_if_set()
         return k, v
@@ -218,26 +215,26 @@ class Int8KVCache:
         if longest < 0:
             raise ValueError("longest must not be negative")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device \
                 or not out.is_contiguous():
             raise TypeError("out must be contiguous, of q's shape and type")
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) \
             if return_lse else None
-        call = abi.KvAttention(type=FLOAT_TYPES[q.dtype], q_heads=heads, q=q.data_ptr(),
-                               q_row_stride=q.stride(0), q_head_stride=q.stride(1),
-                               out=out.data_ptr(),
-                               lse=None if lse is None else lse.data_ptr(), scale=scale,
-                               causal=int(causal), window=window, longest=longest)
+        call = abi.KvAttention(FLOAT_TYPES[q.dtype], heads, q.data_ptr(), q.stride(0),
+                               q.stride(1), out.data_ptr(),
+                               None if lse is None else lse.data_ptr(), scale, int(causal),
+                               window, longest)
         own_status = status is None
         status = status or StatusWord(self.device)
-        with on_device(self.device):
-            nbytes = lib().cim22_cuda_kv_attend_workspace(
-                ctypes.byref(self._view), ctypes.byref(seqs), ctypes.byref(call))
+        cache, seqs, call = ctypes.byref(self._view), ctypes.byref(seqs), ctypes.byref(call)
+        ws = None
+        nbytes = lib().cim22_cuda_kv_attend_workspace(cache, seqs, call)
+        if nbytes:
             ws = (workspace or Workspace(self.device)).get(nbytes)
-            check(lib().cim22_cuda_kv_attend(
-                ctypes.byref(self._view), ctypes.byref(seqs), ctypes.byref(call), _ptr(ws),
-                ws.numel(), _ptr(status.tensor), _stream(self.device)), "cim22_cuda_kv_attend")
+        launch("cim22_cuda_kv_attend", self._index, lib().cim22_cuda_kv_attend, cache, seqs, call,
+               None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+               status.tensor.data_ptr())
         if own_status:
             status.raise_if_set()
         return (out, lse) if return_lse else out

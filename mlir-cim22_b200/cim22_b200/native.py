@@ -127,6 +127,8 @@ EXPORTED = tuple(_SIGNATURES)
 def lib() -> ctypes.CDLL:
     """Load the CUDA backend. Raises ImportError when it has not been built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not LIBRARY.exists():

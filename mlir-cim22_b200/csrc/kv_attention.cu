@@ -1,19 +1,21 @@
 // kv_attention.cu - attention of few query rows over the 8-bit cache, and the
 // dispatch between it and the tensor-memory kernel for prompts.
 //
-// Decode reads every cached code once: bound by HBM. A tile is the 16 rows of
-// an m16n8k16 product (query tokens x the heads that share a kv head), a work
-// item a 16-token group of one kv head, which lies in one page, so its two
-// scales are constants. Warps take groups in turn and need nothing from each
-// other until the end: each lane copies (cp.async) exactly the bytes it later
-// feeds the product with into its own shared-memory slots, six groups deep,
-// so the ring has no barriers and no bank conflicts:
-//   keys    lane (g, c) holds token g's codes 16c .. 16c + 15 of each 64: the
-//           contraction runs over head_dim in the order that makes these its
-//           B fragments, and the queries are laid out to match;
+// Decode reads every cached code once: bound by HBM. The products are taken
+// transposed, S^T = K Q^T and O^T = V^T P^T (m16n8k16), so that 16 tokens or
+// 16 elements of the head fill the 16 rows and a tile needs only 8 query rows
+// (query tokens x the heads that share a kv head). A work item is a 16-token
+// group of one kv head, which lies in one page, so its two scales are
+// constants. Warps take groups in turn and need nothing from each other until
+// the end: each lane copies (cp.async) exactly the bytes it later feeds the
+// products with into its own shared-memory slots, a few groups deep, so the
+// ring has no barriers and no bank conflicts:
+//   keys    lane (g, c) holds codes 16c .. 16c + 15 of each 64 of tokens g and
+//           8 + g: the contraction runs over head_dim in the order that makes
+//           these its A fragments, and the queries are laid out to match;
 //   values  lane (g, c) holds codes 16g .. 16g + 15 (D = 128) of tokens 2c,
-//           2c + 1, 8 + 2c, 9 + 2c: byte permutes make the fragments, and the
-//           output columns come out as 32 neighbouring elements a lane.
+//           2c + 1, 8 + 2c, 9 + 2c: byte permutes make the A fragments, and
+//           neighbouring rows of the result are neighbouring elements.
 // Codes are exact in f16. Queries are scaled by a power of two a row and held
 // as one f16 part (bf16 and f16 inputs lose nothing within 2^-39 of the row's
 // largest) or two (f32: 22 bits); so are the probabilities.
@@ -24,24 +26,37 @@
 namespace cim {
 namespace {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 6;
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
 
+// CTAs an SM by the registers that query tiles and parts take, and the depth
+// of the copies that then fits in shared memory.
+template <int kParts, int kQ> constexpr int kResident = kParts * kQ == 1 ? 4 : kParts * kQ == 2 ? 3 : 2;
 template <int kCh> constexpr int kStageBytes = 16 * 2 * 64 * kCh; // one group of one warp
+template <int kCh, int kParts, int kQ> constexpr int kStages = 24 / (kResident<kParts, kQ> * kCh);
 
 __device__ __forceinline__ uint32_t smem_at(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
-template <int kBytes>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, bool valid) {
+template <int kBytes> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src) {
   if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                 "r"(valid ? 16 : 0)
-                 : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src),
-                 "r"(valid ? 8 : 0)
-                 : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// The 8 x 8 matrix of 16-bit values that a warp's registers hold, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Code + 1152 as f16: what codes_to_half gives before its subtraction.
+__device__ __forceinline__ void codes_to_half_raised(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  w ^= 0x80808080u;
+  lo = __byte_perm(w, 0x64646464u, 0x4140);
+  hi = __byte_perm(w, 0x64646464u, 0x4342);
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -65,17 +80,22 @@ __device__ __forceinline__ void put_row(T *out, int d, int dim, const float (&v)
   }
 }
 
-template <typename T, int kCh, int kParts>
-__global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendArgs a) {
-  constexpr int kTiles = 8 * kCh;     // output tiles: element 8 * kCh * g + j of the head
-  constexpr int kLane = 8 * kCh;      // value bytes a lane holds of a token
+template <typename T, int kCh, int kParts, int kQ>
+__global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
+    kv_decode_kernel(const KvAttendArgs a) {
+  constexpr int kTiles = 4 * kCh;  // 16-element tiles of the head
+  constexpr int kLane = 8 * kCh;   // value bytes a lane holds of a token
+  constexpr int kDepth = kStages<kCh, kParts, kQ>;
+  constexpr int kRows = 8 * kQ;
+  constexpr bool kRaised = kParts == 1; // keys enter with 1152 added
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float row_m[kWarps][16], row_l[kWarps][16], row_e[kWarps][16];
+  __shared__ float row_m[kWarps][kRows], row_l[kWarps][kRows], row_e[kWarps][kRows];
+  __shared__ float4 constants[kWarps][32];
   pdl_launch_dependents();
   pdl_wait();
   const KvView &v = a.v;
   const int b = blockIdx.z, split = blockIdx.x;
-  const int head = blockIdx.y % v.heads, f0 = blockIdx.y / v.heads * 16;
+  const int head = blockIdx.y % v.heads, f0 = blockIdx.y / v.heads * kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const KvSequence s = kv_sequence(v, b);
   if (!s.ok) {
@@ -87,24 +107,85 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendAr
   if (f0 >= rows)
     return;
   const int offset = s.length - s.n; // position of the sequence's row 0
-  const int last = min(f0 + 15, rows - 1);
+  const int last = min(f0 + kRows, rows) - 1;
+  const int pos_first = offset + f0 / a.group, pos_last = offset + last / a.group;
   int lo, hi;
-  key_range(a, s.length, offset + f0 / a.group, offset + last / a.group, lo, hi);
+  key_range(a, s.length, pos_first, pos_last, lo, hi);
   const int first_group = lo >> 4, groups = ((hi + 15) >> 4) - first_group;
   const int each = (groups + a.splits - 1) / a.splits;
   const int begin = first_group + min(groups, split * each);
   const int end = first_group + min(groups, (split + 1) * each);
+  const int count = end > begin + warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;
 
-  // Query rows g and g + 8 as A fragments.
-  uint32_t qa[kParts][kCh * 4][4];
-  float coef[2];
-  int pos[2];
+  const uint32_t ring = smem_at(smem) + warp * kDepth * kStageBytes<kCh>;
+  const int per_page = v.block_log2 - 4; // log2 of the groups a page holds
+  // Lane i of a batch of 32 holds the page of the warp's i-th group.
+  auto pages_of = [&](int j0) {
+    const int j = j0 + lane;
+    int page = -1;
+    if (j < count) {
+      const int64_t group = begin + warp + static_cast<int64_t>(j) * kWarps;
+      page = kv_page(v, b, static_cast<int>(group >> per_page));
+      if (page < 0)
+        atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
+    }
+    return page;
+  };
+  // What a lane reads of a group; lanes past head_dim read nothing (their
+  // slots stay zero).
+  const int k_lane = g * v.dim + 16 * c, v_lane = 2 * c * v.dim + kLane * g;
+  const int64_t side = static_cast<int64_t>(v.dim) << v.block_log2;
+  bool k_in[kCh];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int f = f0 + g + 8 * r;
+  for (int ch = 0; ch < kCh; ++ch)
+    k_in[ch] = 64 * ch + 16 * c < v.dim;
+  const bool v_in = kLane * g < v.dim;
+  if (v.dim < 64 * kCh) {
+    for (int i = lane * 16; i < kDepth * kStageBytes<kCh>; i += 512)
+      *reinterpret_cast<uint4 *>(smem + warp * kDepth * kStageBytes<kCh> + i) = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  }
+  int batch_page = pages_of(0), next_page = pages_of(32);
+  auto issue = [&](int j, int stage) { // every lane copies its bytes of group j
+    if (j < count) {
+      const int page = __shfl_sync(0xffffffffu, (j & 32) == 0 ? batch_page : next_page, j & 31);
+      const int group = begin + warp + j * kWarps;
+      const int token = (group & ((1 << per_page) - 1)) << 4;
+      // A page out of range reads as page 0 (its keys are hidden below).
+      const int8_t *k = kv_codes(v, max(page, 0), head, 0) + token * v.dim;
+      const int8_t *values = k + side + v_lane;
+      const uint32_t slot = ring + stage * kStageBytes<kCh> + lane * 16;
+      k += k_lane;
+#pragma unroll
+      for (int ch = 0; ch < kCh; ++ch)
+        if (k_in[ch]) {
+          copy_async<16>(slot + ch * 512, k + 64 * ch);
+          copy_async<16>(slot + (kCh + ch) * 512, k + 8 * v.dim + 64 * ch);
+        }
+      if (v_in) {
+        const uint32_t to = ring + stage * kStageBytes<kCh> + 2 * kCh * 512 + lane * kLane;
+        copy_async<kLane>(to, values);
+        copy_async<kLane>(to + 32 * kLane, values + v.dim);
+        copy_async<kLane>(to + 64 * kLane, values + 8 * v.dim);
+        copy_async<kLane>(to + 96 * kLane, values + 9 * v.dim);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int j = 0; j < kDepth - 1; ++j)
+    issue(j, j);
+
+  // Query rows f0 + 8 t + g as B fragments (lane (g, c) holds the elements
+  // whose codes lane (., c) holds); results come out for rows 2c and 2c + 1.
+  uint32_t qb[kQ][kParts][kCh * 4][2];
+  float coef[kQ][2], start[kQ][2];
+  int pos[kQ][2];
+#pragma unroll
+  for (int t = 0; t < kQ; ++t) {
+    const int f = f0 + 8 * t + g;
     const bool live = f < rows;
     const int i = live ? f / a.group : 0;
-    pos[r] = live ? offset + i : -0x40000000; // a row past the tile sees nothing that counts
     const T *q = static_cast<const T *>(a.q) + (s.row0 + i) * a.q_row_stride +
                  (head * a.group + (live ? f - i * a.group : 0)) * a.q_head_stride;
     float x[kCh * 16];
@@ -117,113 +198,75 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendAr
 #pragma unroll
       for (int j = 0; j < kVec<T>; ++j) {
         x[e + j] = to_f32(p.at[j]);
-        const float m = fabsf(x[e + j]);
-        amax = nan_max(amax, m);
+        amax = nan_max(amax, fabsf(x[e + j]));
       }
     }
 #pragma unroll
-    for (int o = 1; o < 4; o *= 2) {
-      const float m = __shfl_xor_sync(0xffffffffu, amax, o);
-      amax = nan_max(amax, m);
-    }
-    float factor, inverse;
+    for (int o = 1; o < 4; o *= 2)
+      amax = nan_max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    float factor, inverse, sum = 0.0f;
     row_factor(amax, factor, inverse);
     // A row with NaN or infinity gives NaN wherever it sees a key.
-    coef[r] = amax < INFINITY ? inverse * a.scale_log2 : NAN;
+    const bool wild = !(amax < INFINITY);
+    const float mine = wild ? NAN : inverse * a.scale_log2;
 #pragma unroll
     for (int e = 0; e < kCh * 16; e += 2) {
-      const float y0 = x[e] * factor, y1 = x[e + 1] * factor;
+      const float y0 = wild ? 0.0f : x[e] * factor, y1 = wild ? 0.0f : x[e + 1] * factor;
       const uint32_t h = pack_half(y0, y1);
-      // Elements 4s .. 4s + 3 of a lane are columns 2c, 2c + 1, 2c + 8, 2c + 9.
-      qa[0][e / 4][(e & 2) + r] = h;
-      if constexpr (kParts == 2) {
-        const float2 back = unpack_half(h);
-        qa[1][e / 4][(e & 2) + r] = pack_half(y0 - back.x, y1 - back.y);
-      }
+      const float2 back = unpack_half(h);
+      sum += back.x + back.y;
+      // Elements 4x .. 4x + 3 of a lane are columns 2c, 2c + 1, 2c + 8, 2c + 9.
+      qb[t][0][e / 4][(e & 2) / 2] = h;
+      if constexpr (kParts == 2)
+        qb[t][1][e / 4][(e & 2) / 2] = pack_half(y0 - back.x, y1 - back.y);
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      coef[t][r] = __shfl_sync(0xffffffffu, mine, (2 * c + r) * 4);
+      // The raised keys add 1152 times the row's sum. Its roundings stay 30
+      // times below half a step of bf16 or f16 in the scores.
+      start[t][r] = kRaised ? -1152.0f * __shfl_sync(0xffffffffu, sum, (2 * c + r) * 4) : 0.0f;
+      const int fr = f0 + 8 * t + 2 * c + r;
+      pos[t][r] = fr < rows ? offset + fr / a.group : -0x40000000;
     }
   }
 
-  float o[kTiles][4];
+  float o[kQ][kTiles][4];
+  // l sums the probabilities as the product takes them (it comes from one more
+  // product, by ones), so that their rounding leaves the weights' sum at one;
+  // full sums them unrounded for the logarithm.
+  float m[kQ][2], l[kQ][2], full[kQ][2];
 #pragma unroll
-  for (int j = 0; j < kTiles; ++j)
-    o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-  // l sums the probabilities as the product takes them, so that their rounding
-  // leaves the weights' sum at one; full sums them unrounded for the logarithm.
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, full[2] = {0.0f, 0.0f};
-
-  const uint32_t ring = smem_at(smem) + warp * kStages * kStageBytes<kCh>;
-  const int count = end > begin + warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;
-  // Lane i of a batch of 32 holds what the warp needs of its i-th group.
-  int batch_page = -1, next_page = -1;
-  float batch_k = 0.0f, batch_log = 0.0f, batch_inv = 0.0f;
-  auto pages_of = [&](int j0) {
-    const int j = j0 + lane;
-    int page = -1;
-    if (j < count) {
-      const int64_t group = begin + warp + static_cast<int64_t>(j) * kWarps;
-      page = kv_page(v, b, static_cast<int>(group >> (v.block_log2 - 4)));
-      if (page < 0)
-        atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
-    }
-    return page;
-  };
-  auto issue = [&](int j) { // every lane copies its bytes of group j
-    if (j < count) {
-      const int page = __shfl_sync(0xffffffffu, (j & 32) == 0 ? batch_page : next_page, j & 31);
-      const int64_t group = begin + warp + static_cast<int64_t>(j) * kWarps;
-      const int token = static_cast<int>(group & ((1 << (v.block_log2 - 4)) - 1)) << 4;
-      const int8_t *k = kv_codes(v, max(page, 0), head, 0) + token * v.dim;
-      const int8_t *values = k + (static_cast<int64_t>(v.dim) << v.block_log2);
-      const uint32_t slot = ring + (j % kStages) * kStageBytes<kCh>;
+  for (int t = 0; t < kQ; ++t) {
+    m[t][0] = m[t][1] = kNone;
+    l[t][0] = l[t][1] = full[t][0] = full[t][1] = 0.0f;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int ch = 0; ch < kCh; ++ch) {
-          const int d = 64 * ch + 16 * c;
-          const bool in = page >= 0 && d < v.dim;
-          copy_async<16>(slot + (u * kCh + ch) * 512 + lane * 16,
-                         in ? k + (8 * u + g) * v.dim + d : v.codes, in);
-        }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int d = kLane * g;
-        const bool in = page >= 0 && d < v.dim;
-        copy_async<kLane>(slot + 2 * kCh * 512 + t * 32 * kLane + lane * kLane,
-                          in ? values + ((t & 1) + 2 * c + 8 * (t >> 1)) * v.dim + d : v.codes, in);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
+    for (int j = 0; j < kTiles; ++j)
+      o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.0f;
+  }
+  const bool want_full = kParts == 1 && a.lse != nullptr;
 
   // The pages of groups [64 i, 64 i + 32) are in batch_page, of the next 32 in
-  // next_page; each is refilled when its last group has been issued.
-  batch_page = pages_of(0);
-  next_page = pages_of(32);
-#pragma unroll 1
-  for (int j = 0; j < kStages - 1; ++j)
-    issue(j);
+  // next_page; each is refilled when its last group has been taken.
+  int stage = 0;
 #pragma unroll 1
   for (int j = 0; j < count; ++j) {
     if ((j & 31) == 0) { // scales of groups j .. j + 31 (their pages are still held)
       const int page = (j & 32) == 0 ? batch_page : next_page;
-      batch_k = batch_log = 0.0f;
-      batch_inv = 1.0f;
+      float4 k = make_float4(0.0f, 0.0f, 1.0f, 0.0f);
       if (page >= 0) {
         const float2 sc = *reinterpret_cast<const float2 *>(
             v.scales + (static_cast<int64_t>(page) * v.heads + head) * 2);
         const float sv = fmaxf(sc.y, kKvLeastScale);
-        batch_k = sc.x;
-        batch_log = log2f(sv);
-        batch_inv = 1.0f / sv;
+        k = make_float4(sc.x, log2f(sv), 1.0f / sv, 1.0f);
       }
+      __syncwarp();
+      constants[warp][lane] = k;
+      __syncwarp();
     }
-    const bool usable = __shfl_sync(0xffffffffu, (j & 32) == 0 ? batch_page : next_page, j & 31) >= 0;
-    issue(j + kStages - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-    const uint32_t slot = ring + (j % kStages) * kStageBytes<kCh>;
-    const float sk = __shfl_sync(0xffffffffu, batch_k, j & 31);
-    const float log_sv = __shfl_sync(0xffffffffu, batch_log, j & 31);
-    const float inv_sv = __shfl_sync(0xffffffffu, batch_inv, j & 31);
+    issue(j + kDepth - 1, stage == 0 ? kDepth - 1 : stage - 1);
     if ((j & 31) == 31) { // this batch's pages are no longer needed
       const int refill = pages_of(j + 33);
       if ((j & 32) == 0)
@@ -231,118 +274,139 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendAr
       else
         next_page = refill;
     }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    const uint32_t slot = ring + stage * kStageBytes<kCh> + lane * 16;
+    const uint32_t v_slot = ring + stage * kStageBytes<kCh> + 2 * kCh * 512 + lane * kLane;
+    stage = stage + 1 == kDepth ? 0 : stage + 1;
+    const float4 k = constants[warp][j & 31];
 
-    float sc[2][4];
+    float sc[kQ][4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      sc[u][0] = sc[u][1] = sc[u][2] = sc[u][3] = 0.0f;
+    for (int t = 0; t < kQ; ++t) {
+      sc[t][0] = sc[t][2] = start[t][0];
+      sc[t][1] = sc[t][3] = start[t][1];
+    }
 #pragma unroll
-      for (int ch = 0; ch < kCh; ++ch) {
-        uint32_t w[4];
+    for (int ch = 0; ch < kCh; ++ch) {
+      uint32_t w[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "r"(slot + (u * kCh + ch) * 512 + lane * 16)
+                     : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3])
+                     : "r"(slot + (u * kCh + ch) * 512)
                      : "memory");
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t b0, b1;
-          codes_to_half(w[x], b0, b1);
-          mma_f16(sc[u], qa[0][ch * 4 + x], b0, b1);
+      for (int x = 0; x < 4; ++x) {
+        uint32_t f[4];
+        if constexpr (kRaised) {
+          codes_to_half_raised(w[0][x], f[0], f[2]);
+          codes_to_half_raised(w[1][x], f[1], f[3]);
+        } else {
+          codes_to_half(w[0][x], f[0], f[2]);
+          codes_to_half(w[1][x], f[1], f[3]);
+        }
+#pragma unroll
+        for (int t = 0; t < kQ; ++t) {
           if constexpr (kParts == 2)
-            mma_f16(sc[u], qa[1][ch * 4 + x], b0, b1);
+            mma_f16(sc[t], f, qb[t][1][ch * 4 + x][0], qb[t][1][ch * 4 + x][1]);
+          mma_f16(sc[t], f, qb[t][0][ch * 4 + x][0], qb[t][0][ch * 4 + x][1]);
         }
       }
     }
-    // Exponents relative to the rows' references.
-    const int key0 = static_cast<int>((begin + warp + static_cast<int64_t>(j) * kWarps) << 4);
-    const bool whole = usable && key0 + 15 < s.length &&
-                       (!a.causal || key0 + 15 <= offset + f0 / a.group) &&
-                       (a.window <= 0 || key0 > offset + last / a.group - a.window);
-    uint32_t hidden = 0; // bit 4 u + e
-    if (!whole) {
+    // Exponents relative to the rows' references: element e of sc[t] is token
+    // g + 8 (e / 2) and row 2c + (e % 2).
+    const int key0 = (begin + warp + j * kWarps) << 4;
+    const bool whole = k.w != 0.0f && key0 + 15 < s.length &&
+                       (!a.causal || key0 + 15 <= pos_first) &&
+                       (a.window <= 0 || key0 > pos_last - a.window);
+    uint32_t pb[kQ][kParts][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int t = 0; t < kQ; ++t) {
+      uint32_t hidden = 0;
+      if (!whole) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (!usable || !sees(a, s.length, pos[e >> 1], key0 + 8 * u + 2 * c + (e & 1)))
-            hidden |= 1u << (4 * u + e);
-    }
-    float arg[2][4];
-    auto arguments = [&](int r) {
-      const float factor = coef[r] * sk, shift = log_sv - (m[r] == -INFINITY ? 0.0f : m[r]);
+          if (k.w == 0.0f || !sees(a, s.length, pos[t][e & 1], key0 + g + 8 * (e >> 1)))
+            hidden |= 1u << e;
+      }
+      float arg[4];
+      auto arguments = [&] {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int r = 0; r < 2; ++r) {
+          const float slope = coef[t][r] * k.x, shift = k.y - m[t][r];
+          arg[r] = fmaf(sc[t][r], slope, shift);
+          arg[r + 2] = fmaf(sc[t][r + 2], slope, shift);
+        }
+        if (!whole) {
 #pragma unroll
-        for (int e = 2 * r; e < 2 * r + 2; ++e)
-          arg[u][e] = hidden >> (4 * u + e) & 1 ? -INFINITY : fmaf(sc[u][e], factor, shift);
-    };
-    bool grown = false;
+          for (int e = 0; e < 4; ++e)
+            arg[e] = hidden >> e & 1 ? -INFINITY : arg[e];
+        }
+      };
+      arguments();
+      const float most = fmaxf(fmaxf(arg[0], arg[1]), fmaxf(arg[2], arg[3]));
+      if (__any_sync(0xffffffffu, most > kGrowth<kParts>)) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      arguments(r);
-      const float limit = m[r] == -INFINITY ? -INFINITY : kGrowth<kParts>;
+        for (int r = 0; r < 2; ++r) {
+          const float slope = coef[t][r] * k.x;
+          float top = fmaxf(hidden >> r & 1 ? -INFINITY : fmaf(sc[t][r], slope, k.y),
+                            hidden >> (r + 2) & 1 ? -INFINITY : fmaf(sc[t][r + 2], slope, k.y));
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+          for (int x = 4; x < 32; x *= 2)
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          const float to = top - kTop<kParts>;
+          if (to > m[t][r]) {
+            const float shrink = exp2_approx(m[t][r] - to); // 0 for the first
+            m[t][r] = to;
+            l[t][r] *= shrink;
+            full[t][r] *= shrink;
 #pragma unroll
-        for (int e = 2 * r; e < 2 * r + 2; ++e)
-          grown |= !(arg[u][e] <= limit); // NaN too
-    }
-    if (__any_sync(0xffffffffu, grown)) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float top = arg[0][2 * r];
-        top = nan_max(top, arg[0][2 * r + 1]);
-        top = nan_max(top, arg[1][2 * r]);
-        top = nan_max(top, arg[1][2 * r + 1]);
-#pragma unroll
-        for (int x = 1; x < 4; x *= 2)
-          top = nan_max(top, __shfl_xor_sync(0xffffffffu, top, x));
-        if (top != -INFINITY && (m[r] == -INFINITY || !(top <= kTop<kParts>))) {
-          const float to = (m[r] == -INFINITY ? 0.0f : m[r]) + top - kTop<kParts>;
-          const float shrink = exp2_approx(m[r] - to); // 0 for the first
-          m[r] = to;
-          l[r] *= shrink;
-          full[r] *= shrink;
-#pragma unroll
-          for (int j2 = 0; j2 < kTiles; ++j2) {
-            o[j2][2 * r] *= shrink;
-            o[j2][2 * r + 1] *= shrink;
+            for (int j2 = 0; j2 < kTiles; ++j2) {
+              o[t][j2][r] *= shrink;
+              o[t][j2][r + 2] *= shrink;
+            }
           }
-          arguments(r);
         }
+        arguments();
       }
-    }
-    uint32_t pa[kParts][4];
+      float p[4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int e = 0; e < 4; ++e)
+        p[e] = exp2_approx(arg[e]);
+      if (want_full) {
+        full[t][0] = fmaf(p[0] + p[2], k.z, full[t][0]);
+        full[t][1] = fmaf(p[1] + p[3], k.z, full[t][1]);
+      }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float p0 = exp2_approx(arg[u][2 * r]), p1 = exp2_approx(arg[u][2 * r + 1]);
-        const uint32_t h = pack_half(p0, p1);
-        const float2 back = unpack_half(h);
-        pa[0][2 * u + r] = h;
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t h = pack_half(p[2 * u], p[2 * u + 1]);
+        pb[t][0][u] = transpose8(h);
         if constexpr (kParts == 2) {
-          pa[1][2 * u + r] = pack_half(p0 - back.x, p1 - back.y);
-          l[r] = fmaf(p0 + p1, inv_sv, l[r]);
-        } else {
-          l[r] = fmaf(back.x + back.y, inv_sv, l[r]);
-          full[r] = fmaf(p0 + p1, inv_sv, full[r]);
+          const float2 back = unpack_half(h);
+          pb[t][1][u] = transpose8(pack_half(p[2 * u] - back.x, p[2 * u + 1] - back.y));
         }
       }
+      float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+      if constexpr (kParts == 2)
+        mma_f16(sums, ones, pb[t][1][0], pb[t][1][1]);
+      mma_f16(sums, ones, pb[t][0][0], pb[t][0][1]);
+      l[t][0] = fmaf(sums[0], k.z, l[t][0]);
+      l[t][1] = fmaf(sums[1], k.z, l[t][1]);
+    }
     // Values: pairs of tokens at one element.
     uint32_t w[4][2 * kCh];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const uint32_t at = slot + 2 * kCh * 512 + t * 32 * kLane + lane * kLane;
       if constexpr (kCh == 2)
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(w[t][0]), "=r"(w[t][1]), "=r"(w[t][2]), "=r"(w[t][3])
-                     : "r"(at)
+                     : "r"(v_slot + t * 32 * kLane)
                      : "memory");
       else
         asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
                      : "=r"(w[t][0]), "=r"(w[t][1])
-                     : "r"(at)
+                     : "r"(v_slot + t * 32 * kLane)
                      : "memory");
     }
 #pragma unroll
@@ -354,128 +418,170 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendAr
         codes_to_half(__byte_perm(w[2 * t][x], w[2 * t + 1][x], 0x7362), h[t][2], h[t][3]);
       }
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        if constexpr (kParts == 2) {
-          // The product's own accumulation does not round to nearest: over
-          // many groups in one accumulator that cost f32 outputs half their
-          // accuracy (1.2e-6 against 0.7e-6 relative at 1500 keys), so each
-          // group's products are added to the sum here.
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma_f16(part, pa[1], h[0][y], h[1][y]);
-          mma_f16(part, pa[0], h[0][y], h[1][y]);
+      for (int y = 0; y < 2; ++y) { // rows g and g + 8 are elements 4x + 2y and the next
+        const uint32_t f[4] = {h[0][2 * y], h[0][2 * y + 1], h[1][2 * y], h[1][2 * y + 1]};
 #pragma unroll
-          for (int z = 0; z < 4; ++z)
-            o[4 * x + y][z] += part[z];
-        } else {
-          mma_f16(o[4 * x + y], pa[0], h[0][y], h[1][y]);
+        for (int t = 0; t < kQ; ++t) {
+          if constexpr (kParts == 2) {
+            // The product's own accumulation does not round to nearest: over
+            // many groups in one accumulator that cost f32 outputs half their
+            // accuracy (1.2e-6 against 0.7e-6 relative at 1500 keys), so each
+            // group's products are added to the sum here.
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_f16(part, f, pb[t][1][0], pb[t][1][1]);
+            mma_f16(part, f, pb[t][0][0], pb[t][0][1]);
+#pragma unroll
+            for (int z = 0; z < 4; ++z)
+              o[t][2 * x + y][z] += part[z];
+          } else {
+            mma_f16(o[t][2 * x + y], f, pb[t][0][0], pb[t][0][1]);
+          }
         }
       }
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-#pragma unroll
-    for (int x = 1; x < 4; x *= 2) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
-      full[r] += __shfl_xor_sync(0xffffffffu, full[r], x);
-    }
 
-  // Join the warps: rows [warp][16][64 * kCh] in the ring's memory.
+  // Join the warps: rows [warp][kRows][64 * kCh] in the ring's memory.
   __syncthreads();
   float *joined = reinterpret_cast<float *>(smem);
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = g + 8 * r;
-    if (c == 0) {
-      row_m[warp][row] = m[r];
-      row_l[warp][row] = l[r];
-      row_e[warp][row] = kParts == 2 ? l[r] : full[r];
-    }
-    float *to = joined + (warp * 16 + row) * 64 * kCh;
+  for (int t = 0; t < kQ; ++t)
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      to[kTiles * (2 * c) + j] = o[j][2 * r];
-      to[kTiles * (2 * c + 1) + j] = o[j][2 * r + 1];
+    for (int r = 0; r < 2; ++r) {
+      const int row = 8 * t + 2 * c + r;
+      float e = full[t][r];
+#pragma unroll
+      for (int x = 4; x < 32; x *= 2)
+        e += __shfl_xor_sync(0xffffffffu, e, x);
+      if (g == 0) {
+        row_m[warp][row] = m[t][r];
+        row_l[warp][row] = l[t][r];
+        row_e[warp][row] = want_full ? e : l[t][r];
+      }
+      float2 *to = reinterpret_cast<float2 *>(joined + (warp * kRows + row) * 64 * kCh + kLane * g);
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+        to[j] = make_float2(o[t][j][r], o[t][j][r + 2]);
     }
-  }
   __syncthreads();
-  const int row = threadIdx.x >> 3, d = (threadIdx.x & 7) * kTiles;
+  constexpr int kEach = kCh * kQ == 1 ? 8 : 4 * kCh * kQ; // elements a thread joins
+  constexpr int kAcross = 64 * kCh / kEach;
+  const int row = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kEach;
   const int f = f0 + row;
-  if (f >= rows)
+  if (row >= kRows || f >= rows)
     return;
-  float top = -INFINITY;
+  float top = kNone;
 #pragma unroll
   for (int x = 0; x < kWarps; ++x)
-    top = nan_max(top, row_m[x][row]);
-  float sum = 0.0f, plain = 0.0f, acc[kTiles];
+    top = fmaxf(top, row_m[x][row]);
+  float sum = 0.0f, plain = 0.0f, acc[kEach];
 #pragma unroll
-  for (int j = 0; j < kTiles; ++j)
+  for (int j = 0; j < kEach; ++j)
     acc[j] = 0.0f;
 #pragma unroll
   for (int x = 0; x < kWarps; ++x) {
-    const float share = row_m[x][row] == -INFINITY ? 0.0f : exp2_approx(row_m[x][row] - top);
+    const float share = exp2_approx(row_m[x][row] - top);
     sum = fmaf(row_l[x][row], share, sum);
     plain = fmaf(row_e[x][row], share, plain);
-    if (share != 0.0f) {
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j)
-        acc[j] = fmaf(joined[(x * 16 + row) * 64 * kCh + d + j], share, acc[j]);
-    }
+    for (int j = 0; j < kEach; ++j)
+      acc[j] = fmaf(joined[(x * kRows + row) * 64 * kCh + d + j], share, acc[j]);
   }
   const int i = f / a.group;
   const int64_t at = (s.row0 + i) * a.q_heads + head * a.group + (f - i * a.group);
   if (a.splits > 1) {
-    const int64_t slot = static_cast<int64_t>(split) * v.rows * a.q_heads + at;
-    if ((threadIdx.x & 7) == 0)
-      a.part_ml[slot] = make_float4(top, sum, plain, 0.0f);
-    put_row(a.part_o + slot * v.dim, d, v.dim, acc);
+    const int64_t to = static_cast<int64_t>(split) * v.rows * a.q_heads + at;
+    if (d == 0)
+      a.part_ml[to] = make_float4(top, sum, plain, 0.0f);
+    put_row(a.part_o + to * v.dim, d, v.dim, acc);
     return;
   }
-  const bool some = top > -INFINITY || top != top;
+  const bool some = top > kNone || sum != sum;
   const float share = some ? 1.0f / sum : 0.0f;
 #pragma unroll
-  for (int j = 0; j < kTiles; ++j)
+  for (int j = 0; j < kEach; ++j)
     acc[j] *= share;
   put_row(static_cast<T *>(a.out) + at * v.dim, d, v.dim, acc);
-  if (a.lse && (threadIdx.x & 7) == 0)
+  if (a.lse && d == 0)
     a.lse[at] = some ? (top + log2f(plain)) * 0.69314718055994531f : -INFINITY;
 }
 
-// Joins the parts of the key axis: a warp a row and head.
+// Joins the parts of the key axis: a CTA a row and head, its warps take parts
+// in turn.
 template <typename T>
 __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
+  __shared__ float4 warp_ml[4];
+  __shared__ float4 warp_o[4][32];
   pdl_launch_dependents();
   pdl_wait();
   const KvView &v = a.v;
-  const int b = blockIdx.z, lane = threadIdx.x & 31;
+  const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const KvSequence s = kv_sequence(v, b);
-  const int64_t f = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int64_t f = blockIdx.x;
   if (!s.ok || f >= static_cast<int64_t>(s.n) * a.q_heads)
     return;
   const int64_t at = s.row0 * a.q_heads + f, step = v.rows * a.q_heads;
-  float top = -INFINITY;
-  for (int x = 0; x < a.splits; ++x) {
-    const float m = a.part_ml[x * step + at].x;
-    top = nan_max(top, m);
-  }
-  float sum = 0.0f, plain = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int x = 0; x < a.splits; ++x) {
-    const float4 ml = a.part_ml[x * step + at];
-    const float share = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - top);
-    if (share == 0.0f)
-      continue;
-    sum = fmaf(ml.y, share, sum);
-    plain = fmaf(ml.z, share, plain);
-    if (4 * lane < v.dim) {
-      const float4 p = *reinterpret_cast<const float4 *>(a.part_o + (x * step + at) * v.dim + 4 * lane);
-      acc[0] = fmaf(p.x, share, acc[0]);
-      acc[1] = fmaf(p.y, share, acc[1]);
-      acc[2] = fmaf(p.z, share, acc[2]);
-      acc[3] = fmaf(p.w, share, acc[3]);
+  float m = kNone, sum = 0.0f, plain = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int kAhead = 4;
+  for (int x0 = warp; x0 < a.splits; x0 += 4 * kAhead) {
+    float4 ml[kAhead], p[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t x = x0 + 4 * u;
+      ml[u] = make_float4(kNone, 0.0f, 0.0f, 0.0f);
+      p[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (x < a.splits) {
+        ml[u] = a.part_ml[x * step + at];
+        if (4 * lane < v.dim)
+          p[u] = *reinterpret_cast<const float4 *>(a.part_o + (x * step + at) * v.dim + 4 * lane);
+      }
+    }
+    float to = m;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      to = fmaxf(to, ml[u].x);
+    const float shrink = exp2_approx(m - to);
+    m = to;
+    sum *= shrink;
+    plain *= shrink;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      acc[e] *= shrink;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float share = exp2_approx(ml[u].x - m);
+      sum = fmaf(ml[u].y, share, sum);
+      plain = fmaf(ml[u].z, share, plain);
+      acc[0] = fmaf(p[u].x, share, acc[0]);
+      acc[1] = fmaf(p[u].y, share, acc[1]);
+      acc[2] = fmaf(p[u].z, share, acc[2]);
+      acc[3] = fmaf(p[u].w, share, acc[3]);
     }
   }
-  const bool some = top > -INFINITY || top != top;
+  if (lane == 0)
+    warp_ml[warp] = make_float4(m, sum, plain, 0.0f);
+  warp_o[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  if (warp > 0)
+    return;
+  float top = kNone;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    top = fmaxf(top, warp_ml[x].x);
+  sum = plain = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const float4 ml = warp_ml[x], p = warp_o[x][lane];
+    const float share = exp2_approx(ml.x - top);
+    sum = fmaf(ml.y, share, sum);
+    plain = fmaf(ml.z, share, plain);
+    acc[0] = fmaf(p.x, share, acc[0]);
+    acc[1] = fmaf(p.y, share, acc[1]);
+    acc[2] = fmaf(p.z, share, acc[2]);
+    acc[3] = fmaf(p.w, share, acc[3]);
+  }
+  const bool some = top > kNone || sum != sum;
   const float share = some ? 1.0f / sum : 0.0f;
   if (4 * lane < v.dim) {
     T *out = static_cast<T *>(a.out) + at * v.dim + 4 * lane;
@@ -487,17 +593,18 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
     a.lse[at] = some ? (top + log2f(plain)) * 0.69314718055994531f : -INFINITY;
 }
 
-// Parts of the key axis: enough work items for two resident CTAs an SM, each
-// part at least 256 keys.
-int decode_splits(const KvView &v, int64_t tiles, int64_t longest) {
+// Parts of the key axis: enough work items to fill the resident CTAs once,
+// each part at least 128 keys.
+int decode_splits(const KvView &v, int64_t tiles, int64_t longest, int resident) {
   const int64_t items = std::max<int64_t>(1, tiles * v.heads * v.batch);
-  const int64_t want = (2 * 148 + items - 1) / items;
-  return static_cast<int>(std::max<int64_t>(1, std::min({want, (longest + 255) / 256, int64_t{64}})));
+  const int64_t want = (148 * resident + items - 1) / items;
+  return static_cast<int>(std::max<int64_t>(1, std::min({want, (longest + 127) / 128, int64_t{256}})));
 }
 
 struct Plan {
   bool prompt; // by the tensor-memory kernel
   bool share;  // with one query tile a CTA
+  bool few;    // decode tiles of 8 query rows, not 16
   int splits;
   int64_t tiles;
   size_t bytes; // of the partial results
@@ -507,7 +614,7 @@ struct Plan {
 constexpr int64_t kDecodeRows = 32;
 
 Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
-  Plan p;
+  Plan p{};
   const int64_t group = t.q_heads / v.heads;
   const int64_t rows = std::min<int64_t>(v.most, v.rows) * group;
   const int64_t held = static_cast<int64_t>(v.table_width) << v.block_log2;
@@ -515,8 +622,10 @@ Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   p.prompt = rows > kDecodeRows;
   p.share = p.prompt && (t.type == CIM22_FLOAT32 || rows <= 128);
   if (!p.prompt) {
-    p.tiles = (rows + 15) / 16;
-    p.splits = decode_splits(v, p.tiles, longest);
+    p.few = rows <= 8;
+    p.tiles = (rows + (p.few ? 7 : 15)) / (p.few ? 8 : 16);
+    const int work = (t.type == CIM22_FLOAT32 ? 2 : 1) * (p.few ? 1 : 2);
+    p.splits = decode_splits(v, p.tiles, longest, work == 1 ? 4 : work == 2 ? 3 : 2);
   } else {
     p.tiles = (rows + (p.share ? 127 : 255)) / (p.share ? 128 : 256);
     const int64_t items = p.tiles * v.heads * v.batch;
@@ -550,10 +659,11 @@ bool attend_args(const char *what, const KvView &v, const cim22_kv_attention *t)
   return true;
 }
 
-template <typename T, int kCh, int kParts>
+template <typename T, int kCh, int kParts, int kQ>
 cudaError_t launch_decode(const KvAttendArgs &a, int64_t tiles, cudaStream_t stream) {
-  constexpr size_t bytes = static_cast<size_t>(kWarps) * kStages * kStageBytes<kCh>;
-  const auto kernel = kv_decode_kernel<T, kCh, kParts>;
+  constexpr size_t bytes =
+      static_cast<size_t>(kWarps) * kStages<kCh, kParts, kQ> * kStageBytes<kCh>;
+  const auto kernel = kv_decode_kernel<T, kCh, kParts, kQ>;
   static DynamicSmem allowed;
   if (const cudaError_t e = allowed.allow(kernel, bytes); e != cudaSuccess)
     return e;
@@ -563,13 +673,17 @@ cudaError_t launch_decode(const KvAttendArgs &a, int64_t tiles, cudaStream_t str
 
 template <typename T, int kParts>
 cudaError_t launch_attend(const KvAttendArgs &a, int type, const Plan &plan, cudaStream_t stream) {
-  cudaError_t e = plan.prompt ? kv_prompt_launch(a, type, plan.share, static_cast<int>(plan.tiles), stream)
-                  : a.v.dim > 64 ? launch_decode<T, 2, kParts>(a, plan.tiles, stream)
-                                 : launch_decode<T, 1, kParts>(a, plan.tiles, stream);
+  const bool wide = a.v.dim > 64;
+  cudaError_t e =
+      plan.prompt ? kv_prompt_launch(a, type, plan.share, static_cast<int>(plan.tiles), stream)
+      : plan.few  ? wide ? launch_decode<T, 2, kParts, 1>(a, plan.tiles, stream)
+                         : launch_decode<T, 1, kParts, 1>(a, plan.tiles, stream)
+      : wide      ? launch_decode<T, 2, kParts, 2>(a, plan.tiles, stream)
+                  : launch_decode<T, 1, kParts, 2>(a, plan.tiles, stream);
   if (e == cudaSuccess && a.splits > 1) {
     const int64_t rows = std::min<int64_t>(a.v.most, a.v.rows) * a.q_heads;
-    e = launch_pdl(kv_join_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4), 1, a.v.batch),
-                   dim3(128), 0, stream, a);
+    e = launch_pdl(kv_join_kernel<T>, dim3(static_cast<unsigned>(rows), 1, a.v.batch), dim3(128),
+                   0, stream, a);
   }
   return e;
 }

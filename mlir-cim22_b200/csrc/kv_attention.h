@@ -59,6 +59,8 @@ constexpr float kKvLeastScale = 0x1p-87f;
 // 2^kGrowth before it is set again. f16 (largest 65504, steps of 2^-24) then
 // holds every p to within 2^-11 of itself or 2^-31 of the largest; with two
 // parts (f32 queries), which set it again sooner, to within 2^-22 or 2^-38.
+// kNone: the reference of a row that has seen no key.
+constexpr float kNone = -1e30f;
 template <int kParts> constexpr float kTop = kParts == 2 ? 13.0f : 6.0f;
 template <int kParts> constexpr float kGrowth = kParts == 2 ? 15.0f : 14.0f;
 
