@@ -28,11 +28,12 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 
-// CTAs an SM by the registers that query tiles and parts take, and the depth
-// of the copies that then fits in shared memory.
-template <int kParts, int kQ> constexpr int kResident = kParts * kQ == 1 ? 4 : kParts * kQ == 2 ? 3 : 2;
-template <int kCh> constexpr int kStageBytes = 16 * 2 * 64 * kCh; // one group of one warp
-template <int kCh, int kParts, int kQ> constexpr int kStages = 24 / (kResident<kParts, kQ> * kCh);
+// CTAs an SM by the registers that query tiles and parts take, the groups that
+// a warp then has in its ring, and how many it takes at a time.
+template <int kParts, int kQ> constexpr int kResident = kParts * kQ == 4 ? 2 : 3;
+template <int kCh> constexpr int kGroupBytes = 16 * 2 * 64 * kCh;
+template <int kCh, int kParts, int kQ> constexpr int kRing = 24 / (kResident<kParts, kQ> * kCh);
+template <int kParts, int kQ> constexpr int kTake = kParts * kQ == 1 ? 2 : 1;
 
 __device__ __forceinline__ uint32_t smem_at(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -80,20 +81,23 @@ __device__ __forceinline__ void put_row(T *out, int d, int dim, const float (&v)
   }
 }
 
-template <typename T, int kCh, int kParts, int kQ>
+template <typename T, int kCh, int kParts, int kQ, bool kExact>
 __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     kv_decode_kernel(const KvAttendArgs a) {
   constexpr int kTiles = 4 * kCh;  // 16-element tiles of the head
   constexpr int kLane = 8 * kCh;   // value bytes a lane holds of a token
-  constexpr int kDepth = kStages<kCh, kParts, kQ>;
+  constexpr int kG = kTake<kParts, kQ>; // groups a round
+  constexpr int kRounds = kRing<kCh, kParts, kQ> / kG; // rounds in the ring
+  constexpr int kBytes = kGroupBytes<kCh>;
   constexpr int kRows = 8 * kQ;
   constexpr bool kRaised = kParts == 1; // keys enter with 1152 added
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float row_m[kWarps][kRows], row_l[kWarps][kRows], row_e[kWarps][kRows];
+  __shared__ float row_m[kWarps][kRows], row_l[kWarps][kRows];
   __shared__ float4 constants[kWarps][32];
   pdl_launch_dependents();
   pdl_wait();
   const KvView &v = a.v;
+  const int dim = kExact ? 64 * kCh : v.dim;
   const int b = blockIdx.z, split = blockIdx.x;
   const int head = blockIdx.y % v.heads, f0 = blockIdx.y / v.heads * kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -113,67 +117,72 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   key_range(a, s.length, pos_first, pos_last, lo, hi);
   const int first_group = lo >> 4, groups = ((hi + 15) >> 4) - first_group;
   const int each = (groups + a.splits - 1) / a.splits;
-  const int begin = first_group + min(groups, split * each);
+  const int begin = first_group + min(groups, split * each) + kG * warp;
   const int end = first_group + min(groups, (split + 1) * each);
-  const int count = end > begin + warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;
+  // The warp's i-th group is begin + (i / kG) * kG * kWarps + i % kG; the last
+  // round may run past `end` (its groups are then hidden).
+  const int count = end > begin ? (end - begin + kG * kWarps - 1) / (kG * kWarps) : 0; // rounds
 
-  const uint32_t ring = smem_at(smem) + warp * kDepth * kStageBytes<kCh>;
+  const uint32_t ring = smem_at(smem) + warp * kRounds * kG * kBytes;
   const int per_page = v.block_log2 - 4; // log2 of the groups a page holds
-  // Lane i of a batch of 32 holds the page of the warp's i-th group.
-  auto pages_of = [&](int j0) {
-    const int j = j0 + lane;
-    int page = -1;
-    if (j < count) {
-      const int64_t group = begin + warp + static_cast<int64_t>(j) * kWarps;
-      page = kv_page(v, b, static_cast<int>(group >> per_page));
+  // Lane i of a batch of 32 groups holds where the warp's i-th group begins, in
+  // units of a group's keys; -1 where there is none.
+  auto places_of = [&](int i0) {
+    const int i = i0 + lane;
+    const int group = begin + i / kG * (kG * kWarps) + i % kG;
+    int place = -1;
+    if (i < count * kG && group < end) {
+      const int page = kv_page(v, b, group >> per_page);
       if (page < 0)
         atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
+      else
+        place = (((page * v.heads + head) * 2) << per_page) + (group & ((1 << per_page) - 1));
     }
-    return page;
+    return place;
   };
   // What a lane reads of a group; lanes past head_dim read nothing (their
   // slots stay zero).
-  const int k_lane = g * v.dim + 16 * c, v_lane = 2 * c * v.dim + kLane * g;
-  const int64_t side = static_cast<int64_t>(v.dim) << v.block_log2;
+  const int k_lane = g * dim + 16 * c, v_lane = (dim << v.block_log2) + 2 * c * dim + kLane * g;
   bool k_in[kCh];
 #pragma unroll
   for (int ch = 0; ch < kCh; ++ch)
-    k_in[ch] = 64 * ch + 16 * c < v.dim;
-  const bool v_in = kLane * g < v.dim;
-  if (v.dim < 64 * kCh) {
-    for (int i = lane * 16; i < kDepth * kStageBytes<kCh>; i += 512)
-      *reinterpret_cast<uint4 *>(smem + warp * kDepth * kStageBytes<kCh> + i) = make_uint4(0, 0, 0, 0);
+    k_in[ch] = kExact || 64 * ch + 16 * c < dim;
+  const bool v_in = kExact || kLane * g < dim;
+  if (!kExact) {
+    for (int i = lane * 16; i < kRounds * kG * kBytes; i += 512)
+      *reinterpret_cast<uint4 *>(smem + warp * kRounds * kG * kBytes + i) = make_uint4(0, 0, 0, 0);
     __syncwarp();
   }
-  int batch_page = pages_of(0), next_page = pages_of(32);
-  auto issue = [&](int j, int stage) { // every lane copies its bytes of group j
+  int batch_place = places_of(0), next_place = places_of(32);
+  auto issue = [&](int j, int round) { // every lane copies its bytes of round j
     if (j < count) {
-      const int page = __shfl_sync(0xffffffffu, (j & 32) == 0 ? batch_page : next_page, j & 31);
-      const int group = begin + warp + j * kWarps;
-      const int token = (group & ((1 << per_page) - 1)) << 4;
-      // A page out of range reads as page 0 (its keys are hidden below).
-      const int8_t *k = kv_codes(v, max(page, 0), head, 0) + token * v.dim;
-      const int8_t *values = k + side + v_lane;
-      const uint32_t slot = ring + stage * kStageBytes<kCh> + lane * 16;
-      k += k_lane;
 #pragma unroll
-      for (int ch = 0; ch < kCh; ++ch)
-        if (k_in[ch]) {
-          copy_async<16>(slot + ch * 512, k + 64 * ch);
-          copy_async<16>(slot + (kCh + ch) * 512, k + 8 * v.dim + 64 * ch);
+      for (int u = 0; u < kG; ++u) {
+        const int i = j * kG + u;
+        const int place = __shfl_sync(0xffffffffu, (i & 32) == 0 ? batch_place : next_place, i & 31);
+        // Groups without a place read as place 0 (their keys are hidden below).
+        const int8_t *at = v.codes + static_cast<int64_t>(max(place, 0)) * (16 * dim);
+        const int8_t *k = at + k_lane, *values = at + v_lane;
+        const uint32_t slot = ring + (round * kG + u) * kBytes + lane * 16;
+#pragma unroll
+        for (int ch = 0; ch < kCh; ++ch)
+          if (k_in[ch]) {
+            copy_async<16>(slot + ch * 512, k + 64 * ch);
+            copy_async<16>(slot + (kCh + ch) * 512, k + 8 * dim + 64 * ch);
+          }
+        if (v_in) {
+          const uint32_t to = ring + (round * kG + u) * kBytes + 2 * kCh * 512 + lane * kLane;
+          copy_async<kLane>(to, values);
+          copy_async<kLane>(to + 32 * kLane, values + dim);
+          copy_async<kLane>(to + 64 * kLane, values + 8 * dim);
+          copy_async<kLane>(to + 96 * kLane, values + 9 * dim);
         }
-      if (v_in) {
-        const uint32_t to = ring + stage * kStageBytes<kCh> + 2 * kCh * 512 + lane * kLane;
-        copy_async<kLane>(to, values);
-        copy_async<kLane>(to + 32 * kLane, values + v.dim);
-        copy_async<kLane>(to + 64 * kLane, values + 8 * v.dim);
-        copy_async<kLane>(to + 96 * kLane, values + 9 * v.dim);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll 1
-  for (int j = 0; j < kDepth - 1; ++j)
+  for (int j = 0; j < kRounds - 1; ++j)
     issue(j, j);
 
   // Query rows f0 + 8 t + g as B fragments (lane (g, c) holds the elements
@@ -194,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     for (int e = 0; e < kCh * 16; e += kVec<T>) {
       Pack<T> p;
       if (live)
-        p = load_pack(q, (e / 16) * 64 + 16 * c + e % 16, v.dim);
+        p = load_pack(q, (e / 16) * 64 + 16 * c + e % 16, dim);
 #pragma unroll
       for (int j = 0; j < kVec<T>; ++j) {
         x[e + j] = to_f32(p.at[j]);
@@ -234,31 +243,29 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   }
 
   float o[kQ][kTiles][4];
-  // l sums the probabilities as the product takes them (it comes from one more
-  // product, by ones), so that their rounding leaves the weights' sum at one;
-  // full sums them unrounded for the logarithm.
-  float m[kQ][2], l[kQ][2], full[kQ][2];
+  // l sums the lane's own tokens. It takes the probabilities unrounded: where
+  // value scales differ, what f16 keeps of a small one is not its weight.
+  float m[kQ][2], l[kQ][2];
 #pragma unroll
   for (int t = 0; t < kQ; ++t) {
     m[t][0] = m[t][1] = kNone;
-    l[t][0] = l[t][1] = full[t][0] = full[t][1] = 0.0f;
+    l[t][0] = l[t][1] = 0.0f;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j)
       o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.0f;
   }
-  const bool want_full = kParts == 1 && a.lse != nullptr;
-
-  // The pages of groups [64 i, 64 i + 32) are in batch_page, of the next 32 in
-  // next_page; each is refilled when its last group has been taken.
-  int stage = 0;
+  // The places of groups [64 i, 64 i + 32) are in batch_place, of the next 32
+  // in next_place; each is refilled when its last group has been taken.
+  int round = 0;
 #pragma unroll 1
   for (int j = 0; j < count; ++j) {
-    if ((j & 31) == 0) { // scales of groups j .. j + 31 (their pages are still held)
-      const int page = (j & 32) == 0 ? batch_page : next_page;
-      float4 k = make_float4(0.0f, 0.0f, 1.0f, 0.0f);
-      if (page >= 0) {
-        const float2 sc = *reinterpret_cast<const float2 *>(
-            v.scales + (static_cast<int64_t>(page) * v.heads + head) * 2);
+    const int i0 = j * kG;
+    if ((i0 & 31) == 0) { // scales of groups i0 .. i0 + 31 (their places are still held)
+      const int place = (i0 & 32) == 0 ? batch_place : next_place;
+      float4 k = make_float4(0.0f, 0.0f, 1.0f, 0.0f); // hidden
+      if (place >= 0) {
+        // (page * heads + head) * 2 floats into the scales.
+        const float2 sc = reinterpret_cast<const float2 *>(v.scales)[place >> (per_page + 1)];
         const float sv = fmaxf(sc.y, kKvLeastScale);
         k = make_float4(sc.x, log2f(sv), 1.0f / sv, 1.0f);
       }
@@ -266,91 +273,118 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
       constants[warp][lane] = k;
       __syncwarp();
     }
-    issue(j + kDepth - 1, stage == 0 ? kDepth - 1 : stage - 1);
-    if ((j & 31) == 31) { // this batch's pages are no longer needed
-      const int refill = pages_of(j + 33);
-      if ((j & 32) == 0)
-        batch_page = refill;
+    issue(j + kRounds - 1, round == 0 ? kRounds - 1 : round - 1);
+    if (((i0 + kG) & 31) == 0) { // this batch's places are no longer needed
+      const int refill = places_of(i0 + kG + 32);
+      if ((i0 & 32) == 0)
+        batch_place = refill;
       else
-        next_page = refill;
+        next_place = refill;
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-    const uint32_t slot = ring + stage * kStageBytes<kCh> + lane * 16;
-    const uint32_t v_slot = ring + stage * kStageBytes<kCh> + 2 * kCh * 512 + lane * kLane;
-    stage = stage + 1 == kDepth ? 0 : stage + 1;
-    const float4 k = constants[warp][j & 31];
-
-    float sc[kQ][4];
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRounds - 1) : "memory");
+    const uint32_t slot = ring + round * kG * kBytes + lane * 16;
+    const uint32_t v_slot = ring + round * kG * kBytes + 2 * kCh * 512 + lane * kLane;
+    round = round + 1 == kRounds ? 0 : round + 1;
+    float4 k[kG];
 #pragma unroll
-    for (int t = 0; t < kQ; ++t) {
-      sc[t][0] = sc[t][2] = start[t][0];
-      sc[t][1] = sc[t][3] = start[t][1];
-    }
+    for (int u = 0; u < kG; ++u)
+      k[u] = constants[warp][(i0 + u) & 31];
+
+    float sc[kG][kQ][4];
+#pragma unroll
+    for (int u = 0; u < kG; ++u)
+#pragma unroll
+      for (int t = 0; t < kQ; ++t) {
+        sc[u][t][0] = sc[u][t][2] = start[t][0];
+        sc[u][t][1] = sc[u][t][3] = start[t][1];
+      }
 #pragma unroll
     for (int ch = 0; ch < kCh; ++ch) {
-      uint32_t w[2][4];
+      uint32_t w[kG][2][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3])
-                     : "r"(slot + (u * kCh + ch) * 512)
-                     : "memory");
+      for (int u = 0; u < kG; ++u)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        uint32_t f[4];
-        if constexpr (kRaised) {
-          codes_to_half_raised(w[0][x], f[0], f[2]);
-          codes_to_half_raised(w[1][x], f[1], f[3]);
-        } else {
-          codes_to_half(w[0][x], f[0], f[2]);
-          codes_to_half(w[1][x], f[1], f[3]);
+        for (int z = 0; z < 2; ++z)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[u][z][0]), "=r"(w[u][z][1]), "=r"(w[u][z][2]), "=r"(w[u][z][3])
+                       : "r"(slot + u * kBytes + (z * kCh + ch) * 512)
+                       : "memory");
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int u = 0; u < kG; ++u) {
+          uint32_t f[4];
+          if constexpr (kRaised) {
+            codes_to_half_raised(w[u][0][x], f[0], f[2]);
+            codes_to_half_raised(w[u][1][x], f[1], f[3]);
+          } else {
+            codes_to_half(w[u][0][x], f[0], f[2]);
+            codes_to_half(w[u][1][x], f[1], f[3]);
+          }
+#pragma unroll
+          for (int t = 0; t < kQ; ++t) {
+            if constexpr (kParts == 2)
+              mma_f16(sc[u][t], f, qb[t][1][ch * 4 + x][0], qb[t][1][ch * 4 + x][1]);
+            mma_f16(sc[u][t], f, qb[t][0][ch * 4 + x][0], qb[t][0][ch * 4 + x][1]);
+          }
         }
-#pragma unroll
-        for (int t = 0; t < kQ; ++t) {
-          if constexpr (kParts == 2)
-            mma_f16(sc[t], f, qb[t][1][ch * 4 + x][0], qb[t][1][ch * 4 + x][1]);
-          mma_f16(sc[t], f, qb[t][0][ch * 4 + x][0], qb[t][0][ch * 4 + x][1]);
-        }
-      }
     }
-    // Exponents relative to the rows' references: element e of sc[t] is token
-    // g + 8 (e / 2) and row 2c + (e % 2).
-    const int key0 = (begin + warp + j * kWarps) << 4;
-    const bool whole = k.w != 0.0f && key0 + 15 < s.length &&
-                       (!a.causal || key0 + 15 <= pos_first) &&
-                       (a.window <= 0 || key0 > pos_last - a.window);
-    uint32_t pb[kQ][kParts][2];
+    // Exponents relative to the rows' references: element e of sc is token
+    // g + 8 (e / 2) of its group and row 2c + (e % 2).
+    const int key0 = (begin + j * (kG * kWarps)) << 4;
+    bool whole = key0 + 16 * kG - 1 < s.length &&
+                 (!a.causal || key0 + 16 * kG - 1 <= pos_first) &&
+                 (a.window <= 0 || key0 > pos_last - a.window);
+#pragma unroll
+    for (int u = 0; u < kG; ++u)
+      whole &= k[u].w != 0.0f;
+    uint32_t pb[kG][kQ][kParts][2];
 #pragma unroll
     for (int t = 0; t < kQ; ++t) {
       uint32_t hidden = 0;
       if (!whole) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (k.w == 0.0f || !sees(a, s.length, pos[t][e & 1], key0 + g + 8 * (e >> 1)))
-            hidden |= 1u << e;
-      }
-      float arg[4];
-      auto arguments = [&] {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float slope = coef[t][r] * k.x, shift = k.y - m[t][r];
-          arg[r] = fmaf(sc[t][r], slope, shift);
-          arg[r + 2] = fmaf(sc[t][r + 2], slope, shift);
-        }
-        if (!whole) {
+        for (int u = 0; u < kG; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            arg[e] = hidden >> e & 1 ? -INFINITY : arg[e];
+            if (k[u].w == 0.0f || !sees(a, s.length, pos[t][e & 1], key0 + 16 * u + g + 8 * (e >> 1)))
+              hidden |= 1u << (4 * u + e);
+      }
+      float arg[kG][4];
+      auto arguments = [&] {
+#pragma unroll
+        for (int u = 0; u < kG; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float slope = coef[t][r] * k[u].x, shift = k[u].y - m[t][r];
+            arg[u][r] = fmaf(sc[u][t][r], slope, shift);
+            arg[u][r + 2] = fmaf(sc[u][t][r + 2], slope, shift);
+          }
+        if (!whole) {
+#pragma unroll
+          for (int u = 0; u < kG; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              arg[u][e] = hidden >> (4 * u + e) & 1 ? -INFINITY : arg[u][e];
         }
       };
       arguments();
-      const float most = fmaxf(fmaxf(arg[0], arg[1]), fmaxf(arg[2], arg[3]));
+      float most = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kG; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          most = fmaxf(most, arg[u][e]);
       if (__any_sync(0xffffffffu, most > kGrowth<kParts>)) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float slope = coef[t][r] * k.x;
-          float top = fmaxf(hidden >> r & 1 ? -INFINITY : fmaf(sc[t][r], slope, k.y),
-                            hidden >> (r + 2) & 1 ? -INFINITY : fmaf(sc[t][r + 2], slope, k.y));
+          float top = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < kG; ++u)
+#pragma unroll
+            for (int e = r; e < 4; e += 2)
+              if (!(hidden >> (4 * u + e) & 1))
+                top = fmaxf(top, fmaf(sc[u][t][e], coef[t][r] * k[u].x, k[u].y));
 #pragma unroll
           for (int x = 4; x < 32; x *= 2)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
@@ -359,7 +393,6 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
             const float shrink = exp2_approx(m[t][r] - to); // 0 for the first
             m[t][r] = to;
             l[t][r] *= shrink;
-            full[t][r] *= shrink;
 #pragma unroll
             for (int j2 = 0; j2 < kTiles; ++j2) {
               o[t][j2][r] *= shrink;
@@ -369,72 +402,69 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
         }
         arguments();
       }
-      float p[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        p[e] = exp2_approx(arg[e]);
-      if (want_full) {
-        full[t][0] = fmaf(p[0] + p[2], k.z, full[t][0]);
-        full[t][1] = fmaf(p[1] + p[3], k.z, full[t][1]);
-      }
+      for (int u = 0; u < kG; ++u) {
+        float p[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t h = pack_half(p[2 * u], p[2 * u + 1]);
-        pb[t][0][u] = transpose8(h);
-        if constexpr (kParts == 2) {
-          const float2 back = unpack_half(h);
-          pb[t][1][u] = transpose8(pack_half(p[2 * u] - back.x, p[2 * u + 1] - back.y));
+        for (int e = 0; e < 4; ++e)
+          p[e] = exp2_approx(arg[u][e]);
+        l[t][0] = fmaf(p[0] + p[2], k[u].z, l[t][0]);
+        l[t][1] = fmaf(p[1] + p[3], k[u].z, l[t][1]);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const uint32_t h = pack_half(p[2 * z], p[2 * z + 1]);
+          pb[u][t][0][z] = transpose8(h);
+          if constexpr (kParts == 2) {
+            const float2 back = unpack_half(h);
+            pb[u][t][1][z] = transpose8(pack_half(p[2 * z] - back.x, p[2 * z + 1] - back.y));
+          }
         }
       }
-      float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-      if constexpr (kParts == 2)
-        mma_f16(sums, ones, pb[t][1][0], pb[t][1][1]);
-      mma_f16(sums, ones, pb[t][0][0], pb[t][0][1]);
-      l[t][0] = fmaf(sums[0], k.z, l[t][0]);
-      l[t][1] = fmaf(sums[1], k.z, l[t][1]);
     }
     // Values: pairs of tokens at one element.
-    uint32_t w[4][2 * kCh];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if constexpr (kCh == 2)
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[t][0]), "=r"(w[t][1]), "=r"(w[t][2]), "=r"(w[t][3])
-                     : "r"(v_slot + t * 32 * kLane)
-                     : "memory");
-      else
-        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                     : "=r"(w[t][0]), "=r"(w[t][1])
-                     : "r"(v_slot + t * 32 * kLane)
-                     : "memory");
-    }
+    for (int u = 0; u < kG; ++u) {
+      uint32_t w[4][2 * kCh];
 #pragma unroll
-    for (int x = 0; x < 2 * kCh; ++x) {
-      uint32_t h[2][4]; // token pair, element
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        codes_to_half(__byte_perm(w[2 * t][x], w[2 * t + 1][x], 0x5140), h[t][0], h[t][1]);
-        codes_to_half(__byte_perm(w[2 * t][x], w[2 * t + 1][x], 0x7362), h[t][2], h[t][3]);
+      for (int t = 0; t < 4; ++t) {
+        if constexpr (kCh == 2)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[t][0]), "=r"(w[t][1]), "=r"(w[t][2]), "=r"(w[t][3])
+                       : "r"(v_slot + u * kBytes + t * 32 * kLane)
+                       : "memory");
+        else
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                       : "=r"(w[t][0]), "=r"(w[t][1])
+                       : "r"(v_slot + u * kBytes + t * 32 * kLane)
+                       : "memory");
       }
 #pragma unroll
-      for (int y = 0; y < 2; ++y) { // rows g and g + 8 are elements 4x + 2y and the next
-        const uint32_t f[4] = {h[0][2 * y], h[0][2 * y + 1], h[1][2 * y], h[1][2 * y + 1]};
+      for (int x = 0; x < 2 * kCh; ++x) {
+        uint32_t h[2][4]; // token pair, element
 #pragma unroll
-        for (int t = 0; t < kQ; ++t) {
-          if constexpr (kParts == 2) {
-            // The product's own accumulation does not round to nearest: over
-            // many groups in one accumulator that cost f32 outputs half their
-            // accuracy (1.2e-6 against 0.7e-6 relative at 1500 keys), so each
-            // group's products are added to the sum here.
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_f16(part, f, pb[t][1][0], pb[t][1][1]);
-            mma_f16(part, f, pb[t][0][0], pb[t][0][1]);
+        for (int t = 0; t < 2; ++t) {
+          codes_to_half(__byte_perm(w[2 * t][x], w[2 * t + 1][x], 0x5140), h[t][0], h[t][1]);
+          codes_to_half(__byte_perm(w[2 * t][x], w[2 * t + 1][x], 0x7362), h[t][2], h[t][3]);
+        }
 #pragma unroll
-            for (int z = 0; z < 4; ++z)
-              o[t][2 * x + y][z] += part[z];
-          } else {
-            mma_f16(o[t][2 * x + y], f, pb[t][0][0], pb[t][0][1]);
+        for (int y = 0; y < 2; ++y) { // rows g and g + 8 are elements 4x + 2y and the next
+          const uint32_t f[4] = {h[0][2 * y], h[0][2 * y + 1], h[1][2 * y], h[1][2 * y + 1]};
+#pragma unroll
+          for (int t = 0; t < kQ; ++t) {
+            if constexpr (kParts == 2) {
+              // The product's own accumulation does not round to nearest: over
+              // many groups in one accumulator that cost f32 outputs half their
+              // accuracy (1.2e-6 against 0.7e-6 relative at 1500 keys), so each
+              // group's products are added to the sum here.
+              float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma_f16(part, f, pb[u][t][1][0], pb[u][t][1][1]);
+              mma_f16(part, f, pb[u][t][0][0], pb[u][t][0][1]);
+#pragma unroll
+              for (int z = 0; z < 4; ++z)
+                o[t][2 * x + y][z] += part[z];
+            } else {
+              mma_f16(o[t][2 * x + y], f, pb[u][t][0][0], pb[u][t][0][1]);
+            }
           }
         }
       }
@@ -450,14 +480,12 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = 8 * t + 2 * c + r;
-      float e = full[t][r];
 #pragma unroll
       for (int x = 4; x < 32; x *= 2)
-        e += __shfl_xor_sync(0xffffffffu, e, x);
+        l[t][r] += __shfl_xor_sync(0xffffffffu, l[t][r], x);
       if (g == 0) {
         row_m[warp][row] = m[t][r];
         row_l[warp][row] = l[t][r];
-        row_e[warp][row] = want_full ? e : l[t][r];
       }
       float2 *to = reinterpret_cast<float2 *>(joined + (warp * kRows + row) * 64 * kCh + kLane * g);
 #pragma unroll
@@ -475,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
 #pragma unroll
   for (int x = 0; x < kWarps; ++x)
     top = fmaxf(top, row_m[x][row]);
-  float sum = 0.0f, plain = 0.0f, acc[kEach];
+  float sum = 0.0f, acc[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; ++j)
     acc[j] = 0.0f;
@@ -483,7 +511,6 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   for (int x = 0; x < kWarps; ++x) {
     const float share = exp2_approx(row_m[x][row] - top);
     sum = fmaf(row_l[x][row], share, sum);
-    plain = fmaf(row_e[x][row], share, plain);
 #pragma unroll
     for (int j = 0; j < kEach; ++j)
       acc[j] = fmaf(joined[(x * kRows + row) * 64 * kCh + d + j], share, acc[j]);
@@ -493,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   if (a.splits > 1) {
     const int64_t to = static_cast<int64_t>(split) * v.rows * a.q_heads + at;
     if (d == 0)
-      a.part_ml[to] = make_float4(top, sum, plain, 0.0f);
+      a.part_ml[to] = make_float2(top, sum);
     put_row(a.part_o + to * v.dim, d, v.dim, acc);
     return;
   }
@@ -504,14 +531,14 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     acc[j] *= share;
   put_row(static_cast<T *>(a.out) + at * v.dim, d, v.dim, acc);
   if (a.lse && d == 0)
-    a.lse[at] = some ? (top + log2f(plain)) * 0.69314718055994531f : -INFINITY;
+    a.lse[at] = some ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
 }
 
 // Joins the parts of the key axis: a CTA a row and head, its warps take parts
 // in turn.
 template <typename T>
 __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
-  __shared__ float4 warp_ml[4];
+  __shared__ float2 warp_ml[4];
   __shared__ float4 warp_o[4][32];
   pdl_launch_dependents();
   pdl_wait();
@@ -522,14 +549,15 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
   if (!s.ok || f >= static_cast<int64_t>(s.n) * a.q_heads)
     return;
   const int64_t at = s.row0 * a.q_heads + f, step = v.rows * a.q_heads;
-  float m = kNone, sum = 0.0f, plain = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float m = kNone, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int kAhead = 4;
   for (int x0 = warp; x0 < a.splits; x0 += 4 * kAhead) {
-    float4 ml[kAhead], p[kAhead];
+    float2 ml[kAhead];
+    float4 p[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int64_t x = x0 + 4 * u;
-      ml[u] = make_float4(kNone, 0.0f, 0.0f, 0.0f);
+      ml[u] = make_float2(kNone, 0.0f);
       p[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (x < a.splits) {
         ml[u] = a.part_ml[x * step + at];
@@ -544,7 +572,6 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
     const float shrink = exp2_approx(m - to);
     m = to;
     sum *= shrink;
-    plain *= shrink;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       acc[e] *= shrink;
@@ -552,7 +579,6 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
     for (int u = 0; u < kAhead; ++u) {
       const float share = exp2_approx(ml[u].x - m);
       sum = fmaf(ml[u].y, share, sum);
-      plain = fmaf(ml[u].z, share, plain);
       acc[0] = fmaf(p[u].x, share, acc[0]);
       acc[1] = fmaf(p[u].y, share, acc[1]);
       acc[2] = fmaf(p[u].z, share, acc[2]);
@@ -560,7 +586,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
     }
   }
   if (lane == 0)
-    warp_ml[warp] = make_float4(m, sum, plain, 0.0f);
+    warp_ml[warp] = make_float2(m, sum);
   warp_o[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   __syncthreads();
   if (warp > 0)
@@ -569,13 +595,13 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
 #pragma unroll
   for (int x = 0; x < 4; ++x)
     top = fmaxf(top, warp_ml[x].x);
-  sum = plain = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+  sum = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    const float4 ml = warp_ml[x], p = warp_o[x][lane];
+    const float2 ml = warp_ml[x];
+    const float4 p = warp_o[x][lane];
     const float share = exp2_approx(ml.x - top);
     sum = fmaf(ml.y, share, sum);
-    plain = fmaf(ml.z, share, plain);
     acc[0] = fmaf(p.x, share, acc[0]);
     acc[1] = fmaf(p.y, share, acc[1]);
     acc[2] = fmaf(p.z, share, acc[2]);
@@ -590,15 +616,14 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
       out[j] = from_f32<T>(acc[j] * share);
   }
   if (a.lse && lane == 0)
-    a.lse[at] = some ? (top + log2f(plain)) * 0.69314718055994531f : -INFINITY;
+    a.lse[at] = some ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
 }
 
-// Parts of the key axis: enough work items to fill the resident CTAs once,
-// each part at least 128 keys.
+// Parts of the key axis: as many as keep all work items resident at once (one
+// more would start a second round of CTAs), each part at least 128 keys.
 int decode_splits(const KvView &v, int64_t tiles, int64_t longest, int resident) {
   const int64_t items = std::max<int64_t>(1, tiles * v.heads * v.batch);
-  const int64_t want = (148 * resident + items - 1) / items;
-  return static_cast<int>(std::max<int64_t>(1, std::min({want, (longest + 127) / 128, int64_t{256}})));
+  return static_cast<int>(std::max<int64_t>(1, std::min({148 * resident / items, (longest + 127) / 128, int64_t{256}})));
 }
 
 struct Plan {
@@ -624,8 +649,7 @@ Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   if (!p.prompt) {
     p.few = rows <= 8;
     p.tiles = (rows + (p.few ? 7 : 15)) / (p.few ? 8 : 16);
-    const int work = (t.type == CIM22_FLOAT32 ? 2 : 1) * (p.few ? 1 : 2);
-    p.splits = decode_splits(v, p.tiles, longest, work == 1 ? 4 : work == 2 ? 3 : 2);
+    p.splits = decode_splits(v, p.tiles, longest, t.type == CIM22_FLOAT32 && !p.few ? 2 : 3);
   } else {
     p.tiles = (rows + (p.share ? 127 : 255)) / (p.share ? 128 : 256);
     const int64_t items = p.tiles * v.heads * v.batch;
@@ -633,7 +657,7 @@ Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   }
   p.bytes = p.splits == 1 ? 0
                           : static_cast<size_t>(p.splits) * v.rows * t.q_heads *
-                                (static_cast<size_t>(v.dim) * 4 + 16);
+                                (static_cast<size_t>(v.dim) * 4 + 8);
   return p;
 }
 
@@ -659,11 +683,10 @@ bool attend_args(const char *what, const KvView &v, const cim22_kv_attention *t)
   return true;
 }
 
-template <typename T, int kCh, int kParts, int kQ>
+template <typename T, int kCh, int kParts, int kQ, bool kExact>
 cudaError_t launch_decode(const KvAttendArgs &a, int64_t tiles, cudaStream_t stream) {
-  constexpr size_t bytes =
-      static_cast<size_t>(kWarps) * kStages<kCh, kParts, kQ> * kStageBytes<kCh>;
-  const auto kernel = kv_decode_kernel<T, kCh, kParts, kQ>;
+  constexpr size_t bytes = static_cast<size_t>(kWarps) * kRing<kCh, kParts, kQ> * kGroupBytes<kCh>;
+  const auto kernel = kv_decode_kernel<T, kCh, kParts, kQ, kExact>;
   static DynamicSmem allowed;
   if (const cudaError_t e = allowed.allow(kernel, bytes); e != cudaSuccess)
     return e;
@@ -671,15 +694,20 @@ cudaError_t launch_decode(const KvAttendArgs &a, int64_t tiles, cudaStream_t str
                     dim3(kThreads), bytes, stream, a);
 }
 
+template <typename T, int kParts, int kQ>
+cudaError_t launch_decode(const KvAttendArgs &a, int64_t tiles, cudaStream_t stream) {
+  return a.v.dim == 128  ? launch_decode<T, 2, kParts, kQ, true>(a, tiles, stream)
+         : a.v.dim > 64  ? launch_decode<T, 2, kParts, kQ, false>(a, tiles, stream)
+         : a.v.dim == 64 ? launch_decode<T, 1, kParts, kQ, true>(a, tiles, stream)
+                         : launch_decode<T, 1, kParts, kQ, false>(a, tiles, stream);
+}
+
 template <typename T, int kParts>
 cudaError_t launch_attend(const KvAttendArgs &a, int type, const Plan &plan, cudaStream_t stream) {
-  const bool wide = a.v.dim > 64;
   cudaError_t e =
       plan.prompt ? kv_prompt_launch(a, type, plan.share, static_cast<int>(plan.tiles), stream)
-      : plan.few  ? wide ? launch_decode<T, 2, kParts, 1>(a, plan.tiles, stream)
-                         : launch_decode<T, 1, kParts, 1>(a, plan.tiles, stream)
-      : wide      ? launch_decode<T, 2, kParts, 2>(a, plan.tiles, stream)
-                  : launch_decode<T, 1, kParts, 2>(a, plan.tiles, stream);
+      : plan.few  ? launch_decode<T, kParts, 1>(a, plan.tiles, stream)
+                  : launch_decode<T, kParts, 2>(a, plan.tiles, stream);
   if (e == cudaSuccess && a.splits > 1) {
     const int64_t rows = std::min<int64_t>(a.v.most, a.v.rows) * a.q_heads;
     e = launch_pdl(kv_join_kernel<T>, dim3(static_cast<unsigned>(rows), 1, a.v.batch), dim3(128),
@@ -743,7 +771,7 @@ int cim22_cuda_kv_attend(const cim22_kv_cache *cache, const cim22_kv_sequences *
   a.window = attention->window;
   a.splits = plan.splits;
   a.part_o = static_cast<float *>(workspace);
-  a.part_ml = plan.bytes ? reinterpret_cast<float4 *>(a.part_o + static_cast<size_t>(plan.splits) * v.rows * a.q_heads * v.dim)
+  a.part_ml = plan.bytes ? reinterpret_cast<float2 *>(a.part_o + static_cast<size_t>(plan.splits) * v.rows * a.q_heads * v.dim)
                          : nullptr;
   a.status = status;
   const auto s = static_cast<cudaStream_t>(stream);

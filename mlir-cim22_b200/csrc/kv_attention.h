@@ -17,7 +17,7 @@ struct KvAttendArgs {
   int q_heads, group, causal, window;
   int splits;     // parts of the key axis
   float *part_o;  // [splits][rows * q_heads][dim], relative to 2^m, when splits > 1
-  float4 *part_ml; // [splits][rows * q_heads] (m, l, unrounded l, -)
+  float2 *part_ml; // [splits][rows * q_heads] (m, l)
   int32_t *status;
 };
 

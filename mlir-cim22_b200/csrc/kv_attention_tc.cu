@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       }
       if (live && ok) {
         if (apart)
-          a.part_ml[slot] = make_float4(some ? m : kNone, l, l, 0.0f);
+          a.part_ml[slot] = make_float2(some ? m : kNone, l);
         else if (a.lse)
           a.lse[at] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
       }

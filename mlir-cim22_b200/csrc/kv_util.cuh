@@ -83,7 +83,7 @@ __device__ __forceinline__ KvSequence kv_sequence(const KvView &v, int b) {
     const int64_t n = static_cast<int64_t>(v.starts[b + 1]) - s.row0;
     s.n = n < 0 || n > v.most ? -1 : static_cast<int>(n);
   }
-  s.ok = s.n >= 0 && s.row0 >= 0 && s.row0 + s.n <= v.rows && s.length >= 0 && s.length <= kKvLongest &&
+  s.ok = s.n >= 0 && s.row0 >= 0 && s.row0 + s.n <= v.rows && s.length >= 0 && s.length <= kKvLongest && (v.pages > 0 || s.length == 0) &&
          s.length <= (static_cast<int64_t>(v.table_width) << v.block_log2);
   if (!s.ok)
     s.n = s.length = 0;
