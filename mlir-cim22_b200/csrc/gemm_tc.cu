@@ -1701,6 +1701,24 @@ bool encode_nchw_box(CUtensorMap *map, const float *x, uint64_t W, uint64_t H, u
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_kv_groups(CUtensorMap *map, const int8_t *codes, uint64_t dim, uint64_t block,
+                      uint64_t planes, uint64_t pages, uint32_t inner) {
+  auto fn = encode_fn();
+  if (!fn)
+    return false;
+  const cuuint64_t dims[4] = {dim, block, planes, pages ? pages : 1};
+  const cuuint64_t strides[3] = {dim, dim * block, dim * block * planes};
+  const cuuint32_t box[4] = {inner, 16, 2, 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  // An empty cache has no address; nothing is then copied through the map.
+  void *base = pages ? const_cast<int8_t *>(codes) : reinterpret_cast<void *>(uintptr_t{1024});
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE,
+            inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool encode_prepared_store(CUtensorMap *map, void *base, uint64_t rows, uint64_t k_pad,
                            bool b16) {
   auto fn = encode_fn();

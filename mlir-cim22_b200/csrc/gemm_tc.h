@@ -83,6 +83,13 @@ bool launch_int8(const int8_t *A, int64_t a_rows, int64_t a_cols, const int8_t *
 bool encode_nchw_box(CUtensorMap *map, const float *x, uint64_t W, uint64_t H, uint64_t C,
                      uint64_t N, uint32_t wb, uint32_t hb, uint32_t cb, uint32_t nb);
 
+// Tensor map of an 8-bit key/value cache, codes [pages][planes][block][dim],
+// with boxes of one 16-token group's keys and values: 2 planes x 16 tokens x
+// `inner` bytes (64 or 128, at least dim; zeros past dim), rows swizzled over
+// 64 or 128 bytes.
+bool encode_kv_groups(CUtensorMap *map, const int8_t *codes, uint64_t dim, uint64_t block,
+                      uint64_t planes, uint64_t pages, uint32_t inner);
+
 // Tensor map of prepared activation columns [rows][k_pad] (int8, or BF16
 // with b16) for TMA stores of 32-row x 64-element boxes from a swizzled
 // shared-memory tile: 64-byte swizzle for int8 rows, 128-byte for BF16 rows.

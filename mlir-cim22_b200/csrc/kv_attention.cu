@@ -7,19 +7,23 @@
 // (query tokens x the heads that share a kv head). A work item is a 16-token
 // group of one kv head, which lies in one page, so its two scales are
 // constants. Warps take groups in turn and need nothing from each other until
-// the end: each lane copies (cp.async) exactly the bytes it later feeds the
-// products with into its own shared-memory slots, a few groups deep, so the
-// ring has no barriers and no bank conflicts:
-//   keys    lane (g, c) holds codes 16c .. 16c + 15 of each 64 of tokens g and
-//           8 + g: the contraction runs over head_dim in the order that makes
-//           these its A fragments, and the queries are laid out to match;
-//   values  lane (g, c) holds codes 16g .. 16g + 15 (D = 128) of tokens 2c,
-//           2c + 1, 8 + 2c, 9 + 2c: byte permutes make the A fragments, and
-//           neighbouring rows of the result are neighbouring elements.
+// the end: each has its own ring of swizzled shared-memory tiles that one bulk
+// tensor copy a group fills (per-lane asynchronous copies of the same bytes
+// stopped at 3.4 TB/s, whatever was done with them).
+//   keys    lane (g, c) takes codes 16c .. 16c + 15 of each 64 of tokens t(g)
+//           and 8 + t(g): the contraction runs over head_dim in the order that
+//           makes these its A fragments, and the queries are laid out to match;
+//   values  lane (g, c) takes 16 codes (D = 128) of tokens t(2c), t(2c + 1) and
+//           those plus 8: byte permutes make the A fragments, and neighbouring
+//           rows of the result are neighbouring elements.
+// t and the elements that a lane takes are chosen so that eight neighbouring
+// lanes read eight different 16-byte banks of the swizzled rows.
 // Codes are exact in f16. Queries are scaled by a power of two a row and held
 // as one f16 part (bf16 and f16 inputs lose nothing within 2^-39 of the row's
 // largest) or two (f32: 22 bits); so are the probabilities.
+#include "gemm_tc.h"
 #include "kv_attention.h"
+#include "tma_util.cuh"
 
 #include <algorithm>
 
@@ -37,13 +41,6 @@ template <int kParts, int kQ> constexpr int kTake = kParts * kQ == 1 ? 2 : 1;
 
 __device__ __forceinline__ uint32_t smem_at(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-template <int kBytes> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src) {
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // The 8 x 8 matrix of 16-bit values that a warp's registers hold, transposed.
@@ -81,9 +78,9 @@ __device__ __forceinline__ void put_row(T *out, int d, int dim, const float (&v)
   }
 }
 
-template <typename T, int kCh, int kParts, int kQ, bool kExact>
+template <typename T, int kCh, int kParts, int kQ>
 __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
-    kv_decode_kernel(const KvAttendArgs a) {
+    kv_decode_kernel(const KvAttendArgs a, const __grid_constant__ CUtensorMap codes) {
   constexpr int kTiles = 4 * kCh;  // 16-element tiles of the head
   constexpr int kLane = 8 * kCh;   // value bytes a lane holds of a token
   constexpr int kG = kTake<kParts, kQ>; // groups a round
@@ -91,13 +88,14 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   constexpr int kBytes = kGroupBytes<kCh>;
   constexpr int kRows = 8 * kQ;
   constexpr bool kRaised = kParts == 1; // keys enter with 1152 added
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t raw[];
+  uint8_t *smem = raw + ((1024u - (smem_at(raw) & 1023u)) & 1023u);
+  __shared__ uint64_t full[kWarps][kRounds];
   __shared__ float row_m[kWarps][kRows], row_l[kWarps][kRows];
   __shared__ float4 constants[kWarps][32];
   pdl_launch_dependents();
   pdl_wait();
   const KvView &v = a.v;
-  const int dim = kExact ? 64 * kCh : v.dim;
   const int b = blockIdx.z, split = blockIdx.x;
   const int head = blockIdx.y % v.heads, f0 = blockIdx.y / v.heads * kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -123,67 +121,61 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   // round may run past `end` (its groups are then hidden).
   const int count = end > begin ? (end - begin + kG * kWarps - 1) / (kG * kWarps) : 0; // rounds
 
-  const uint32_t ring = smem_at(smem) + warp * kRounds * kG * kBytes;
+  uint8_t *ring = smem + warp * kRounds * kG * kBytes;
+  if (lane == 0)
+    for (int i = 0; i < kRounds; ++i)
+      barrier_init(&full[warp][i], 1);
+  __syncwarp();
   const int per_page = v.block_log2 - 4; // log2 of the groups a page holds
-  // Lane i of a batch of 32 groups holds where the warp's i-th group begins, in
-  // units of a group's keys; -1 where there is none.
-  auto places_of = [&](int i0) {
+  // Lane i of a batch of 32 groups holds the page of the warp's i-th group; -1
+  // where there is none.
+  auto pages_of = [&](int i0) {
     const int i = i0 + lane;
     const int group = begin + i / kG * (kG * kWarps) + i % kG;
-    int place = -1;
+    int page = -1;
     if (i < count * kG && group < end) {
-      const int page = kv_page(v, b, group >> per_page);
+      page = kv_page(v, b, group >> per_page);
       if (page < 0)
         atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
-      else
-        place = (((page * v.heads + head) * 2) << per_page) + (group & ((1 << per_page) - 1));
     }
-    return place;
+    return page;
   };
-  // What a lane reads of a group; lanes past head_dim read nothing (their
-  // slots stay zero).
-  const int k_lane = g * dim + 16 * c, v_lane = (dim << v.block_log2) + 2 * c * dim + kLane * g;
-  bool k_in[kCh];
-#pragma unroll
-  for (int ch = 0; ch < kCh; ++ch)
-    k_in[ch] = kExact || 64 * ch + 16 * c < dim;
-  const bool v_in = kExact || kLane * g < dim;
-  if (!kExact) {
-    for (int i = lane * 16; i < kRounds * kG * kBytes; i += 512)
-      *reinterpret_cast<uint4 *>(smem + warp * kRounds * kG * kBytes + i) = make_uint4(0, 0, 0, 0);
-    __syncwarp();
-  }
-  int batch_place = places_of(0), next_place = places_of(32);
-  auto issue = [&](int j, int round) { // every lane copies its bytes of round j
+  int batch_page = pages_of(0), next_page = pages_of(32);
+  // One copy a group: 16 tokens of keys and of values (elements past head_dim
+  // arrive as zeros). Groups without a page keep what the slot held (any codes
+  // are finite, and they are hidden below).
+  auto issue = [&](int j, int round) {
     if (j < count) {
+      int page[kG], bytes = 0;
 #pragma unroll
       for (int u = 0; u < kG; ++u) {
         const int i = j * kG + u;
-        const int place = __shfl_sync(0xffffffffu, (i & 32) == 0 ? batch_place : next_place, i & 31);
-        // Groups without a place read as place 0 (their keys are hidden below).
-        const int8_t *at = v.codes + static_cast<int64_t>(max(place, 0)) * (16 * dim);
-        const int8_t *k = at + k_lane, *values = at + v_lane;
-        const uint32_t slot = ring + (round * kG + u) * kBytes + lane * 16;
+        page[u] = __shfl_sync(0xffffffffu, (i & 32) == 0 ? batch_page : next_page, i & 31);
+        bytes += page[u] >= 0 ? kBytes : 0;
+      }
+      if (lane == 0) {
+        barrier_expect_tx(&full[warp][round], bytes);
 #pragma unroll
-        for (int ch = 0; ch < kCh; ++ch)
-          if (k_in[ch]) {
-            copy_async<16>(slot + ch * 512, k + 64 * ch);
-            copy_async<16>(slot + (kCh + ch) * 512, k + 8 * dim + 64 * ch);
-          }
-        if (v_in) {
-          const uint32_t to = ring + (round * kG + u) * kBytes + 2 * kCh * 512 + lane * kLane;
-          copy_async<kLane>(to, values);
-          copy_async<kLane>(to + 32 * kLane, values + dim);
-          copy_async<kLane>(to + 64 * kLane, values + 8 * dim);
-          copy_async<kLane>(to + 96 * kLane, values + 9 * dim);
-        }
+        for (int u = 0; u < kG; ++u)
+          if (page[u] >= 0)
+            tma_load_4d(ring + (round * kG + u) * kBytes, &codes, &full[warp][round], 0,
+                        ((begin + j * (kG * kWarps) + u) & ((1 << per_page) - 1)) << 4, 2 * head,
+                        page[u]);
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll 1
   for (int j = 0; j < kRounds - 1; ++j)
     issue(j, j);
+
+  // Token of row g, and where the lane's bytes of a group lie (comment above).
+  const int token = kCh == 2 ? (g >> 1) | (g & 1) << 2 : g;
+  const int chunk = kCh == 2 ? token : g; // the lane's 8 * kCh value elements
+  const uint32_t k_at = smem_at(ring) + token * 64 * kCh +
+                        ((c ^ (kCh == 2 ? token : g >> 1)) << 4);
+  const uint32_t v_at = smem_at(ring) + 16 * 64 * kCh +
+                        (kCh == 2 ? c * 128 + ((chunk ^ c) << 4)
+                                  : 2 * c * 64 + (((g >> 1) ^ c) << 4) + (g & 1) * 8);
 
   // Query rows f0 + 8 t + g as B fragments (lane (g, c) holds the elements
   // whose codes lane (., c) holds); results come out for rows 2c and 2c + 1.
@@ -203,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     for (int e = 0; e < kCh * 16; e += kVec<T>) {
       Pack<T> p;
       if (live)
-        p = load_pack(q, (e / 16) * 64 + 16 * c + e % 16, dim);
+        p = load_pack(q, (e / 16) * 64 + 16 * c + e % 16, v.dim);
 #pragma unroll
       for (int j = 0; j < kVec<T>; ++j) {
         x[e + j] = to_f32(p.at[j]);
@@ -254,37 +246,45 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     for (int j = 0; j < kTiles; ++j)
       o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.0f;
   }
-  // The places of groups [64 i, 64 i + 32) are in batch_place, of the next 32
-  // in next_place; each is refilled when its last group has been taken.
-  int round = 0;
+  // The pages of groups [64 i, 64 i + 32) are in batch_page, of the next 32 in
+  // next_page; each is refilled when its last group has been taken.
+  int round = 0, parity = 0, issued = min(count, kRounds - 1);
+  bool ok = true;
 #pragma unroll 1
   for (int j = 0; j < count; ++j) {
     const int i0 = j * kG;
-    if ((i0 & 31) == 0) { // scales of groups i0 .. i0 + 31 (their places are still held)
-      const int place = (i0 & 32) == 0 ? batch_place : next_place;
+    if ((i0 & 31) == 0) { // scales of groups i0 .. i0 + 31 (their pages are still held)
+      const int page = (i0 & 32) == 0 ? batch_page : next_page;
       float4 k = make_float4(0.0f, 0.0f, 1.0f, 0.0f); // hidden
-      if (place >= 0) {
-        // (page * heads + head) * 2 floats into the scales.
-        const float2 sc = reinterpret_cast<const float2 *>(v.scales)[place >> (per_page + 1)];
+      if (page >= 0) {
+        const float2 sc = *reinterpret_cast<const float2 *>(
+            v.scales + (static_cast<int64_t>(page) * v.heads + head) * 2);
         const float sv = fmaxf(sc.y, kKvLeastScale);
         k = make_float4(sc.x, log2f(sv), 1.0f / sv, 1.0f);
       }
       __syncwarp();
       constants[warp][lane] = k;
-      __syncwarp();
     }
+    __syncwarp(); // every lane is done with the slot that is filled next
     issue(j + kRounds - 1, round == 0 ? kRounds - 1 : round - 1);
-    if (((i0 + kG) & 31) == 0) { // this batch's places are no longer needed
-      const int refill = places_of(i0 + kG + 32);
+    issued = min(count, j + kRounds);
+    if (((i0 + kG) & 31) == 0) { // this batch's pages are no longer needed
+      const int refill = pages_of(i0 + kG + 32);
       if ((i0 & 32) == 0)
-        batch_place = refill;
+        batch_page = refill;
       else
-        next_place = refill;
+        next_page = refill;
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(kRounds - 1) : "memory");
-    const uint32_t slot = ring + round * kG * kBytes + lane * 16;
-    const uint32_t v_slot = ring + round * kG * kBytes + 2 * kCh * 512 + lane * kLane;
+    ok = __all_sync(0xffffffffu, barrier_wait(&full[warp][round], parity));
+    if (!ok) {
+      // Leave only when the copies in flight have landed, or never will.
+      for (int x = j; x < issued; ++x)
+        barrier_wait(&full[warp][x % kRounds], (x / kRounds) & 1);
+      break;
+    }
+    const uint32_t slot = round * kG * kBytes;
     round = round + 1 == kRounds ? 0 : round + 1;
+    parity ^= round == 0;
     float4 k[kG];
 #pragma unroll
     for (int u = 0; u < kG; ++u)
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
         for (int z = 0; z < 2; ++z)
           asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(w[u][z][0]), "=r"(w[u][z][1]), "=r"(w[u][z][2]), "=r"(w[u][z][3])
-                       : "r"(slot + u * kBytes + (z * kCh + ch) * 512)
+                       : "r"((k_at ^ (64 * ch)) + slot + u * kBytes + z * 8 * 64 * kCh)
                        : "memory");
 #pragma unroll
       for (int x = 0; x < 4; ++x)
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
         }
     }
     // Exponents relative to the rows' references: element e of sc is token
-    // g + 8 (e / 2) of its group and row 2c + (e % 2).
+    // t(g) + 8 (e / 2) of its group and row 2c + (e % 2).
     const int key0 = (begin + j * (kG * kWarps)) << 4;
     bool whole = key0 + 16 * kG - 1 < s.length &&
                  (!a.causal || key0 + 16 * kG - 1 <= pos_first) &&
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
         for (int u = 0; u < kG; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (k[u].w == 0.0f || !sees(a, s.length, pos[t][e & 1], key0 + 16 * u + g + 8 * (e >> 1)))
+            if (k[u].w == 0.0f || !sees(a, s.length, pos[t][e & 1], key0 + 16 * u + token + 8 * (e >> 1)))
               hidden |= 1u << (4 * u + e);
       }
       float arg[kG][4];
@@ -430,12 +430,13 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
         if constexpr (kCh == 2)
           asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(w[t][0]), "=r"(w[t][1]), "=r"(w[t][2]), "=r"(w[t][3])
-                       : "r"(v_slot + u * kBytes + t * 32 * kLane)
+                       : "r"((v_at ^ (64 * (t & 1))) + slot + u * kBytes +
+                             ((t & 1) * 4 + (t >> 1) * 8) * 128)
                        : "memory");
         else
           asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
                        : "=r"(w[t][0]), "=r"(w[t][1])
-                       : "r"(v_slot + u * kBytes + t * 32 * kLane)
+                       : "r"(v_at + slot + u * kBytes + ((t & 1) + (t >> 1) * 8) * 64)
                        : "memory");
       }
 #pragma unroll
@@ -470,7 +471,8 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
       }
     }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (!ok && lane == 0)
+    atomicOr(a.status, CIM22_STATUS_TIMEOUT);
 
   // Join the warps: rows [warp][kRows][64 * kCh] in the ring's memory.
   __syncthreads();
@@ -487,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
         row_m[warp][row] = m[t][r];
         row_l[warp][row] = l[t][r];
       }
-      float2 *to = reinterpret_cast<float2 *>(joined + (warp * kRows + row) * 64 * kCh + kLane * g);
+      float2 *to = reinterpret_cast<float2 *>(joined + (warp * kRows + row) * 64 * kCh + kLane * chunk);
 #pragma unroll
       for (int j = 0; j < kTiles; ++j)
         to[j] = make_float2(o[t][j][r], o[t][j][r + 2]);
@@ -683,23 +685,26 @@ bool attend_args(const char *what, const KvView &v, const cim22_kv_attention *t)
   return true;
 }
 
-template <typename T, int kCh, int kParts, int kQ, bool kExact>
+template <typename T, int kCh, int kParts, int kQ>
 cudaError_t launch_decode(const KvAttendArgs &a, int64_t tiles, cudaStream_t stream) {
-  constexpr size_t bytes = static_cast<size_t>(kWarps) * kRing<kCh, kParts, kQ> * kGroupBytes<kCh>;
-  const auto kernel = kv_decode_kernel<T, kCh, kParts, kQ, kExact>;
+  constexpr size_t bytes =
+      static_cast<size_t>(kWarps) * kRing<kCh, kParts, kQ> * kGroupBytes<kCh> + 1024;
+  const auto kernel = kv_decode_kernel<T, kCh, kParts, kQ>;
   static DynamicSmem allowed;
   if (const cudaError_t e = allowed.allow(kernel, bytes); e != cudaSuccess)
     return e;
+  CUtensorMap codes;
+  if (!tc::encode_kv_groups(&codes, a.v.codes, a.v.dim, 1 << a.v.block_log2, 2 * a.v.heads,
+                            a.v.pages, 64 * kCh))
+    return cudaErrorInvalidValue;
   return launch_pdl(kernel, dim3(a.splits, static_cast<unsigned>(tiles * a.v.heads), a.v.batch),
-                    dim3(kThreads), bytes, stream, a);
+                    dim3(kThreads), bytes, stream, a, codes);
 }
 
 template <typename T, int kParts, int kQ>
 cudaError_t launch_decode(const KvAttendArgs &a, int64_t tiles, cudaStream_t stream) {
-  return a.v.dim == 128  ? launch_decode<T, 2, kParts, kQ, true>(a, tiles, stream)
-         : a.v.dim > 64  ? launch_decode<T, 2, kParts, kQ, false>(a, tiles, stream)
-         : a.v.dim == 64 ? launch_decode<T, 1, kParts, kQ, true>(a, tiles, stream)
-                         : launch_decode<T, 1, kParts, kQ, false>(a, tiles, stream);
+  return a.v.dim > 64 ? launch_decode<T, 2, kParts, kQ>(a, tiles, stream)
+                      : launch_decode<T, 1, kParts, kQ>(a, tiles, stream);
 }
 
 template <typename T, int kParts>
