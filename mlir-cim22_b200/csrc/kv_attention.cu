@@ -65,17 +65,43 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// One row's final (or partial) output element range.
-template <typename T, int kCount>
-__device__ __forceinline__ void put_row(T *out, int d, int dim, const float (&v)[kCount]) {
+// A float of the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ float peer_load(const float *mine, int rank, int cluster) {
+  if (cluster == 1)
+    return *mine;
+  float x;
+  asm volatile("{\n .reg .b32 at;\n mapa.shared::cluster.u32 at, %1, %2;\n"
+               " ld.shared::cluster.f32 %0, [at];\n}\n"
+               : "=f"(x)
+               : "r"(smem_at(mine)), "r"(rank)
+               : "memory");
+  return x;
+}
+
+// kE neighbouring ones.
+template <int kE>
+__device__ __forceinline__ void peer_load(const float *mine, int rank, int cluster, float (&x)[kE]) {
+  if (cluster == 1) {
 #pragma unroll
-  for (int i = 0; i < kCount; i += kVec<T>) {
-    Pack<T> o;
-#pragma unroll
-    for (int j = 0; j < kVec<T>; ++j)
-      o.at[j] = from_f32<T>(v[i + j]);
-    store_pack(out, d + i, dim, o);
+    for (int e = 0; e < kE; ++e)
+      x[e] = mine[e];
+  } else if constexpr (kE == 4) {
+    asm volatile("{\n .reg .b32 at;\n mapa.shared::cluster.u32 at, %4, %5;\n"
+                 " ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [at];\n}\n"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+                 : "r"(smem_at(mine)), "r"(rank)
+                 : "memory");
+  } else {
+    asm volatile("{\n .reg .b32 at;\n mapa.shared::cluster.u32 at, %2, %3;\n"
+                 " ld.shared::cluster.v2.f32 {%0, %1}, [at];\n}\n"
+                 : "=f"(x[0]), "=f"(x[1])
+                 : "r"(smem_at(mine)), "r"(rank)
+                 : "memory");
   }
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 template <typename T, int kCh, int kParts, int kQ>
@@ -140,7 +166,32 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     }
     return page;
   };
-  int batch_page = pages_of(0), next_page = pages_of(32);
+  // Query row f0 + 8 t + g, the lane's 16 elements of each 64: on their way
+  // before the copies of the codes are.
+  Pack<T> query[kQ][kCh * 16 / kVec<T>];
+#pragma unroll
+  for (int t = 0; t < kQ; ++t) {
+    const int f = f0 + 8 * t + g;
+    if (f < rows) {
+      const int i = f / a.group;
+      const T *q = static_cast<const T *>(a.q) + (s.row0 + i) * a.q_row_stride +
+                   (head * a.group + f - i * a.group) * a.q_head_stride;
+#pragma unroll
+      for (int e = 0; e < kCh * 16; e += kVec<T>) {
+        const int d = (e / 16) * 64 + 16 * c + e % 16;
+        if (d < v.dim) { // head_dim is a multiple of 16
+          if (a.q_aligned) {
+            query[t][e / kVec<T>].raw = __ldg(reinterpret_cast<const uint4 *>(q + d));
+          } else {
+#pragma unroll
+            for (int j = 0; j < kVec<T>; ++j)
+              query[t][e / kVec<T>].at[j] = q[d + j];
+          }
+        }
+      }
+    }
+  }
+  int batch_page = pages_of(0), next_page = -1;
   // One copy a group: 16 tokens of keys and of values (elements past head_dim
   // arrive as zeros). Groups without a page keep what the slot held (any codes
   // are finite, and they are hidden below).
@@ -164,6 +215,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
       }
     }
   };
+  next_page = pages_of(32); // (the first rounds take batch_page alone)
 #pragma unroll 1
   for (int j = 0; j < kRounds - 1; ++j)
     issue(j, j);
@@ -184,23 +236,12 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   int pos[kQ][2];
 #pragma unroll
   for (int t = 0; t < kQ; ++t) {
-    const int f = f0 + 8 * t + g;
-    const bool live = f < rows;
-    const int i = live ? f / a.group : 0;
-    const T *q = static_cast<const T *>(a.q) + (s.row0 + i) * a.q_row_stride +
-                 (head * a.group + (live ? f - i * a.group : 0)) * a.q_head_stride;
     float x[kCh * 16];
     float amax = 0.0f;
 #pragma unroll
-    for (int e = 0; e < kCh * 16; e += kVec<T>) {
-      Pack<T> p;
-      if (live)
-        p = load_pack(q, (e / 16) * 64 + 16 * c + e % 16, v.dim);
-#pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) {
-        x[e + j] = to_f32(p.at[j]);
-        amax = nan_max(amax, fabsf(x[e + j]));
-      }
+    for (int e = 0; e < kCh * 16; ++e) {
+      x[e] = to_f32(query[t][e / kVec<T>].at[e % kVec<T>]);
+      amax = nan_max(amax, fabsf(x[e]));
     }
 #pragma unroll
     for (int o = 1; o < 4; o *= 2)
@@ -474,7 +515,9 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   if (!ok && lane == 0)
     atomicOr(a.status, CIM22_STATUS_TIMEOUT);
 
-  // Join the warps: rows [warp][kRows][64 * kCh] in the ring's memory.
+  // Join the warps of the cluster's CTAs, which hold parts of one key axis:
+  // rows [warp][kRows][64 * kCh] in the rings' memory, each CTA finishing every
+  // cl-th row from all of them.
   __syncthreads();
   float *joined = reinterpret_cast<float *>(smem);
 #pragma unroll
@@ -494,46 +537,74 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
       for (int j = 0; j < kTiles; ++j)
         to[j] = make_float2(o[t][j][r], o[t][j][r + 2]);
     }
-  __syncthreads();
-  constexpr int kEach = kCh * kQ == 1 ? 8 : 4 * kCh * kQ; // elements a thread joins
-  constexpr int kAcross = 64 * kCh / kEach;
-  const int row = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kEach;
-  const int f = f0 + row;
-  if (row >= kRows || f >= rows)
-    return;
-  float top = kNone;
+  const int cl = a.cluster, rank = split % cl;
+  if (cl > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  // A warp a row, 2 * kCh neighbouring elements a lane.
+  constexpr int kE = 2 * kCh;
+  const int d = kE * lane;
+#pragma unroll 1
+  for (int row = rank + cl * warp; row < kRows; row += cl * kWarps) {
+    const int f = f0 + row;
+    if (f >= rows)
+      break;
+    // Lane 4 p + x weighs what warp x of CTA p holds.
+    const bool there = lane >> 2 < cl;
+    const float mine = there ? peer_load(&row_m[lane & 3][row], lane >> 2, cl) : kNone;
+    float sum = there ? peer_load(&row_l[lane & 3][row], lane >> 2, cl) : 0.0f;
+    float top = mine;
 #pragma unroll
-  for (int x = 0; x < kWarps; ++x)
-    top = fmaxf(top, row_m[x][row]);
-  float sum = 0.0f, acc[kEach];
+    for (int o = 16; o; o >>= 1)
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float share = exp2_approx(mine - top);
+    sum *= share;
 #pragma unroll
-  for (int j = 0; j < kEach; ++j)
-    acc[j] = 0.0f;
+    for (int o = 16; o; o >>= 1)
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    float acc[kE];
 #pragma unroll
-  for (int x = 0; x < kWarps; ++x) {
-    const float share = exp2_approx(row_m[x][row] - top);
-    sum = fmaf(row_l[x][row], share, sum);
+    for (int e = 0; e < kE; ++e)
+      acc[e] = 0.0f;
+#pragma unroll 2
+    for (int p = 0; p < cl; ++p) {
+      float part[kWarps][kE];
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      acc[j] = fmaf(joined[(x * kRows + row) * 64 * kCh + d + j], share, acc[j]);
+      for (int x = 0; x < kWarps; ++x)
+        peer_load(&joined[(x * kRows + row) * 64 * kCh + d], p, cl, part[x]);
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        const float w = __shfl_sync(0xffffffffu, share, 4 * p + x);
+#pragma unroll
+        for (int e = 0; e < kE; ++e)
+          acc[e] = fmaf(part[x][e], w, acc[e]);
+      }
+    }
+    if (d >= v.dim)
+      continue;
+    const int i = f / a.group;
+    const int64_t at = (s.row0 + i) * a.q_heads + head * a.group + (f - i * a.group);
+    if (a.splits > cl) {
+      const int64_t to = static_cast<int64_t>(split / cl) * v.rows * a.q_heads + at;
+      if (d == 0)
+        a.part_ml[to] = make_float2(top, sum);
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+        a.part_o[to * v.dim + d + e] = acc[e];
+    } else {
+      const bool some = top > kNone || sum != sum;
+      const float scale = some ? 1.0f / sum : 0.0f;
+      T *out = static_cast<T *>(a.out) + at * v.dim + d;
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+        out[e] = from_f32<T>(acc[e] * scale);
+      if (a.lse && d == 0)
+        a.lse[at] = some ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+    }
   }
-  const int i = f / a.group;
-  const int64_t at = (s.row0 + i) * a.q_heads + head * a.group + (f - i * a.group);
-  if (a.splits > 1) {
-    const int64_t to = static_cast<int64_t>(split) * v.rows * a.q_heads + at;
-    if (d == 0)
-      a.part_ml[to] = make_float2(top, sum);
-    put_row(a.part_o + to * v.dim, d, v.dim, acc);
-    return;
-  }
-  const bool some = top > kNone || sum != sum;
-  const float share = some ? 1.0f / sum : 0.0f;
-#pragma unroll
-  for (int j = 0; j < kEach; ++j)
-    acc[j] *= share;
-  put_row(static_cast<T *>(a.out) + at * v.dim, d, v.dim, acc);
-  if (a.lse && d == 0)
-    a.lse[at] = some ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+  if (cl > 1)
+    cluster_sync(); // no CTA leaves while others read its memory
 }
 
 // Joins the parts of the key axis: a CTA a row and head, its warps take parts
@@ -553,7 +624,8 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
   const int64_t at = s.row0 * a.q_heads + f, step = v.rows * a.q_heads;
   float m = kNone, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int kAhead = 4;
-  for (int x0 = warp; x0 < a.splits; x0 += 4 * kAhead) {
+  const int parts = a.splits / a.cluster;
+  for (int x0 = warp; x0 < parts; x0 += 4 * kAhead) {
     float2 ml[kAhead];
     float4 p[kAhead];
 #pragma unroll
@@ -561,7 +633,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
       const int64_t x = x0 + 4 * u;
       ml[u] = make_float2(kNone, 0.0f);
       p[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (x < a.splits) {
+      if (x < parts) {
         ml[u] = a.part_ml[x * step + at];
         if (4 * lane < v.dim)
           p[u] = *reinterpret_cast<const float4 *>(a.part_o + (x * step + at) * v.dim + 4 * lane);
@@ -622,17 +694,34 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
 }
 
 // Parts of the key axis: as many as keep all work items resident at once (one
-// more would start a second round of CTAs), each part at least 128 keys.
-int decode_splits(const KvView &v, int64_t tiles, int64_t longest, int resident) {
-  const int64_t items = std::max<int64_t>(1, tiles * v.heads * v.batch);
-  return static_cast<int>(std::max<int64_t>(1, std::min({148 * resident / items, (longest + 127) / 128, int64_t{256}})));
+// more would start a second round of CTAs), each of at least 128 keys. Items
+// that fill every place by themselves are halved once, which evens out
+// sequences of unequal length (64 of 1,000-8,191 tokens, 8 kv heads: 141 -> 131
+// us); fewer are left whole (32 of 4,000 in f32: 76 us, halved 94). Parts are joined within the kernel as clusters:
+// all of them up to four, up to eight at a time where every CTA has an SM to
+// itself, else in pairs (larger clusters leave places on the SMs empty: one
+// sequence of 200,000 tokens 60 -> 76 us with eight), and the rest by
+// kv_join_kernel.
+void decode_parts(const KvView &v, int64_t tiles, int64_t longest, int resident, int &splits,
+                  int &cluster) {
+  const int64_t items = std::max<int64_t>(1, tiles * v.heads * v.batch), slots = 148 * resident;
+  const int64_t want = 2 * items > slots
+                           ? std::min<int64_t>(items >= slots && items < 4 * slots ? 2 : 1, longest / 512)
+                           : std::min<int64_t>(slots / items, (longest + 127) / 128);
+  splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, 256)));
+  if (splits <= 4 || (splits <= 8 && items * splits <= 148))
+    cluster = splits;
+  else
+    cluster = items * splits <= 148 ? 8 : 2;
+  splits = splits / cluster * cluster;
 }
 
 struct Plan {
   bool prompt; // by the tensor-memory kernel
   bool share;  // with one query tile a CTA
   bool few;    // decode tiles of 8 query rows, not 16
-  int splits;
+  int splits;  // parts of the key axis,
+  int cluster; // so many of them joined within the kernel
   int64_t tiles;
   size_t bytes; // of the partial results
 };
@@ -651,15 +740,18 @@ Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   if (!p.prompt) {
     p.few = rows <= 8;
     p.tiles = (rows + (p.few ? 7 : 15)) / (p.few ? 8 : 16);
-    p.splits = decode_splits(v, p.tiles, longest, t.type == CIM22_FLOAT32 && !p.few ? 2 : 3);
+    decode_parts(v, p.tiles, longest, t.type == CIM22_FLOAT32 && !p.few ? 2 : 3, p.splits,
+                 p.cluster);
   } else {
     p.tiles = (rows + (p.share ? 127 : 255)) / (p.share ? 128 : 256);
     const int64_t items = p.tiles * v.heads * v.batch;
+    p.cluster = 1;
     p.splits = static_cast<int>(std::max<int64_t>(1, std::min({148 / std::max<int64_t>(1, items), (longest + 1023) / 1024, int64_t{64}})));
   }
-  p.bytes = p.splits == 1 ? 0
-                          : static_cast<size_t>(p.splits) * v.rows * t.q_heads *
-                                (static_cast<size_t>(v.dim) * 4 + 8);
+  const int parts = p.splits / p.cluster;
+  p.bytes = parts == 1 ? 0
+                       : static_cast<size_t>(parts) * v.rows * t.q_heads *
+                             (static_cast<size_t>(v.dim) * 4 + 8);
   return p;
 }
 
@@ -697,8 +789,20 @@ cudaError_t launch_decode(const KvAttendArgs &a, int64_t tiles, cudaStream_t str
   if (!tc::encode_kv_groups(&codes, a.v.codes, a.v.dim, 1 << a.v.block_log2, 2 * a.v.heads,
                             a.v.pages, 64 * kCh))
     return cudaErrorInvalidValue;
-  return launch_pdl(kernel, dim3(a.splits, static_cast<unsigned>(tiles * a.v.heads), a.v.batch),
-                    dim3(kThreads), bytes, stream, a, codes);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.splits, static_cast<unsigned>(tiles * a.v.heads), a.v.batch);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a, codes);
 }
 
 template <typename T, int kParts, int kQ>
@@ -713,7 +817,7 @@ cudaError_t launch_attend(const KvAttendArgs &a, int type, const Plan &plan, cud
       plan.prompt ? kv_prompt_launch(a, type, plan.share, static_cast<int>(plan.tiles), stream)
       : plan.few  ? launch_decode<T, kParts, 1>(a, plan.tiles, stream)
                   : launch_decode<T, kParts, 2>(a, plan.tiles, stream);
-  if (e == cudaSuccess && a.splits > 1) {
+  if (e == cudaSuccess && a.splits > a.cluster) {
     const int64_t rows = std::min<int64_t>(a.v.most, a.v.rows) * a.q_heads;
     e = launch_pdl(kv_join_kernel<T>, dim3(static_cast<unsigned>(rows), 1, a.v.batch), dim3(128),
                    0, stream, a);
@@ -772,11 +876,14 @@ int cim22_cuda_kv_attend(const cim22_kv_cache *cache, const cim22_kv_sequences *
   a.scale_log2 = attention->scale * 1.4426950408889634f;
   a.q_heads = attention->q_heads;
   a.group = attention->q_heads / v.heads;
+  a.q_aligned = (reinterpret_cast<uintptr_t>(a.q) |
+                 (a.q_row_stride | a.q_head_stride) * float_size(attention->type)) % 16 == 0;
   a.causal = attention->causal != 0;
   a.window = attention->window;
   a.splits = plan.splits;
+  a.cluster = plan.cluster;
   a.part_o = static_cast<float *>(workspace);
-  a.part_ml = plan.bytes ? reinterpret_cast<float2 *>(a.part_o + static_cast<size_t>(plan.splits) * v.rows * a.q_heads * v.dim)
+  a.part_ml = plan.bytes ? reinterpret_cast<float2 *>(a.part_o + static_cast<size_t>(plan.splits / plan.cluster) * v.rows * a.q_heads * v.dim)
                          : nullptr;
   a.status = status;
   const auto s = static_cast<cudaStream_t>(stream);

@@ -11,13 +11,15 @@ struct KvAttendArgs {
   KvView v;
   const void *q;
   int64_t q_row_stride, q_head_stride;
+  bool q_aligned; // every row starts on a 16-byte boundary
   void *out;
   float *lse;
   float scale_log2; // softmax scale * log2(e)
   int q_heads, group, causal, window;
-  int splits;     // parts of the key axis
-  float *part_o;  // [splits][rows * q_heads][dim], relative to 2^m, when splits > 1
-  float2 *part_ml; // [splits][rows * q_heads] (m, l)
+  int splits;     // parts of the key axis,
+  int cluster;    // so many neighbouring ones joined within the kernel
+  float *part_o;   // [splits / cluster][rows * q_heads][dim], relative to 2^m,
+  float2 *part_ml; // [splits / cluster][rows * q_heads] (m, l), when not one
   int32_t *status;
 };
 
