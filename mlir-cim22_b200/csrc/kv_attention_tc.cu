@@ -137,6 +137,57 @@ __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[32]) {
                : "memory");
 }
 
+// The same without waiting: tmem_loaded() orders the registers' use.
+__device__ __forceinline__ void tmem_load_start(uint32_t at, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, "
+               "%9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+               "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+                 "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                 "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+                 "=r"(r[30]), "=r"(r[31])
+               : "r"(at)
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// a * b + c and a + b of pairs, each half rounding as the scalar operation.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, "
                "%9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
@@ -515,21 +566,43 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const float4 *scale = sm.scale[tile & 3];
+      // The largest exponent of the row, t = score * log2(e) + log2(scale of v).
       float top = -INFINITY;
+      uint32_t x[2][32];
+      tmem_load_start(s_at, x[0]);
+      if (whole) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t x[32];
-        tmem_load(s_at + 32 * c, x);
-        const uint32_t seen = whole ? 0xffffffffu : visible(c);
+        for (int c = 0; c < 4; ++c) {
+          tmem_loaded(x[c & 1]);
+          if (c < 3)
+            tmem_load_start(s_at + 32 * (c + 1), x[(c + 1) & 1]);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          float best = -INFINITY;
+          for (int g = 0; g < 2; ++g) {
+            const uint32_t *y = x[c & 1] + 16 * g;
+            float best = __uint_as_float(y[0]);
 #pragma unroll
-          for (int i = 16 * g; i < 16 * g + 16; ++i)
-            best = fmaxf(best, whole || (seen >> i & 1) ? __uint_as_float(x[i]) : -INFINITY);
-          const float4 sc = scale[2 * c + g];
-          if (best != -INFINITY)
+            for (int i = 1; i < 15; i += 2)
+              best = max3(best, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+            best = fmaxf(best, __uint_as_float(y[15]));
+            const float4 sc = scale[2 * c + g];
             top = nan_max(top, fmaf(best, coef * sc.x, sc.y));
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          tmem_load(s_at + 32 * c, x[0]);
+          const uint32_t seen = visible(c);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            float best = -INFINITY;
+#pragma unroll
+            for (int i = 16 * g; i < 16 * g + 16; ++i)
+              best = fmaxf(best, seen >> i & 1 ? __uint_as_float(x[0][i]) : -INFINITY);
+            const float4 sc = scale[2 * c + g];
+            if (best != -INFINITY)
+              top = nan_max(top, fmaf(best, coef * sc.x, sc.y));
+          }
         }
       }
       // Set the row's reference again when its probabilities outgrow f16.
@@ -557,39 +630,51 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         }
       }
       const float origin = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t x[32];
-        tmem_load(s_at + 32 * c, x);
-        const uint32_t seen = whole ? 0xffffffffu : visible(c);
+      // Probabilities of 32 scores, over the scores just read.
+      auto probabilities = [&](int c, const uint32_t (&y)[32], uint32_t seen, bool all) {
         uint32_t high[16], low[16];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const float4 sc = scale[2 * c + g];
           const float slope = coef * sc.x, shift = sc.y - origin;
-          float sum = 0.0f;
+          float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (int i = 16 * g; i < 16 * g + 16; i += 2) {
-            float e0 = fmaf(__uint_as_float(x[i]), slope, shift);
-            float e1 = fmaf(__uint_as_float(x[i + 1]), slope, shift);
-            if (!whole) {
-              e0 = seen >> i & 1 ? e0 : -INFINITY;
-              e1 = seen >> (i + 1) & 1 ? e1 : -INFINITY;
+            float2 e = fma2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])),
+                            make_float2(slope, slope), make_float2(shift, shift));
+            if (!all) {
+              e.x = seen >> i & 1 ? e.x : -INFINITY;
+              e.y = seen >> (i + 1) & 1 ? e.y : -INFINITY;
             }
-            const float p0 = exp2_approx(e0), p1 = exp2_approx(e1);
-            sum += p0 + p1;
-            high[i / 2] = pack_half(p0, p1);
+            const float2 p = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+            sum = add2(sum, p);
+            high[i / 2] = pack_half(p.x, p.y);
             if constexpr (kParts == 2) {
               const float2 back = unpack_half(high[i / 2]);
-              low[i / 2] = pack_half(p0 - back.x, p1 - back.y);
+              low[i / 2] = pack_half(p.x - back.x, p.y - back.y);
             }
           }
-          l = fmaf(sum, sc.z, l);
+          l = fmaf(sum.x + sum.y, sc.z, l);
         }
-        // Over the scores just read.
         tmem_store16(s_at + 32 * c, high);
         if constexpr (kParts == 2)
           tmem_store16(s_at + 32 * c + 16, low);
+      };
+      if (whole) {
+        tmem_load_start(s_at, x[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_loaded(x[c & 1]);
+          if (c < 3)
+            tmem_load_start(s_at + 32 * (c + 1), x[(c + 1) & 1]);
+          probabilities(c, x[c & 1], 0, true);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          tmem_load(s_at + 32 * c, x[0]);
+          probabilities(c, x[0], visible(c), false);
+        }
       }
       tmem_stored();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
