@@ -11,6 +11,7 @@
 //                   (16 bytes a load, exact in f16) into 128-byte-swizzled
 //                   shared-memory tiles, alternately into a ring of four
 //   warp 12         issues the products: S = Q K^T, then O += P V
+//   warp 13         looks up the pages and scales of the tiles to come
 // Query rows are the tokens of a sequence times the heads that share a kv
 // head, so a tile of keys is converted once for up to 256 rows. The codes'
 // scales stay out of the products: a group of 16 tokens lies in one page, and
@@ -33,10 +34,12 @@ constexpr uint64_t kWaitLimit = 2000000000ull; // ns
 template <int kCh> struct alignas(1024) PromptSmem {
   uint8_t q[2][kCh * kPanel];    // query tiles, or the two parts of one
   uint8_t kv[4][kCh * kPanel];   // keys of tile j at 2 (j % 2), values after
-  float4 scale[4][8];            // of tile j % 4: key scale, log2 and inverse of the value scale
+  // Of tile j % 4's groups of 16 tokens: key scale, log2 and inverse of the
+  // value scale, and where the keys begin in units of a group's keys (-1: none).
+  float4 scale[4][8];
   float coef[2 * kTile];         // what turns a row's product into an exponent
   float join[3][kTile];
-  uint64_t kv_full[4], kv_empty[4], scale_full[4];
+  uint64_t kv_full[4], kv_empty[4], index_full[4];
   uint64_t s_full[2], p_full[2], o_full[2], done;
   uint32_t tmem;
   int failed;
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     for (int i = 0; i < 4; ++i) {
       bar_init(&sm.kv_full[i], 128);
       bar_init(&sm.kv_empty[i], 1);
-      bar_init(&sm.scale_full[i], 1);
+      bar_init(&sm.index_full[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(&sm.s_full[i], 1);
@@ -362,29 +365,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     // ----------------------------------------------------------- products
     if (lane == 0) {
       constexpr uint32_t kS = idesc_f16(kTile, kTile, false), kO = idesc_f16(kTile, kD, true);
-      const uint32_t q_at = smem_at(sm.q), kv_at = smem_at(sm.kv);
+      // An address in a descriptor counts 16 bytes in its low bits, so a step
+      // is an addition (one thread issues every product: building descriptors
+      // anew for each took longer than the products).
+      const uint64_t q_desc = desc_k_major(smem_at(sm.q)), k_desc = desc_k_major(smem_at(sm.kv)),
+                     v_desc = desc_mn_major(smem_at(sm.kv));
+      constexpr uint32_t kSlot = kCh * kPanel / 16;
       auto scores = [&](int st, int tile) { // S of stream st
-        const uint32_t qt = q_at + (kShare ? 0 : st) * kCh * kPanel;
-        const uint32_t kt = kv_at + 2 * (tile & 1) * kCh * kPanel;
+        const uint64_t qt = q_desc + (kShare ? 0 : st) * kSlot;
+        const uint64_t kt = k_desc + 2 * (tile & 1) * kSlot;
+        const uint32_t to = tmem + st * kTile;
 #pragma unroll
         for (int part = 0; part < kParts; ++part) // the small part first
 #pragma unroll
           for (int i = 0; i < 4 * kCh; ++i) {
-            const uint32_t step = (i / 4) * kPanel + (i % 4) * 32;
-            mma_ss(tmem + st * kTile, desc_k_major(qt + (kParts - 1 - part) * kCh * kPanel + step),
-                   desc_k_major(kt + step), kS, part + i > 0);
+            const uint32_t step = ((i / 4) * kPanel + (i % 4) * 32) / 16;
+            mma_ss(to, qt + ((kParts - 1 - part) * kSlot + step), kt + step, kS, part + i > 0);
           }
         commit(&sm.s_full[st]);
       };
       auto outputs = [&](int st, int tile, bool fresh) { // O of stream st
-        const uint32_t vt = kv_at + (2 * (tile & 1) + 1) * kCh * kPanel;
+        const uint64_t vt = v_desc + (2 * (tile & 1) + 1) * kSlot;
+        const uint32_t to = tmem + 2 * kTile + st * kD, from = tmem + st * kTile;
 #pragma unroll
         for (int part = 0; part < kParts; ++part)
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            mma_ts(tmem + 2 * kTile + st * kD,
-                   tmem + st * kTile + (i / 2) * 32 + (i % 2) * 8 + (kParts - 1 - part) * 16,
-                   desc_mn_major(vt + i * 2048), kO, !fresh || part + i > 0);
+            mma_ts(to, from + ((i / 2) * 32 + (i % 2) * 8 + (kParts - 1 - part) * 16),
+                   vt + i * (2048 / 16), kO, !fresh || part + i > 0);
         commit(&sm.o_full[st]);
       };
       bool ok = true;
@@ -454,33 +462,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     const int token = kCh == 2 ? (quarter >> 1) * 2 + (r >> 2) : quarter * 2 + (r >> 2);
     const int part = kCh == 2 ? (quarter & 1) * 4 + (r & 3) : (r & 3);
     const bool inside = part * 16 < v.dim;
-    const int64_t per_page = static_cast<int64_t>(v.heads) * 2 << v.block_log2;
-    const int in_page = (1 << v.block_log2) - 1;
-
-    // Lane i (mod 8) holds the page of the tile's i-th group of 16 tokens.
-    auto pages_of = [&](int tile) {
-      int page = -1;
-      const int key = key_base + tile * kTile + (lane & 7) * 16;
-      if (tile < count && key < s.length) {
-        page = kv_page(v, b, key >> v.block_log2);
-        if (page < 0 && t < 8)
-          atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
-      }
-      return page;
-    };
-    uint4 hold[2][kSteps];
-    auto load = [&](int tile, int side, int pages, uint4 (&to)[kSteps]) {
-      const int key0 = key_base + tile * kTile;
+    const int lane_at = (token & 15) * v.dim + part * 16, side_at = v.dim << v.block_log2;
+    // 16-byte pieces of a tile's keys or values, all in flight at once.
+    auto load = [&](int tile, int side, uint4 (&to)[kSteps]) {
+      const float4 *index = sm.scale[tile & 3];
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        const int at = i * kTokens + token;
-        const int page = __shfl_sync(0xffffffffu, pages, at >> 4);
+        const int place = __float_as_int(index[(i * kTokens + token) >> 4].w);
         to[i] = make_uint4(0, 0, 0, 0);
-        if (page >= 0 && inside) {
-          const int64_t row = page * per_page + (static_cast<int64_t>(head * 2 + side) << v.block_log2) +
-                              ((key0 + at) & in_page);
-          to[i] = __ldg(reinterpret_cast<const uint4 *>(v.codes + row * v.dim + part * 16));
-        }
+        if (place >= 0 && inside)
+          to[i] = __ldg(reinterpret_cast<const uint4 *>(
+              v.codes + static_cast<int64_t>(place) * (16 * v.dim) + side * side_at + lane_at));
       }
     };
     auto store = [&](int slot, const uint4 (&from)[kSteps]) {
@@ -499,41 +491,78 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         *reinterpret_cast<uint4 *>(row + (((chunk + 1) ^ (at & 7)) << 4)) = y;
       }
     };
-    int pages = pages_of(0), next = pages_of(1);
-    load(0, 0, pages, hold[0]);
+    uint4 hold[2][kSteps];
+    if (count > 0 && bar_wait(&sm.index_full[0], 0, failed)) {
+      load(0, 0, hold[0]);
+      load(0, 1, hold[1]);
+    }
     for (int j = 0; j < count; ++j) {
       const int slot = 2 * (j & 1), round = j >> 1;
-      load(j, 1, pages, hold[1]);
-      if (t < 8) { // scales of the tile's groups
-        float4 sc = make_float4(0.0f, -INFINITY, 0.0f, 0.0f); // hidden
-        if (pages >= 0) {
-          const float2 two = *reinterpret_cast<const float2 *>(
-              v.scales + (static_cast<int64_t>(pages) * v.heads + head) * 2);
-          const float sv = fmaxf(two.y, kKvLeastScale);
-          sc = make_float4(two.x, log2f(sv), 1.0f / sv, 0.0f);
-        }
-        sm.scale[j & 3][t] = sc;
-      }
-      if (t < 32) {
-        __syncwarp();
-        if (t == 0)
-          bar_arrive(&sm.scale_full[j & 3]);
-      }
+      const bool more = j + 1 < count;
       if (round > 0 && !bar_wait(&sm.kv_empty[slot], (round - 1) & 1, failed))
         break;
       store(slot, hold[0]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_arrive(&sm.kv_full[slot]);
-      const int after = pages_of(j + 2);
-      if (j + 1 < count)
-        load(j + 1, 0, next, hold[0]);
+      if (more) {
+        if (!bar_wait(&sm.index_full[(j + 1) & 3], ((j + 1) >> 2) & 1, failed))
+          break;
+        load(j + 1, 0, hold[0]);
+      }
       if (round > 0 && !bar_wait(&sm.kv_empty[slot + 1], (round - 1) & 1, failed))
         break;
       store(slot + 1, hold[1]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_arrive(&sm.kv_full[slot + 1]);
-      pages = next;
-      next = after;
+      if (more)
+        load(j + 1, 1, hold[1]);
+    }
+  } else if (warp == 13) {
+    // --------------------------------------------------------- pages, scales
+    // Lane i takes the tile's i-th group of 16 tokens; table entries are loaded
+    // two tiles ahead and scales one, so that neither is waited for here.
+    const int per_page = v.block_log2 - 4;
+    auto entry_of = [&](int tile) { // the table's entry, unchecked; -1: no token
+      const int key = key_base + tile * kTile + (lane & 7) * 16;
+      return tile < count && key < s.length ? v.table[b * v.table_stride + (key >> v.block_log2)]
+                                            : -1;
+    };
+    auto scales_of = [&](int tile, int entry, int &place) {
+      const int key = key_base + tile * kTile + (lane & 7) * 16;
+      const bool good = entry >= 0 && entry < v.pages;
+      if (!good && lane < 8 && tile < count && key < s.length)
+        atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
+      place = good ? (((entry * v.heads + head) * 2) << per_page) +
+                         ((key >> 4) & ((1 << per_page) - 1))
+                   : -1;
+      return good ? *reinterpret_cast<const float2 *>(
+                        v.scales + (static_cast<int64_t>(entry) * v.heads + head) * 2)
+                  : make_float2(0.0f, 0.0f);
+    };
+    int place, entry = entry_of(0), next_entry = entry_of(1);
+    float2 two = scales_of(0, entry, place);
+    for (int j = 0; j < count; ++j) {
+      const int after = entry_of(j + 2);
+      int next_place;
+      const float2 next = scales_of(j + 1, next_entry, next_place);
+      // Slot j % 4 held tile j - 4, whose readers are done when the values of
+      // tile j - 3 have been used. (They cannot be overtaken by those of tile
+      // j - 1, which are converted after this index has been read.)
+      const bool ok = j < 4 || bar_wait(&sm.kv_empty[2 * ((j - 3) & 1) + 1], ((j - 3) >> 1) & 1, failed);
+      if (!__all_sync(0xffffffffu, ok))
+        break;
+      if (lane < 8) {
+        const float sv = fmaxf(two.y, kKvLeastScale);
+        sm.scale[j & 3][lane] = place < 0
+                                    ? make_float4(0.0f, -INFINITY, 0.0f, __int_as_float(-1)) // hidden
+                                    : make_float4(two.x, log2f(sv), 1.0f / sv, __int_as_float(place));
+      }
+      __syncwarp();
+      if (lane == 0)
+        bar_arrive(&sm.index_full[j & 3]);
+      two = next;
+      place = next_place;
+      next_entry = after;
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------- softmax
@@ -559,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         const int x = min(max(from - 32 * c, 0), 32), y = min(max(to - 32 * c, 0), 32);
         return y > x ? (0xffffffffu >> (32 - (y - x))) << x : 0u;
       };
-      ok = bar_wait(&sm.scale_full[tile & 3], (tile >> 2) & 1, failed) &&
+      ok = bar_wait(&sm.index_full[tile & 3], (tile >> 2) & 1, failed) &&
            bar_wait(&sm.s_full[st], n & 1, failed);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok)
