@@ -1,17 +1,22 @@
 // kv_attention_tc.cu - attention of prompts and chunks over the 8-bit cache on
 // the tensor cores (tcgen05, operands and accumulators in TMEM).
 //
-// Bound by the tensor cores and, about as much, by the exponentials: a 128 x
-// 128 tile of scores takes 2 x 512 cycles of f16 products (head_dim 128) and
-// 1,024 of the special-function units. A CTA therefore runs two streams of
-// 128 query rows, so that one's products cover the other's softmax:
-//   warps 0-3, 4-7  softmax of stream 0 and 1: a thread a row, scores from
-//                   TMEM, probabilities back over them as the f16 A operand
-//   warps 8-11      converters: 128-token tiles of keys and values, int8 codes
-//                   (16 bytes a load, exact in f16) into 128-byte-swizzled
-//                   shared-memory tiles, alternately into a ring of four
+// Bound by the tensor cores, shared memory and the exponentials, about equally:
+// 128 rows x 128 keys (head_dim 128) take 2 x 512 cycles of f16 products, whose
+// operands fill shared memory's 128 bytes a cycle, and 1,024 of the
+// special-function units. A CTA therefore runs two streams of 128 query rows,
+// so that one's products cover the other's softmax:
+//   warps 0-3, 4-7  softmax of stream 0 and 1: a thread a row, its 128 scores
+//                   from TMEM into registers (which these warps take over from
+//                   the others), probabilities back over them as the f16 A
+//                   operand
+//   warps 8-11      converters: 64 tokens of keys, then of values, at a time,
+//                   int8 codes (16 bytes a load, exact in f16) into
+//                   128-byte-swizzled tiles of 128 tokens, two each
 //   warp 12         issues the products: S = Q K^T, then O += P V
-//   warp 13         looks up the pages and scales of the tiles to come
+//   warp 13         looks up the pages and scales of the tokens to come
+// (Two buffers of 64 keys a stream, which let products run ahead, were slower:
+// a product of 64 keys still reads all of its query tile.)
 // Query rows are the tokens of a sequence times the heads that share a kv
 // head, so a tile of keys is converted once for up to 256 rows. The codes'
 // scales stay out of the products: a group of 16 tokens lies in one page, and
@@ -27,19 +32,21 @@
 namespace cim {
 namespace {
 
-constexpr int kThreads = 512, kTile = 128;
-constexpr int kPanel = kTile * 128; // bytes: 128 rows of 64 f16
+constexpr int kThreads = 512, kM = 128, kTile = 128; // query rows a stream, keys a tile
+constexpr int kSub = 64, kIndex = 8; // tokens converted at a time, and indexed ahead
+constexpr int kPanel = 128 * 128;    // bytes: 128 rows of 64 f16
 constexpr uint64_t kWaitLimit = 2000000000ull; // ns
 
 template <int kCh> struct alignas(1024) PromptSmem {
-  uint8_t q[2][kCh * kPanel];    // query tiles, or the two parts of one
-  uint8_t kv[4][kCh * kPanel];   // keys of tile j at 2 (j % 2), values after
-  // Of tile j % 4's groups of 16 tokens: key scale, log2 and inverse of the
+  uint8_t q[2][kCh * kPanel]; // query tiles, or the two parts of one
+  uint8_t kv[2][2][kCh * kPanel]; // keys and values of tile j at j % 2
+  // Of the groups of 16 tokens of part j (64 tokens) at j % kIndex: key scale, log2 and inverse of the
   // value scale, and where the keys begin in units of a group's keys (-1: none).
-  float4 scale[4][8];
-  float coef[2 * kTile];         // what turns a row's product into an exponent
-  float join[3][kTile];
-  uint64_t kv_full[4], kv_empty[4], index_full[4];
+  float4 scale[kIndex][kSub / 16];
+  float coef[2 * kM];            // what turns a row's product into an exponent
+  float join[2][kM];
+  uint64_t kv_full[2][4], kv_empty[2][2]; // of parts and of tiles
+  uint64_t index_full[kIndex], index_empty[kIndex];
   uint64_t s_full[2], p_full[2], o_full[2], done;
   uint32_t tmem;
   int failed;
@@ -86,13 +93,13 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *fa
 
 // Matrix descriptors, 128-byte swizzle. K-major (queries, keys): rows of 128
 // bytes in 1024-byte atoms. MN-major (values): a row holds 64 elements of one
-// token; 64-element panels kPanel apart, 8-token atoms 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t at) {
-  return ((at & 0x3ffffull) >> 4) | (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 46) |
-         (uint64_t{2} << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t at) {
-  return desc_k_major(at) | (uint64_t{kPanel >> 4} << 16);
+// token; 64-element panels kPanel apart, 8-token atoms 1024 bytes apart. The
+// low word counts the address in 16 bytes, so a step within a tile is an
+// addition to it; the high word is a constant.
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k_major(uint32_t at) { return (at & 0x3ffff) >> 4; }
+__device__ __forceinline__ uint32_t desc_mn_major(uint32_t at) {
+  return desc_k_major(at) | (kPanel >> 4) << 16;
 }
 
 // kind::f16 with f16 A and B and f32 accumulators (format 1 at bit 4); B is
@@ -102,20 +109,30 @@ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) {
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                        uint32_t accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-               "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+  asm volatile("{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n"
+               " mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d),
+               "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
                : "memory");
 }
 
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                        uint32_t accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-               "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+  asm volatile("{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n"
+               " mov.b64 b, {%2, %5};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d),
+               "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
                : "memory");
+}
+
+// One thread of a converged warp.
+__device__ __forceinline__ bool elect() {
+  uint32_t yes;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(yes));
+  return yes != 0;
 }
 
 __device__ __forceinline__ void commit(uint64_t *bar) {
@@ -191,15 +208,29 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, "
-               "%9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
-               "%24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-               "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-               "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-               "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
-               "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+// In the order written: all of a tile's at once would not leave registers for
+// its scores.
+__device__ __forceinline__ float4 load_scale(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+               "tcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7])
+               : "r"(at)
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
 
@@ -253,14 +284,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   PromptSmem<kCh> &sm =
       *reinterpret_cast<PromptSmem<kCh> *>(raw + ((1024u - (smem_at(raw) & 1023u)) & 1023u));
   const KvView &v = a.v;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kRows = kShare ? kTile : 2 * kTile; // query rows of this CTA
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  constexpr int kRows = kShare ? kM : 2 * kM; // query rows of this CTA
   constexpr int kD = 64 * kCh;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4; ++i) {
-      bar_init(&sm.kv_full[i], 128);
-      bar_init(&sm.kv_empty[i], 1);
+    for (int side = 0; side < 2; ++side) {
+      for (int i = 0; i < 4; ++i)
+        bar_init(&sm.kv_full[side][i], 128);
+      for (int i = 0; i < 2; ++i)
+        bar_init(&sm.kv_empty[side][i], 1);
+    }
+    for (int i = 0; i < kIndex; ++i) {
       bar_init(&sm.index_full[i], 1);
+      // The converters' warps, and those of the streams that take the part.
+      bar_init(&sm.index_empty[i], 4 + (kShare ? 4 : 8));
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(&sm.s_full[i], 1);
@@ -297,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   int lo, hi;
   key_range(a, s.length, offset + f0 / a.group, offset + last / a.group, lo, hi);
   const int first16 = lo >> 4;
-  const int all = (((hi + 15) >> 4) - first16 + 7) / 8; // tiles of 128 keys
+  const int all = (((hi + 15) >> 4) - first16 + kTile / 16 - 1) / (kTile / 16); // tiles
   const int each = (all + a.splits - 1) / a.splits;
   const int tile0 = min(all, split * each), count = min(all, tile0 + each) - tile0;
   const int key_base = (first16 << 4) + tile0 * kTile; // of this CTA's tile 0
@@ -342,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       const float2 back = unpack_half(h[i / 2]);
       l[i / 2] = pack_half(y0 - back.x, y1 - back.y);
     }
-    uint8_t *to = sm.q[kShare ? 0 : r / kTile] + (d / 64) * kPanel + (r % kTile) * 128 +
+    uint8_t *to = sm.q[kShare ? 0 : r / kM] + (d / 64) * kPanel + (r % kM) * 128 +
                   ((((d % 64) / 8) ^ (r & 7)) << 4) + (d % 8) * 2;
     if constexpr (kCh == 2) {
       *reinterpret_cast<uint2 *>(to) = make_uint2(h[0], h[1]);
@@ -358,223 +395,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = sm.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0); // columns: scores [stream][128], outputs [stream][kD]
   int *failed = &sm.failed;
 
-  if (warp == 12) {
-    // ----------------------------------------------------------- products
-    if (lane == 0) {
-      constexpr uint32_t kS = idesc_f16(kTile, kTile, false), kO = idesc_f16(kTile, kD, true);
-      // An address in a descriptor counts 16 bytes in its low bits, so a step
-      // is an addition (one thread issues every product: building descriptors
-      // anew for each took longer than the products).
-      const uint64_t q_desc = desc_k_major(smem_at(sm.q)), k_desc = desc_k_major(smem_at(sm.kv)),
-                     v_desc = desc_mn_major(smem_at(sm.kv));
-      constexpr uint32_t kSlot = kCh * kPanel / 16;
-      auto scores = [&](int st, int tile) { // S of stream st
-        const uint64_t qt = q_desc + (kShare ? 0 : st) * kSlot;
-        const uint64_t kt = k_desc + 2 * (tile & 1) * kSlot;
-        const uint32_t to = tmem + st * kTile;
-#pragma unroll
-        for (int part = 0; part < kParts; ++part) // the small part first
-#pragma unroll
-          for (int i = 0; i < 4 * kCh; ++i) {
-            const uint32_t step = ((i / 4) * kPanel + (i % 4) * 32) / 16;
-            mma_ss(to, qt + ((kParts - 1 - part) * kSlot + step), kt + step, kS, part + i > 0);
-          }
-        commit(&sm.s_full[st]);
-      };
-      auto outputs = [&](int st, int tile, bool fresh) { // O of stream st
-        const uint64_t vt = v_desc + (2 * (tile & 1) + 1) * kSlot;
-        const uint32_t to = tmem + 2 * kTile + st * kD, from = tmem + st * kTile;
-#pragma unroll
-        for (int part = 0; part < kParts; ++part)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            mma_ts(to, from + ((i / 2) * 32 + (i % 2) * 8 + (kParts - 1 - part) * 16),
-                   vt + i * (2048 / 16), kO, !fresh || part + i > 0);
-        commit(&sm.o_full[st]);
-      };
-      bool ok = true;
-      auto wait = [&](uint64_t *bar, uint32_t parity) {
-        ok = ok && bar_wait(bar, parity, failed);
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        return ok;
-      };
-      if constexpr (kShare) {
-        for (int j = 0; j < 2 && j < count; ++j)
-          if (wait(&sm.kv_full[2 * (j & 1)], (j >> 1) & 1)) {
-            scores(j & 1, j);
-            commit(&sm.kv_empty[2 * (j & 1)]);
-          }
-        for (int j = 0; j < count && ok; ++j) {
-          const int st = j & 1, slot = 2 * (j & 1);
-          if (!wait(&sm.kv_full[slot + 1], (j >> 1) & 1) || !wait(&sm.p_full[st], (j >> 1) & 1))
-            break;
-          outputs(st, j, j < 2);
-          commit(&sm.kv_empty[slot + 1]);
-          if (j + 2 < count) {
-            if (!wait(&sm.kv_full[slot], ((j + 2) >> 1) & 1))
-              break;
-            scores(st, j + 2);
-            commit(&sm.kv_empty[slot]);
-          }
-        }
-      } else if (count > 0) {
-        if (wait(&sm.kv_full[0], 0)) {
-          scores(0, 0);
-          scores(1, 0);
-          commit(&sm.kv_empty[0]);
-        }
-        for (int j = 0; j < count && ok; ++j) {
-          const int slot = 2 * (j & 1), next = 2 * ((j + 1) & 1);
-          if (!wait(&sm.kv_full[slot + 1], (j >> 1) & 1))
-            break;
-          for (int st = 0; st < 2 && ok; ++st) {
-            if (!wait(&sm.p_full[st], j & 1))
-              break;
-            outputs(st, j, j == 0);
-            if (st == 1)
-              commit(&sm.kv_empty[slot + 1]);
-            if (j + 1 < count) {
-              if (st == 0 && !wait(&sm.kv_full[next], ((j + 1) >> 1) & 1))
-                break;
-              scores(st, j + 1);
-              if (st == 1)
-                commit(&sm.kv_empty[next]);
-            }
-          }
-        }
-      }
-      // Nothing of this CTA may be in flight when its TMEM is freed.
-      commit(&sm.done);
-      int unused = 0;
-      bar_wait(&sm.done, 0, &unused);
-    }
-  } else if (warp >= 8 && warp < 12) {
-    // ---------------------------------------------------------- converters
-    // A thread loads 16 codes (one token's sixteenth part p of 64 or 128) a
-    // step; eight neighbouring lanes hold two tokens of one panel, so that
-    // their 16-byte stores fall in different banks.
-    constexpr int kSteps = 4 * kCh;          // steps of kTile tokens
-    constexpr int kTokens = kTile / kSteps;  // tokens a step
-    const int t = threadIdx.x - 256, quarter = t >> 3, r = t & 7;
-    const int token = kCh == 2 ? (quarter >> 1) * 2 + (r >> 2) : quarter * 2 + (r >> 2);
-    const int part = kCh == 2 ? (quarter & 1) * 4 + (r & 3) : (r & 3);
-    const bool inside = part * 16 < v.dim;
-    const int lane_at = (token & 15) * v.dim + part * 16, side_at = v.dim << v.block_log2;
-    // 16-byte pieces of a tile's keys or values, all in flight at once.
-    auto load = [&](int tile, int side, uint4 (&to)[kSteps]) {
-      const float4 *index = sm.scale[tile & 3];
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int place = __float_as_int(index[(i * kTokens + token) >> 4].w);
-        to[i] = make_uint4(0, 0, 0, 0);
-        if (place >= 0 && inside)
-          to[i] = __ldg(reinterpret_cast<const uint4 *>(
-              v.codes + static_cast<int64_t>(place) * (16 * v.dim) + side * side_at + lane_at));
-      }
-    };
-    auto store = [&](int slot, const uint4 (&from)[kSteps]) {
-      uint8_t *base = sm.kv[slot] + (part / 4) * kPanel;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int at = i * kTokens + token;
-        uint4 x, y;
-        codes_to_half(from[i].x, x.x, x.y);
-        codes_to_half(from[i].y, x.z, x.w);
-        codes_to_half(from[i].z, y.x, y.y);
-        codes_to_half(from[i].w, y.z, y.w);
-        uint8_t *row = base + at * 128;
-        const int chunk = (part & 3) * 2;
-        *reinterpret_cast<uint4 *>(row + ((chunk ^ (at & 7)) << 4)) = x;
-        *reinterpret_cast<uint4 *>(row + (((chunk + 1) ^ (at & 7)) << 4)) = y;
-      }
-    };
-    uint4 hold[2][kSteps];
-    if (count > 0 && bar_wait(&sm.index_full[0], 0, failed)) {
-      load(0, 0, hold[0]);
-      load(0, 1, hold[1]);
-    }
-    for (int j = 0; j < count; ++j) {
-      const int slot = 2 * (j & 1), round = j >> 1;
-      const bool more = j + 1 < count;
-      if (round > 0 && !bar_wait(&sm.kv_empty[slot], (round - 1) & 1, failed))
-        break;
-      store(slot, hold[0]);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(&sm.kv_full[slot]);
-      if (more) {
-        if (!bar_wait(&sm.index_full[(j + 1) & 3], ((j + 1) >> 2) & 1, failed))
-          break;
-        load(j + 1, 0, hold[0]);
-      }
-      if (round > 0 && !bar_wait(&sm.kv_empty[slot + 1], (round - 1) & 1, failed))
-        break;
-      store(slot + 1, hold[1]);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(&sm.kv_full[slot + 1]);
-      if (more)
-        load(j + 1, 1, hold[1]);
-    }
-  } else if (warp == 13) {
-    // --------------------------------------------------------- pages, scales
-    // Lane i takes the tile's i-th group of 16 tokens; table entries are loaded
-    // two tiles ahead and scales one, so that neither is waited for here.
-    const int per_page = v.block_log2 - 4;
-    auto entry_of = [&](int tile) { // the table's entry, unchecked; -1: no token
-      const int key = key_base + tile * kTile + (lane & 7) * 16;
-      return tile < count && key < s.length ? v.table[b * v.table_stride + (key >> v.block_log2)]
-                                            : -1;
-    };
-    auto scales_of = [&](int tile, int entry, int &place) {
-      const int key = key_base + tile * kTile + (lane & 7) * 16;
-      const bool good = entry >= 0 && entry < v.pages;
-      if (!good && lane < 8 && tile < count && key < s.length)
-        atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
-      place = good ? (((entry * v.heads + head) * 2) << per_page) +
-                         ((key >> 4) & ((1 << per_page) - 1))
-                   : -1;
-      return good ? *reinterpret_cast<const float2 *>(
-                        v.scales + (static_cast<int64_t>(entry) * v.heads + head) * 2)
-                  : make_float2(0.0f, 0.0f);
-    };
-    int place, entry = entry_of(0), next_entry = entry_of(1);
-    float2 two = scales_of(0, entry, place);
-    for (int j = 0; j < count; ++j) {
-      const int after = entry_of(j + 2);
-      int next_place;
-      const float2 next = scales_of(j + 1, next_entry, next_place);
-      // Slot j % 4 held tile j - 4, whose readers are done when the values of
-      // tile j - 3 have been used. (They cannot be overtaken by those of tile
-      // j - 1, which are converted after this index has been read.)
-      const bool ok = j < 4 || bar_wait(&sm.kv_empty[2 * ((j - 3) & 1) + 1], ((j - 3) >> 1) & 1, failed);
-      if (!__all_sync(0xffffffffu, ok))
-        break;
-      if (lane < 8) {
-        const float sv = fmaxf(two.y, kKvLeastScale);
-        sm.scale[j & 3][lane] = place < 0
-                                    ? make_float4(0.0f, -INFINITY, 0.0f, __int_as_float(-1)) // hidden
-                                    : make_float4(two.x, log2f(sv), 1.0f / sv, __int_as_float(place));
-      }
-      __syncwarp();
-      if (lane == 0)
-        bar_arrive(&sm.index_full[j & 3]);
-      two = next;
-      place = next_place;
-      next_entry = after;
-    }
-  } else if (warp < 8) {
+  // Registers: 128 a thread at launch, 256 x 168 + 256 x 88 from here on
+  // (the launch checks that it has them).
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ------------------------------------------------------------- softmax
     const int st = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + st * kTile + lanes, o_at = tmem + 2 * kTile + st * kD + lanes;
-    const int f = f0 + (kShare ? 0 : st * kTile) + row;
+    const int f = f0 + (kShare ? 0 : st * kM) + row;
     const bool live = f < rows;
     const int pos = offset + (live ? f / a.group : 0);
     const int row_hi = !live ? 0 : a.causal ? min(s.length, pos + 1) : s.length;
     const int row_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const float coef = sm.coef[kShare ? row : st * kTile + row];
+    const float coef = sm.coef[kShare ? row : st * kM + row];
     float m = -INFINITY, l = 0.0f;
     const int mine = kShare ? (count - st + 1) / 2 : count;
     bool ok = true;
@@ -588,50 +425,58 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         const int x = min(max(from - 32 * c, 0), 32), y = min(max(to - 32 * c, 0), 32);
         return y > x ? (0xffffffffu >> (32 - (y - x))) << x : 0u;
       };
-      ok = bar_wait(&sm.index_full[tile & 3], (tile >> 2) & 1, failed) &&
+      const int part0 = (2 * tile) % kIndex;
+      ok = bar_wait(&sm.index_full[part0], (2 * tile / kIndex) & 1, failed) &&
+           bar_wait(&sm.index_full[part0 + 1], (2 * tile / kIndex) & 1, failed) &&
            bar_wait(&sm.s_full[st], n & 1, failed);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok)
         break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const float4 *scale = sm.scale[tile & 3];
+      const uint32_t scale_at = smem_at(sm.scale[part0]); // of the tile's eight groups
       // The largest exponent of the row, t = score * log2(e) + log2(scale of v).
       float top = -INFINITY;
-      uint32_t x[2][32];
-      tmem_load_start(s_at, x[0]);
-      if (whole) {
+      // One part: the scores stay in registers. Two: there is no room beside
+      // both parts, they are read again.
+      constexpr bool kHold = kParts == 1;
+      uint32_t x[kHold ? 4 : 1][32];
+      auto hide = [&](int c, uint32_t (&y)[32]) {
+        const uint32_t seen = visible(c);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_loaded(x[c & 1]);
-          if (c < 3)
-            tmem_load_start(s_at + 32 * (c + 1), x[(c + 1) & 1]);
+        for (int i = 0; i < 32; ++i)
+          y[i] = seen >> i & 1 ? y[i] : 0xff800000u; // -infinity: hidden
+      };
+      if constexpr (kHold) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const uint32_t *y = x[c & 1] + 16 * g;
-            float best = __uint_as_float(y[0]);
+        for (int c = 0; c < 4; ++c)
+          tmem_load_start(s_at + 32 * c, x[c]);
 #pragma unroll
-            for (int i = 1; i < 15; i += 2)
-              best = max3(best, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
-            best = fmaxf(best, __uint_as_float(y[15]));
-            const float4 sc = scale[2 * c + g];
-            top = nan_max(top, fmaf(best, coef * sc.x, sc.y));
-          }
+        for (int c = 0; c < 4; ++c)
+          tmem_loaded(x[c]);
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            hide(c, x[c]);
         }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if constexpr (!kHold) {
           tmem_load(s_at + 32 * c, x[0]);
-          const uint32_t seen = visible(c);
+          if (!whole)
+            hide(c, x[0]);
+        }
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float best = -INFINITY;
+        for (int g = 0; g < 2; ++g) {
+          const uint32_t *y = x[kHold ? c : 0] + 16 * g;
+          float best = __uint_as_float(y[0]);
 #pragma unroll
-            for (int i = 16 * g; i < 16 * g + 16; ++i)
-              best = fmaxf(best, seen >> i & 1 ? __uint_as_float(x[0][i]) : -INFINITY);
-            const float4 sc = scale[2 * c + g];
-            if (best != -INFINITY)
-              top = nan_max(top, fmaf(best, coef * sc.x, sc.y));
-          }
+          for (int i = 1; i < 15; i += 2)
+            best = max3(best, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+          best = fmaxf(best, __uint_as_float(y[15]));
+          const float4 sc = load_scale(scale_at + (2 * c + g) * 16);
+          if (whole || best != -INFINITY)
+            top = nan_max(top, fmaf(best, coef * sc.x, sc.y));
         }
       }
       // Set the row's reference again when its probabilities outgrow f16.
@@ -648,32 +493,40 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
             break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-          for (int c = 0; c < 2 * kCh; ++c) {
-            uint32_t x[32];
-            tmem_load(o_at + 32 * c, x);
+          for (int c = 0; c < 8 * kCh; ++c) { // few columns at a time: the scores are held
+            uint32_t y[8];
+            tmem_load8(o_at + 8 * c, y);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              x[i] = __float_as_uint(__uint_as_float(x[i]) * shrink);
-            tmem_store32(o_at + 32 * c, x);
+            for (int i = 0; i < 8; ++i)
+              y[i] = __float_as_uint(__uint_as_float(y[i]) * shrink);
+            tmem_store8(o_at + 8 * c, y);
           }
         }
       }
       const float origin = m == -INFINITY ? 0.0f : m;
-      // Probabilities of 32 scores, over the scores just read.
-      auto probabilities = [&](int c, const uint32_t (&y)[32], uint32_t seen, bool all) {
+      // Probabilities over the scores just read: of every 32 columns 16 hold
+      // their f16, the next 16 the small parts.
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if constexpr (!kHold) {
+          tmem_load(s_at + 32 * c, x[0]);
+          if (!whole)
+            hide(c, x[0]);
+        }
+        const uint32_t *y = x[kHold ? c : 0];
         uint32_t high[16], low[16];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const float4 sc = scale[2 * c + g];
+          const float4 sc = load_scale(scale_at + (2 * c + g) * 16);
           const float slope = coef * sc.x, shift = sc.y - origin;
           float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (int i = 16 * g; i < 16 * g + 16; i += 2) {
             float2 e = fma2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])),
                             make_float2(slope, slope), make_float2(shift, shift));
-            if (!all) {
-              e.x = seen >> i & 1 ? e.x : -INFINITY;
-              e.y = seen >> (i + 1) & 1 ? e.y : -INFINITY;
+            if (!whole) { // a slope of zero has made NaN of what is hidden
+              e.x = y[i] == 0xff800000u ? -INFINITY : e.x;
+              e.y = y[i + 1] == 0xff800000u ? -INFINITY : e.y;
             }
             const float2 p = make_float2(exp2_approx(e.x), exp2_approx(e.y));
             sum = add2(sum, p);
@@ -688,33 +541,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         tmem_store16(s_at + 32 * c, high);
         if constexpr (kParts == 2)
           tmem_store16(s_at + 32 * c + 16, low);
-      };
-      if (whole) {
-        tmem_load_start(s_at, x[0]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_loaded(x[c & 1]);
-          if (c < 3)
-            tmem_load_start(s_at + 32 * (c + 1), x[(c + 1) & 1]);
-          probabilities(c, x[c & 1], 0, true);
-        }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          tmem_load(s_at + 32 * c, x[0]);
-          probabilities(c, x[0], visible(c), false);
-        }
       }
       tmem_stored();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       bar_arrive(&sm.p_full[st]);
+      if (lane < 2) // the warp is done with the tile's scales
+        bar_arrive(&sm.index_empty[part0 + lane]);
     }
     if (ok && mine > 0)
       ok = bar_wait(&sm.o_full[st], (mine - 1) & 1, failed);
     ok = __all_sync(0xffffffffu, ok);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     float share = 1.0f, other = 0.0f;
-    float *joined = reinterpret_cast<float *>(sm.kv[0]); // [element][row]
+    float *joined = reinterpret_cast<float *>(sm.kv); // [element][row]
     if constexpr (kShare) {
       // Every product has completed (both streams have waited for theirs).
       asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -728,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
             tmem_load(o_at + 32 * c, x);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              joined[(32 * c + i) * kTile + row] = __uint_as_float(x[i]);
+              joined[(32 * c + i) * kM + row] = __uint_as_float(x[i]);
           }
         }
       }
@@ -760,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
           float o = share == 0.0f ? 0.0f : __uint_as_float(x[k]) * share;
           if constexpr (kShare)
             if (other != 0.0f)
-              o = fmaf(joined[(32 * c + k) * kTile + row], other, o);
+              o = fmaf(joined[(32 * c + k) * kM + row], other, o);
           y[k] = some ? o * scale : 0.0f;
         }
         if (live && ok) {
@@ -792,6 +631,212 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
           a.lse[at] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
       }
     }
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // ---------------------------------------------------------- converters
+    // A thread loads 16 codes of a token a step; eight neighbouring lanes hold two tokens of one panel, so that
+    // their 16-byte stores fall in different banks.
+    constexpr int kSteps = 2 * kCh;         // steps a part of 64 tokens
+    constexpr int kTokens = kSub / kSteps;  // tokens a step
+    const int t = threadIdx.x - 256, quarter = t >> 3, r = t & 7;
+    const int token = kCh == 2 ? (quarter >> 1) * 2 + (r >> 2) : quarter * 2 + (r >> 2);
+    const int part = kCh == 2 ? (quarter & 1) * 4 + (r & 3) : (r & 3);
+    const bool inside = part * 16 < v.dim;
+    const int lane_at = (token & 15) * v.dim + part * 16, side_at = v.dim << v.block_log2;
+    // 16-byte pieces of a part's keys or values, all in flight at once.
+    auto load = [&](int j, int side, uint4 (&to)[kSteps]) {
+      const float4 *index = sm.scale[j % kIndex];
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int place = __float_as_int(index[(i * kTokens + token) >> 4].w);
+        to[i] = make_uint4(0, 0, 0, 0);
+        if (place >= 0 && inside)
+          to[i] = __ldg(reinterpret_cast<const uint4 *>(
+              v.codes + static_cast<int64_t>(place) * (16 * v.dim) + side * side_at + lane_at));
+      }
+    };
+    auto store = [&](int side, int j, const uint4 (&from)[kSteps]) {
+      uint8_t *base = sm.kv[side][(j >> 1) & 1] + (part / 4) * kPanel + (j & 1) * (kSub * 128);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int at = i * kTokens + token;
+        uint4 x, y;
+        codes_to_half(from[i].x, x.x, x.y);
+        codes_to_half(from[i].y, x.z, x.w);
+        codes_to_half(from[i].z, y.x, y.y);
+        codes_to_half(from[i].w, y.z, y.w);
+        uint8_t *row = base + at * 128;
+        const int chunk = (part & 3) * 2;
+        *reinterpret_cast<uint4 *>(row + ((chunk ^ (at & 7)) << 4)) = x;
+        *reinterpret_cast<uint4 *>(row + (((chunk + 1) ^ (at & 7)) << 4)) = y;
+      }
+    };
+    uint4 hold[2][kSteps];
+    const int parts = 2 * count;
+    auto used = [&](int j) { // this warp has read part j's places
+      __syncwarp();
+      if (lane == 0)
+        bar_arrive(&sm.index_empty[j % kIndex]);
+    };
+    bool ok = parts == 0 || bar_wait(&sm.index_full[0], 0, failed);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok && parts > 0) {
+      load(0, 0, hold[0]);
+      load(0, 1, hold[1]);
+      used(0);
+    }
+    for (int j = 0; j < parts && ok; ++j) {
+      const bool more = j + 1 < parts;
+      // A tile's slot was emptied by the product of the tile before last.
+      if (j >= 4)
+        ok = bar_wait(&sm.kv_empty[0][(j >> 1) & 1], ((j >> 2) - 1) & 1, failed);
+      store(0, j, hold[0]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(&sm.kv_full[0][j & 3]);
+      if (more) {
+        ok = bar_wait(&sm.index_full[(j + 1) % kIndex], ((j + 1) / kIndex) & 1, failed) && ok;
+        load(j + 1, 0, hold[0]);
+      }
+      if (j >= 4)
+        ok = bar_wait(&sm.kv_empty[1][(j >> 1) & 1], ((j >> 2) - 1) & 1, failed) && ok;
+      store(1, j, hold[1]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(&sm.kv_full[1][j & 3]);
+      if (more) {
+        load(j + 1, 1, hold[1]);
+        used(j + 1);
+      }
+      ok = __all_sync(0xffffffffu, ok);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 12) {
+      // ----------------------------------------------------------- products
+      constexpr uint32_t kS = idesc_f16(kM, kTile, false), kO = idesc_f16(kM, kD, true);
+      constexpr uint32_t kSlot = kCh * kPanel / 16;
+      const uint32_t q_desc = desc_k_major(smem_at(sm.q)), k_desc = desc_k_major(smem_at(sm.kv[0])),
+                     v_desc = desc_mn_major(smem_at(sm.kv[1]));
+      bool ok = true;
+      auto wait = [&](uint64_t *bar, uint32_t parity) {
+        ok = __all_sync(0xffffffffu, ok && bar_wait(bar, parity, failed));
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        return ok;
+      };
+      // Round n of a stream takes its n-th tile. Rounds go by twos, so that
+      // slots are constants; the warp stays together and elects a thread for
+      // each run of products, so that their operands are uniform (one thread
+      // by itself took twice as long to issue a product as the product does).
+      const int rounds = kShare ? (count + 1) / 2 : count;
+      auto ready = [&](int side, int tile, int slot) { // both parts of a tile
+        return wait(&sm.kv_full[side][2 * slot], (tile >> 1) & 1) &&
+               wait(&sm.kv_full[side][2 * slot + 1], (tile >> 1) & 1);
+      };
+      auto scores = [&](int st, int n, int u) { // u = n mod 2
+        const int tile = kShare ? 2 * n + st : n, slot = kShare ? st : u;
+        if (tile >= count || !ready(0, tile, slot))
+          return;
+        if (elect()) {
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) // the small part first
+#pragma unroll
+            for (int i = 0; i < 4 * kCh; ++i)
+              mma_ss(tmem + st * kTile,
+                     q_desc + ((kShare ? 0 : st) * kSlot + (kParts - 1 - part) * kSlot +
+                               ((i / 4) * kPanel + (i % 4) * 32) / 16),
+                     k_desc + (slot * kSlot + ((i / 4) * kPanel + (i % 4) * 32) / 16), kS,
+                     part + i > 0);
+          commit(&sm.s_full[st]);
+          if (kShare || st == 1)
+            commit(&sm.kv_empty[0][slot]);
+        }
+        __syncwarp();
+      };
+      auto outputs = [&](int st, int n, int u) {
+        const int tile = kShare ? 2 * n + st : n, slot = kShare ? st : u;
+        if (tile >= count || !ready(1, tile, slot) || !wait(&sm.p_full[st], n & 1))
+          return;
+        if (elect()) {
+#pragma unroll
+          for (int part = 0; part < kParts; ++part)
+#pragma unroll
+            for (int i = 0; i < kTile / 16; ++i)
+              mma_ts(tmem + 2 * kTile + st * kD,
+                     tmem + st * kTile + ((i / 2) * 32 + (i % 2) * 8 + (kParts - 1 - part) * 16),
+                     v_desc + (slot * kSlot + i * (2048 / 16)), kO, n > 0 || part + i > 0);
+          commit(&sm.o_full[st]);
+          if (kShare || st == 1)
+            commit(&sm.kv_empty[1][slot]);
+        }
+        __syncwarp();
+      };
+      scores(0, 0, 0);
+      if (ok)
+        scores(1, 0, 0);
+#pragma unroll 1
+      for (int n0 = 0; n0 < rounds && ok; n0 += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            if (ok)
+              outputs(st, n0 + u, u);
+            if (ok)
+              scores(st, n0 + u + 1, u ^ 1);
+          }
+      }
+      // Nothing of this CTA may be in flight when its TMEM is freed.
+      if (elect())
+        commit(&sm.done);
+      __syncwarp();
+      int unused = 0;
+      bar_wait(&sm.done, 0, &unused);
+    } else if (warp == 13) {
+      // --------------------------------------------------------- pages, scales
+      // Lane i takes a part's i-th group of 16 tokens; table entries are loaded
+      // two parts ahead and scales one, so that neither is waited for here.
+      const int per_page = v.block_log2 - 4;
+      const int parts = 2 * count;
+      auto key_of = [&](int j) { return key_base + j * kSub + (lane & 3) * 16; };
+      auto entry_of = [&](int j) { // the table's entry, unchecked; -1: no token
+        const int key = key_of(j);
+        return j < parts && key < s.length ? v.table[b * v.table_stride + (key >> v.block_log2)] : -1;
+      };
+      auto scales_of = [&](int j, int entry, int &place) {
+        const int key = key_of(j);
+        const bool good = entry >= 0 && entry < v.pages;
+        if (!good && lane < 4 && j < parts && key < s.length)
+          atomicOr(a.status, CIM22_STATUS_CACHE_INDEX);
+        place = good ? (((entry * v.heads + head) * 2) << per_page) +
+                           ((key >> 4) & ((1 << per_page) - 1))
+                     : -1;
+        return good ? *reinterpret_cast<const float2 *>(
+                          v.scales + (static_cast<int64_t>(entry) * v.heads + head) * 2)
+                    : make_float2(0.0f, 0.0f);
+      };
+      int place, entry = entry_of(0), next_entry = entry_of(1);
+      float2 two = scales_of(0, entry, place);
+      for (int j = 0; j < parts; ++j) {
+        const int after = entry_of(j + 2);
+        int next_place;
+        const float2 next = scales_of(j + 1, next_entry, next_place);
+        const bool ok = j < kIndex ||
+                        bar_wait(&sm.index_empty[j % kIndex], ((j / kIndex) - 1) & 1, failed);
+        if (!__all_sync(0xffffffffu, ok))
+          break;
+        if (lane < 4) {
+          const float sv = fmaxf(two.y, kKvLeastScale);
+          sm.scale[j % kIndex][lane] = place < 0
+                                      ? make_float4(0.0f, -INFINITY, 0.0f, __int_as_float(-1)) // hidden
+                                      : make_float4(two.x, log2f(sv), 1.0f / sv, __int_as_float(place));
+        }
+        __syncwarp();
+        if (lane == 0)
+          bar_arrive(&sm.index_full[j % kIndex]);
+        two = next;
+        place = next_place;
+        next_entry = after;
+      }
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -810,6 +855,14 @@ cudaError_t launch_prompt(const KvAttendArgs &a, int tiles, cudaStream_t stream)
   static DynamicSmem allowed;
   if (const cudaError_t e = allowed.allow(kernel, bytes); e != cudaSuccess)
     return e;
+  // The softmax warps wait for registers that the others give up: there have to
+  // be as many as the kernel hands around.
+  static const int registers = [&] {
+    cudaFuncAttributes attr{};
+    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
+  }();
+  if (registers != 128)
+    return cudaErrorLaunchOutOfResources;
   return launch_pdl(kernel, dim3(a.splits, static_cast<unsigned>(tiles * a.v.heads), a.v.batch),
                     dim3(kThreads), bytes, stream, a, tiles);
 }
