@@ -6,17 +6,17 @@
 // operands fill shared memory's 128 bytes a cycle, and 1,024 of the
 // special-function units. A CTA therefore runs two streams of 128 query rows,
 // so that one's products cover the other's softmax:
-//   warps 0-3, 4-7  softmax of stream 0 and 1: a thread a row, its 128 scores
-//                   from TMEM into registers (which these warps take over from
-//                   the others), probabilities back over them as the f16 A
-//                   operand
+//   warps 0-3, 4-7  softmax of stream 0 and 1: a thread a row, scores from
+//                   TMEM, probabilities back over them as the f16 A operand
 //   warps 8-11      converters: 64 tokens of keys, then of values, at a time,
 //                   int8 codes (16 bytes a load, exact in f16) into
 //                   128-byte-swizzled tiles of 128 tokens, two each
 //   warp 12         issues the products: S = Q K^T, then O += P V
 //   warp 13         looks up the pages and scales of the tokens to come
 // (Two buffers of 64 keys a stream, which let products run ahead, were slower:
-// a product of 64 keys still reads all of its query tile.)
+// a product of 64 keys still reads all of its query tile. So were all 128
+// scores of a row in registers, with or without more registers for these
+// warps.)
 // Query rows are the tokens of a sequence times the heads that share a kv
 // head, so a tile of keys is converted once for up to 256 rows. The codes'
 // scales stay out of the products: a group of 16 tokens lies in one page, and
@@ -234,6 +234,26 @@ __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&r)[8])
                : "memory");
 }
 
+// 2^x of a pair on the FMA units, which are idle while the special-function
+// units work at their limit: n = rint(x) by adding 1.5 * 2^23, a polynomial in
+// f = x - n of [-0.5, 0.5] (least largest relative error, fitted by reweighted
+// least squares: 2.7e-6), n added to the exponent bits. Below 2^-120 it stays
+// there.
+__device__ __forceinline__ float2 exp2_pair(float2 x) {
+  x.x = fmaxf(x.x, -120.0f);
+  x.y = fmaxf(x.y, -120.0f);
+  const float2 magic = make_float2(12582912.0f, 12582912.0f);
+  const float2 r = add2(x, magic);
+  const float2 n = add2(r, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+  float2 p = fma2(f, make_float2(9.5701022e-3f, 9.5701022e-3f), make_float2(5.5917863e-2f, 5.5917863e-2f));
+  p = fma2(p, f, make_float2(0.24024744f, 0.24024744f));
+  p = fma2(p, f, make_float2(0.69312179f, 0.69312179f));
+  p = fma2(p, f, make_float2(0.99999928f, 0.99999928f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
+}
+
 __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, "
                "%9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
@@ -249,28 +269,28 @@ __device__ __forceinline__ void tmem_stored() {
 
 // kCount neighbouring elements of a query row as f32, zero from `dim` on.
 template <typename T, int kCount>
-__device__ __forceinline__ void load_few(const T *row, int d, int dim, float (&x)[kCount]) {
+__device__ __forceinline__ void load_few(const T *row, int d, int dim, bool aligned,
+                                         float (&x)[kCount]) {
   constexpr int kBytes = kCount * static_cast<int>(sizeof(T));
   union {
     uint32_t raw[kBytes / 4];
     T at[kCount];
   } p;
-  const T *at = row + d;
-  if (d >= dim) { // head_dim is a multiple of 16: all or nothing
 #pragma unroll
-    for (int i = 0; i < kBytes / 4; ++i)
-      p.raw[i] = 0;
-  } else if ((reinterpret_cast<uintptr_t>(at) & (kBytes - 1)) == 0) {
-    if constexpr (kBytes == 16)
-      *reinterpret_cast<uint4 *>(p.raw) = *reinterpret_cast<const uint4 *>(at);
-    else if constexpr (kBytes == 8)
-      *reinterpret_cast<uint2 *>(p.raw) = *reinterpret_cast<const uint2 *>(at);
-    else
-      p.raw[0] = *reinterpret_cast<const uint32_t *>(at);
-  } else {
+  for (int i = 0; i < kBytes / 4; ++i)
+    p.raw[i] = 0;
+  if (d < dim) { // head_dim is a multiple of 16: all or nothing
+    if (!aligned) {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i)
-      p.at[i] = at[i];
+      for (int i = 0; i < kCount; ++i)
+        p.at[i] = row[d + i];
+    } else if constexpr (kBytes == 16) {
+      *reinterpret_cast<uint4 *>(p.raw) = __ldg(reinterpret_cast<const uint4 *>(row + d));
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2 *>(p.raw) = __ldg(reinterpret_cast<const uint2 *>(row + d));
+    } else {
+      p.raw[0] = __ldg(reinterpret_cast<const uint32_t *>(row + d));
+    }
   }
 #pragma unroll
   for (int i = 0; i < kCount; ++i)
@@ -354,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       const int i = f / a.group;
       load_few<T, kE>(static_cast<const T *>(a.q) + (s.row0 + i) * a.q_row_stride +
                           (head * a.group + f - i * a.group) * a.q_head_stride,
-                      d, v.dim, x);
+                      d, v.dim, a.q_aligned, x);
     }
     float amax = 0.0f;
 #pragma unroll
@@ -398,10 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0); // columns: scores [stream][128], outputs [stream][kD]
   int *failed = &sm.failed;
 
-  // Registers: 128 a thread at launch, 256 x 168 + 256 x 88 from here on
-  // (the launch checks that it has them).
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ------------------------------------------------------------- softmax
     const int st = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -412,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     const int row_hi = !live ? 0 : a.causal ? min(s.length, pos + 1) : s.length;
     const int row_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     const float coef = sm.coef[kShare ? row : st * kM + row];
-    float m = -INFINITY, l = 0.0f;
+    float m = kNone, l = 0.0f;
     const int mine = kShare ? (count - st + 1) / 2 : count;
     bool ok = true;
 #pragma unroll 1
@@ -434,66 +451,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t scale_at = smem_at(sm.scale[part0]); // of the tile's eight groups
-      // The largest exponent of the row, t = score * log2(e) + log2(scale of v).
-      float top = -INFINITY;
-      // One part: the scores stay in registers. Two: there is no room beside
-      // both parts, they are read again.
-      constexpr bool kHold = kParts == 1;
-      uint32_t x[kHold ? 4 : 1][32];
       auto hide = [&](int c, uint32_t (&y)[32]) {
         const uint32_t seen = visible(c);
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          y[i] = seen >> i & 1 ? y[i] : 0xff800000u; // -infinity: hidden
+          y[i] = seen >> i & 1 ? y[i] : 0xff800000u; // -infinity
       };
-      if constexpr (kHold) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_load_start(s_at + 32 * c, x[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_loaded(x[c]);
-        if (!whole) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            hide(c, x[c]);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if constexpr (!kHold) {
-          tmem_load(s_at + 32 * c, x[0]);
-          if (!whole)
-            hide(c, x[0]);
-        }
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const uint32_t *y = x[kHold ? c : 0] + 16 * g;
-          float best = __uint_as_float(y[0]);
-#pragma unroll
-          for (int i = 1; i < 15; i += 2)
-            best = max3(best, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
-          best = fmaxf(best, __uint_as_float(y[15]));
-          const float4 sc = load_scale(scale_at + (2 * c + g) * 16);
-          if (whole || best != -INFINITY)
-            top = nan_max(top, fmaf(best, coef * sc.x, sc.y));
-        }
-      }
-      // Set the row's reference again when its probabilities outgrow f16.
-      const bool set = top != -INFINITY &&
-                       (m == -INFINITY || !(top - m <= kGrowth<kParts>));
-      if (__any_sync(0xffffffffu, set)) {
-        const float m_new = set ? top - kTop<kParts> : m;
-        const float shrink = set ? exp2_approx(m - m_new) : 1.0f; // 0 for the first
-        m = m_new;
+      // Score to exponent: a positive slope (of nearly nothing where the row or
+      // the scale is zero) leaves what is hidden at -infinity.
+      auto slope_of = [&](float key_scale) {
+        const float slope = coef * key_scale;
+        return slope < 1e-37f ? 1e-37f : slope;
+      };
+      // A new reference for the rows that outgrew theirs (the first is kNone).
+      auto refer = [&](bool grown, float to) {
+        const float shrink = grown ? exp2_approx(m - to) : 1.0f; // 0 for the first
+        m = grown ? to : m;
         l *= shrink;
         if (n > 0) {
           ok = __all_sync(0xffffffffu, bar_wait(&sm.o_full[st], (n - 1) & 1, failed));
-          if (!ok)
-            break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-          for (int c = 0; c < 8 * kCh; ++c) { // few columns at a time: the scores are held
+          for (int c = 0; ok && c < 8 * kCh; ++c) { // few columns at a time: the scores are held
             uint32_t y[8];
             tmem_load8(o_at + 8 * c, y);
 #pragma unroll
@@ -502,46 +481,81 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
             tmem_store8(o_at + 8 * c, y);
           }
         }
-      }
-      const float origin = m == -INFINITY ? 0.0f : m;
-      // Probabilities over the scores just read: of every 32 columns 16 hold
-      // their f16, the next 16 the small parts.
+      };
+      // The scores are read once for the largest exponent and once more for the
+      // probabilities, 32 at a time with the next 32 on their way: held whole
+      // they cost more register moves than the second reading.
+      uint32_t x[2][32];
+      float top = -INFINITY;
+      tmem_load_start(s_at, x[0]);
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if constexpr (!kHold) {
-          tmem_load(s_at + 32 * c, x[0]);
+        for (int h = 0; h < 2; ++h) {
+          tmem_loaded(x[h]);
+          if (h == 0 || c == 0)
+            tmem_load_start(s_at + 32 * (c + h + 1), x[h ^ 1]);
           if (!whole)
-            hide(c, x[0]);
-        }
-        const uint32_t *y = x[kHold ? c : 0];
-        uint32_t high[16], low[16];
+            hide(c + h, x[h]);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float4 sc = load_scale(scale_at + (2 * c + g) * 16);
-          const float slope = coef * sc.x, shift = sc.y - origin;
-          float2 sum = make_float2(0.0f, 0.0f);
+          for (int g = 0; g < 2; ++g) {
+            const uint32_t *y = x[h] + 16 * g;
+            float best = max3(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]));
+            float next = max3(__uint_as_float(y[3]), __uint_as_float(y[4]), __uint_as_float(y[5]));
 #pragma unroll
-          for (int i = 16 * g; i < 16 * g + 16; i += 2) {
-            float2 e = fma2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])),
-                            make_float2(slope, slope), make_float2(shift, shift));
-            if (!whole) { // a slope of zero has made NaN of what is hidden
-              e.x = y[i] == 0xff800000u ? -INFINITY : e.x;
-              e.y = y[i + 1] == 0xff800000u ? -INFINITY : e.y;
+            for (int i = 6; i < 14; i += 4) {
+              best = max3(best, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+              next = max3(next, __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
             }
-            const float2 p = make_float2(exp2_approx(e.x), exp2_approx(e.y));
-            sum = add2(sum, p);
-            high[i / 2] = pack_half(p.x, p.y);
-            if constexpr (kParts == 2) {
-              const float2 back = unpack_half(high[i / 2]);
-              low[i / 2] = pack_half(p.x - back.x, p.y - back.y);
-            }
+            best = max3(best, __uint_as_float(y[14]), __uint_as_float(y[15]));
+            const float4 sc = load_scale(scale_at + (2 * (c + h) + g) * 16);
+            top = fmaxf(top, fmaf(fmaxf(best, next), slope_of(sc.x), sc.y));
           }
-          l = fmaf(sum.x + sum.y, sc.z, l);
         }
-        tmem_store16(s_at + 32 * c, high);
-        if constexpr (kParts == 2)
-          tmem_store16(s_at + 32 * c + 16, low);
       }
+      tmem_load_start(s_at, x[0]);
+      const bool grown = top > (m == kNone ? -INFINITY : m + kGrowth<kParts>);
+      if (__any_sync(0xffffffffu, grown))
+        refer(grown, top - kTop<kParts>);
+      const float origin = m == kNone ? 0.0f : m;
+      // Probabilities over the scores: of every 32 columns 16 hold their f16,
+      // the next 16 the small parts.
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tmem_loaded(x[h]);
+          if (h == 0 || c == 0)
+            tmem_load_start(s_at + 32 * (c + h + 1), x[h ^ 1]);
+          if (!whole)
+            hide(c + h, x[h]);
+          uint32_t high[16], low[16];
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float4 sc = load_scale(scale_at + (2 * (c + h) + g) * 16);
+            const float slope = slope_of(sc.x), shift = sc.y - origin;
+            float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 16 * g; i < 16 * g + 16; i += 2) {
+              const float2 e = fma2(make_float2(__uint_as_float(x[h][i]), __uint_as_float(x[h][i + 1])),
+                                    make_float2(slope, slope), make_float2(shift, shift));
+              const float2 q = kParts == 1 && i % 8 == 6 ? exp2_pair(e) : make_float2(exp2_approx(e.x), exp2_approx(e.y));
+              sum = add2(sum, q);
+              high[i / 2] = pack_half(q.x, q.y);
+              if constexpr (kParts == 2) {
+                const float2 back = unpack_half(high[i / 2]);
+                low[i / 2] = pack_half(q.x - back.x, q.y - back.y);
+              }
+            }
+            l = fmaf(sum.x + sum.y, sc.z, l);
+          }
+          tmem_store16(s_at + 32 * (c + h), high);
+          if constexpr (kParts == 2)
+            tmem_store16(s_at + 32 * (c + h) + 16, low);
+        }
+      }
+      if (!ok)
+        break;
       tmem_stored();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       bar_arrive(&sm.p_full[st]);
@@ -558,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       // Every product has completed (both streams have waited for theirs).
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (st == 1) {
-        sm.join[0][row] = mine > 0 ? m : -INFINITY;
+        sm.join[0][row] = mine > 0 ? m : kNone;
         sm.join[1][row] = l;
         if (mine > 0) {
 #pragma unroll 1
@@ -574,14 +588,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (st == 0) {
         const float m1 = sm.join[0][row];
-        const float most = nan_max(m, m1);
-        share = m == -INFINITY ? 0.0f : exp2_approx(m - most);
-        other = m1 == -INFINITY ? 0.0f : exp2_approx(m1 - most);
-        l = l * share + (m1 == -INFINITY ? 0.0f : sm.join[1][row] * other);
+        const float most = fmaxf(m, m1);
+        share = m == kNone ? 0.0f : exp2_approx(m - most);
+        other = m1 == kNone ? 0.0f : exp2_approx(m1 - most);
+        l = l * share + sm.join[1][row] * other; // NaN stays
         m = most;
       }
     }
-    const bool some = m != -INFINITY;
+    const bool some = m != kNone || l != l; // l of a row that sees with NaN is NaN
     if (!kShare || st == 0) {
       const bool apart = a.splits > 1;
       const float scale = !some ? 0.0f : apart ? 1.0f : 1.0f / l;
@@ -626,13 +640,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       }
       if (live && ok) {
         if (apart)
-          a.part_ml[slot] = make_float2(some ? m : kNone, l);
+          a.part_ml[slot] = make_float2(m, l);
         else if (a.lse)
           a.lse[at] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
       }
     }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ---------------------------------------------------------- converters
     // A thread loads 16 codes of a token a step; eight neighbouring lanes hold two tokens of one panel, so that
     // their 16-byte stores fall in different banks.
@@ -709,7 +722,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       ok = __all_sync(0xffffffffu, ok);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 12) {
       // ----------------------------------------------------------- products
       constexpr uint32_t kS = idesc_f16(kM, kTile, false), kO = idesc_f16(kM, kD, true);
@@ -855,14 +867,6 @@ cudaError_t launch_prompt(const KvAttendArgs &a, int tiles, cudaStream_t stream)
   static DynamicSmem allowed;
   if (const cudaError_t e = allowed.allow(kernel, bytes); e != cudaSuccess)
     return e;
-  // The softmax warps wait for registers that the others give up: there have to
-  // be as many as the kernel hands around.
-  static const int registers = [&] {
-    cudaFuncAttributes attr{};
-    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
-  }();
-  if (registers != 128)
-    return cudaErrorLaunchOutOfResources;
   return launch_pdl(kernel, dim3(a.splits, static_cast<unsigned>(tiles * a.v.heads), a.v.batch),
                     dim3(kThreads), bytes, stream, a, tiles);
 }
