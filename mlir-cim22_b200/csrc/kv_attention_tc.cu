@@ -6,13 +6,15 @@
 // operands fill shared memory's 128 bytes a cycle, and 1,024 of the
 // special-function units. A CTA therefore runs two streams of 128 query rows,
 // so that one's products cover the other's softmax:
-//   warps 0-3, 4-7  softmax of stream 0 and 1: a thread a row, scores from
-//                   TMEM, probabilities back over them as the f16 A operand
-//   warps 8-11      converters: 64 tokens of keys, then of values, at a time,
+//   warps 0-7, 8-15 softmax of stream 0 and 1: two threads a row, one for each
+//                   64 keys of a tile, scores from TMEM, probabilities back over
+//                   them as the f16 A operand (one thread a row left too few
+//                   warps to keep the special-function units busy)
+//   warps 16-19     converters: 64 tokens of keys, then of values, at a time,
 //                   int8 codes (16 bytes a load, exact in f16) into
 //                   128-byte-swizzled tiles of 128 tokens, two each
-//   warp 12         issues the products: S = Q K^T, then O += P V
-//   warp 13         looks up the pages and scales of the tokens to come
+//   warp 20         issues the products: S = Q K^T, then O += P V
+//   warp 21         looks up the pages and scales of the tokens to come
 // (Two buffers of 64 keys a stream, which let products run ahead, were slower:
 // a product of 64 keys still reads all of its query tile. So were all 128
 // scores of a row in registers, with or without more registers for these
@@ -32,7 +34,7 @@
 namespace cim {
 namespace {
 
-constexpr int kThreads = 512, kM = 128, kTile = 128; // query rows a stream, keys a tile
+constexpr int kThreads = 768, kM = 128, kTile = 128; // query rows a stream, keys a tile
 constexpr int kSub = 64, kIndex = 8; // tokens converted at a time, and indexed ahead
 constexpr int kPanel = 128 * 128;    // bytes: 128 rows of 64 f16
 constexpr uint64_t kWaitLimit = 2000000000ull; // ns
@@ -44,7 +46,8 @@ template <int kCh> struct alignas(1024) PromptSmem {
   // value scale, and where the keys begin in units of a group's keys (-1: none).
   float4 scale[kIndex][kSub / 16];
   float coef[2 * kM];            // what turns a row's product into an exponent
-  float join[2][kM];
+  float join[2][kM], sums[2][2][kM];
+  float tops[2][2][2][kM];       // [tile % 2][stream][half]
   uint64_t kv_full[2][4], kv_empty[2][2]; // of parts and of tiles
   uint64_t index_full[kIndex], index_empty[kIndex];
   uint64_t s_full[2], p_full[2], o_full[2], done;
@@ -157,29 +160,22 @@ __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[32]) {
                : "memory");
 }
 
-// The same without waiting: tmem_loaded() orders the registers' use.
-__device__ __forceinline__ void tmem_load_start(uint32_t at, uint32_t (&r)[32]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, "
-               "%9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
-               "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+// 16 columns without waiting: tmem_loaded() orders the registers' use.
+__device__ __forceinline__ void tmem_load_start(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, "
+               "%9, %10, %11, %12, %13, %14, %15}, [%16];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
                  "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-                 "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-                 "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
-                 "=r"(r[30]), "=r"(r[31])
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(at)
                : "memory");
 }
 
-__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
                  "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
-                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                 "+r"(r[30]), "+r"(r[31])
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
 }
@@ -254,15 +250,6 @@ __device__ __forceinline__ float2 exp2_pair(float2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
 }
 
-__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, "
-               "%9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-               "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-               "r"(r[14]), "r"(r[15])
-               : "memory");
-}
-
 __device__ __forceinline__ void tmem_stored() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -321,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(&sm.s_full[i], 1);
-      bar_init(&sm.p_full[i], 128);
+      bar_init(&sm.p_full[i], 256);
       bar_init(&sm.o_full[i], 1);
     }
     bar_init(&sm.done, 1);
@@ -343,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   const int rows = s.n * a.group;
   if (f0 >= rows)
     return;
-  if (warp == 12) {
+  if (warp == 20) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
                      smem_at(&sm.tmem))
                  : "memory");
@@ -418,9 +405,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0); // columns: scores [stream][128], outputs [stream][kD]
   int *failed = &sm.failed;
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ------------------------------------------------------------- softmax
-    const int st = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int st = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + st * kTile + lanes, o_at = tmem + 2 * kTile + st * kD + lanes;
     const int f = f0 + (kShare ? 0 : st * kM) + row;
@@ -437,25 +424,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       const int tile = kShare ? 2 * n + st : n;
       const int key0 = key_base + tile * kTile;
       const int from = min(max(row_lo - key0, 0), kTile), to = min(max(row_hi - key0, 0), kTile);
-      const bool whole = __all_sync(0xffffffffu, from == 0 && to == kTile);
-      auto visible = [&](int c) -> uint32_t { // of scores 32 c .. 32 c + 31
-        const int x = min(max(from - 32 * c, 0), 32), y = min(max(to - 32 * c, 0), 32);
-        return y > x ? (0xffffffffu >> (32 - (y - x))) << x : 0u;
-      };
-      const int part0 = (2 * tile) % kIndex;
-      ok = bar_wait(&sm.index_full[part0], (2 * tile / kIndex) & 1, failed) &&
-           bar_wait(&sm.index_full[part0 + 1], (2 * tile / kIndex) & 1, failed) &&
-           bar_wait(&sm.s_full[st], n & 1, failed);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok)
-        break;
+      const bool whole =
+          __all_sync(0xffffffffu, from <= kSub * half && to >= kSub * (half + 1));
+      const int part0 = (2 * tile + half) % kIndex;
+      // After a wait that ran out the loop goes on (later ones then return at
+      // once): the other half's warp meets this one at a barrier in each round.
+      ok = bar_wait(&sm.index_full[part0], ((2 * tile + half) / kIndex) & 1, failed) && ok;
+      ok = bar_wait(&sm.s_full[st], n & 1, failed) && ok;
+      __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t scale_at = smem_at(sm.scale[part0]); // of the tile's eight groups
-      auto hide = [&](int c, uint32_t (&y)[32]) {
-        const uint32_t seen = visible(c);
+      const uint32_t scale_at = smem_at(sm.scale[part0]); // of the half's four groups
+      auto hide = [&](int g, uint32_t (&y)[16]) {
+        const int key = kSub * half + 16 * g;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          y[i] = seen >> i & 1 ? y[i] : 0xff800000u; // -infinity
+        for (int i = 0; i < 16; ++i)
+          y[i] = key + i >= from && key + i < to ? y[i] : 0xff800000u; // -infinity
       };
       // Score to exponent: a positive slope (of nearly nothing where the row or
       // the scale is zero) leaves what is hidden at -infinity.
@@ -469,10 +452,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         m = grown ? to : m;
         l *= shrink;
         if (n > 0) {
-          ok = __all_sync(0xffffffffu, bar_wait(&sm.o_full[st], (n - 1) & 1, failed));
+          ok = bar_wait(&sm.o_full[st], (n - 1) & 1, failed) && ok;
+          __syncwarp();
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-          for (int c = 0; ok && c < 8 * kCh; ++c) { // few columns at a time: the scores are held
+          for (int c = half * 4 * kCh; c < (half + 1) * 4 * kCh; ++c) { // its half of O
             uint32_t y[8];
             tmem_load8(o_at + 8 * c, y);
 #pragma unroll
@@ -483,100 +467,104 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         }
       };
       // The scores are read once for the largest exponent and once more for the
-      // probabilities, 32 at a time with the next 32 on their way: held whole
-      // they cost more register moves than the second reading.
-      uint32_t x[2][32];
+      // probabilities, 16 (a group of one scale) at a time with the next 16 on
+      // their way.
+      const uint32_t from_at = s_at + kSub * half;
+      uint32_t x[2][16];
       float top = -INFINITY;
-      tmem_load_start(s_at, x[0]);
-#pragma unroll 1
-      for (int c = 0; c < 4; c += 2) {
+      tmem_load_start(from_at, x[0]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          tmem_loaded(x[h]);
-          if (h == 0 || c == 0)
-            tmem_load_start(s_at + 32 * (c + h + 1), x[h ^ 1]);
-          if (!whole)
-            hide(c + h, x[h]);
+      for (int g = 0; g < 4; ++g) {
+        uint32_t(&y)[16] = x[g & 1];
+        tmem_loaded(y);
+        tmem_load_start(from_at + 16 * ((g + 1) & 3), x[(g & 1) ^ 1]); // at last group 0 again
+        if (!whole)
+          hide(g, y);
+        float best = max3(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]));
+        float next = max3(__uint_as_float(y[3]), __uint_as_float(y[4]), __uint_as_float(y[5]));
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const uint32_t *y = x[h] + 16 * g;
-            float best = max3(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]));
-            float next = max3(__uint_as_float(y[3]), __uint_as_float(y[4]), __uint_as_float(y[5]));
-#pragma unroll
-            for (int i = 6; i < 14; i += 4) {
-              best = max3(best, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
-              next = max3(next, __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
-            }
-            best = max3(best, __uint_as_float(y[14]), __uint_as_float(y[15]));
-            const float4 sc = load_scale(scale_at + (2 * (c + h) + g) * 16);
-            top = fmaxf(top, fmaf(fmaxf(best, next), slope_of(sc.x), sc.y));
-          }
+        for (int i = 6; i < 14; i += 4) {
+          best = max3(best, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+          next = max3(next, __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
         }
+        best = max3(best, __uint_as_float(y[14]), __uint_as_float(y[15]));
+        const float4 sc = load_scale(scale_at + g * 16);
+        top = fmaxf(top, fmaf(fmaxf(best, next), slope_of(sc.x), sc.y));
       }
-      tmem_load_start(s_at, x[0]);
+      // Both halves of a row have one reference.
+      sm.tops[n & 1][st][half][row] = top;
+      asm volatile("bar.sync %0, 64;" ::"r"(2 + st * 4 + (warp & 3)) : "memory");
+      top = fmaxf(top, sm.tops[n & 1][st][half ^ 1][row]);
       const bool grown = top > (m == kNone ? -INFINITY : m + kGrowth<kParts>);
       if (__any_sync(0xffffffffu, grown))
         refer(grown, top - kTop<kParts>);
       const float origin = m == kNone ? 0.0f : m;
       // Probabilities over the scores: of every 32 columns 16 hold their f16,
       // the next 16 the small parts.
-#pragma unroll 1
-      for (int c = 0; c < 4; c += 2) {
+      uint32_t low[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          tmem_loaded(x[h]);
-          if (h == 0 || c == 0)
-            tmem_load_start(s_at + 32 * (c + h + 1), x[h ^ 1]);
-          if (!whole)
-            hide(c + h, x[h]);
-          uint32_t high[16], low[16];
+      for (int g = 0; g < 4; ++g) {
+        uint32_t(&y)[16] = x[g & 1];
+        tmem_loaded(y);
+        // The small parts of an even group go over the next group's scores,
+        // which have been read by now.
+        if (kParts == 2 && (g & 1))
+          tmem_store8(from_at + (g >> 1) * 32 + 16, low);
+        if (g < 3)
+          tmem_load_start(from_at + 16 * (g + 1), x[(g & 1) ^ 1]);
+        if (!whole)
+          hide(g, y);
+        const float4 sc = load_scale(scale_at + g * 16);
+        const float slope = slope_of(sc.x), shift = sc.y - origin;
+        uint32_t high[8];
+        float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 sc = load_scale(scale_at + (2 * (c + h) + g) * 16);
-            const float slope = slope_of(sc.x), shift = sc.y - origin;
-            float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int i = 16 * g; i < 16 * g + 16; i += 2) {
-              const float2 e = fma2(make_float2(__uint_as_float(x[h][i]), __uint_as_float(x[h][i + 1])),
-                                    make_float2(slope, slope), make_float2(shift, shift));
-              const float2 q = kParts == 1 && i % 8 == 6 ? exp2_pair(e) : make_float2(exp2_approx(e.x), exp2_approx(e.y));
-              sum = add2(sum, q);
-              high[i / 2] = pack_half(q.x, q.y);
-              if constexpr (kParts == 2) {
-                const float2 back = unpack_half(high[i / 2]);
-                low[i / 2] = pack_half(q.x - back.x, q.y - back.y);
-              }
-            }
-            l = fmaf(sum.x + sum.y, sc.z, l);
+        for (int i = 0; i < 16; i += 2) {
+          const float2 e = fma2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])),
+                                make_float2(slope, slope), make_float2(shift, shift));
+          const float2 q = kParts == 1 && i % 8 == 6
+                               ? exp2_pair(e)
+                               : make_float2(exp2_approx(e.x), exp2_approx(e.y));
+          sum = add2(sum, q);
+          high[i / 2] = pack_half(q.x, q.y);
+          if constexpr (kParts == 2) {
+            const float2 back = unpack_half(high[i / 2]);
+            low[i / 2] = pack_half(q.x - back.x, q.y - back.y);
           }
-          tmem_store16(s_at + 32 * (c + h), high);
-          if constexpr (kParts == 2)
-            tmem_store16(s_at + 32 * (c + h) + 16, low);
         }
+        l = fmaf(sum.x + sum.y, sc.z, l);
+        const uint32_t at = from_at + (g >> 1) * 32 + (g & 1) * 8;
+        tmem_store8(at, high);
+        if (kParts == 2 && (g & 1))
+          tmem_store8(at + 16, low);
       }
-      if (!ok)
-        break;
       tmem_stored();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       bar_arrive(&sm.p_full[st]);
-      if (lane < 2) // the warp is done with the tile's scales
-        bar_arrive(&sm.index_empty[part0 + lane]);
+      if (lane == 0) // the warp is done with its part's scales
+        bar_arrive(&sm.index_empty[part0]);
     }
-    if (ok && mine > 0)
-      ok = bar_wait(&sm.o_full[st], (mine - 1) & 1, failed);
+    if (mine > 0)
+      ok = bar_wait(&sm.o_full[st], (mine - 1) & 1, failed) && ok;
     ok = __all_sync(0xffffffffu, ok);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // Each thread finishes its half of the row's elements with the whole row's sum.
     float share = 1.0f, other = 0.0f;
     float *joined = reinterpret_cast<float *>(sm.kv); // [element][row]
+    sm.sums[st][half][row] = l;
+    asm volatile("bar.sync %0, 64;" ::"r"(2 + st * 4 + (warp & 3)) : "memory");
+    l = sm.sums[st][0][row] + sm.sums[st][1][row];
     if constexpr (kShare) {
       // Every product has completed (both streams have waited for theirs).
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, 512;" ::: "memory");
       if (st == 1) {
-        sm.join[0][row] = mine > 0 ? m : kNone;
-        sm.join[1][row] = l;
+        if (half == 0) {
+          sm.join[0][row] = mine > 0 ? m : kNone;
+          sm.join[1][row] = l;
+        }
         if (mine > 0) {
 #pragma unroll 1
-          for (int c = 0; c < 2 * kCh; ++c) {
+          for (int c = half * kCh; c < (half + 1) * kCh; ++c) {
             uint32_t x[32];
             tmem_load(o_at + 32 * c, x);
 #pragma unroll
@@ -585,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
           }
         }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, 512;" ::: "memory");
       if (st == 0) {
         const float m1 = sm.join[0][row];
         const float most = fmaxf(m, m1);
@@ -603,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       const int64_t at = (s.row0 + i) * a.q_heads + head * a.group + (live ? f - i * a.group : 0);
       const int64_t slot = static_cast<int64_t>(split) * v.rows * a.q_heads + at;
 #pragma unroll 1
-      for (int c = 0; c < 2 * kCh; ++c) {
+      for (int c = half * kCh; c < (half + 1) * kCh; ++c) {
         uint32_t x[32];
         tmem_load(o_at + 32 * c, x);
         float y[32];
@@ -638,20 +626,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
           }
         }
       }
-      if (live && ok) {
+      if (live && ok && half == 0) {
         if (apart)
           a.part_ml[slot] = make_float2(m, l);
         else if (a.lse)
           a.lse[at] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ---------------------------------------------------------- converters
     // A thread loads 16 codes of a token a step; eight neighbouring lanes hold two tokens of one panel, so that
     // their 16-byte stores fall in different banks.
     constexpr int kSteps = 2 * kCh;         // steps a part of 64 tokens
     constexpr int kTokens = kSub / kSteps;  // tokens a step
-    const int t = threadIdx.x - 256, quarter = t >> 3, r = t & 7;
+    const int t = threadIdx.x - 512, quarter = t >> 3, r = t & 7;
     const int token = kCh == 2 ? (quarter >> 1) * 2 + (r >> 2) : quarter * 2 + (r >> 2);
     const int part = kCh == 2 ? (quarter & 1) * 4 + (r & 3) : (r & 3);
     const bool inside = part * 16 < v.dim;
@@ -722,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       ok = __all_sync(0xffffffffu, ok);
     }
   } else {
-    if (warp == 12) {
+    if (warp == 20) {
       // ----------------------------------------------------------- products
       constexpr uint32_t kS = idesc_f16(kM, kTile, false), kO = idesc_f16(kM, kD, true);
       constexpr uint32_t kSlot = kCh * kPanel / 16;
@@ -802,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       __syncwarp();
       int unused = 0;
       bar_wait(&sm.done, 0, &unused);
-    } else if (warp == 13) {
+    } else if (warp == 21) {
       // --------------------------------------------------------- pages, scales
       // Lane i takes a part's i-th group of 16 tokens; table entries are loaded
       // two parts ahead and scales one, so that neither is waited for here.
@@ -854,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   __syncthreads();
   if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(failed))
     atomicOr(a.status, CIM22_STATUS_TIMEOUT);
-  if (warp == 12) {
+  if (warp == 20) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
