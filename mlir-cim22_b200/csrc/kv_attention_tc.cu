@@ -68,30 +68,37 @@ __device__ __forceinline__ void bar_arrive(uint64_t *bar) {
 }
 
 // Waits for the phase of the given parity, for at most kWaitLimit of the
-// global timer; gives up sooner when another role has.
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *failed) {
-  const uint32_t at = smem_at(bar);
+// global timer; gives up sooner when another role has. The first try is all
+// that most waits need; what follows is kept out of line and short, since the
+// waiting warps' polls compete with the working ones for issue slots.
+__device__ __forceinline__ bool bar_try(uint32_t at, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+               " selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(done)
+               : "r"(at), "r"(parity)
+               : "memory");
+  return done;
+}
+
+__device__ __noinline__ bool bar_wait_long(uint32_t at, uint32_t parity, int *failed) {
   uint64_t start = 0;
-  for (uint32_t i = 1;; ++i) {
-    uint32_t done;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-                 " selp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(done)
-                 : "r"(at), "r"(parity)
-                 : "memory");
-    if (done)
-      return true;
-    if ((i & 31) == 0) {
-      uint64_t now;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-      if (start == 0)
-        start = now;
-      if (now - start > kWaitLimit || *reinterpret_cast<volatile int *>(failed)) {
-        *reinterpret_cast<volatile int *>(failed) = 1;
-        return false;
-      }
+  while (!bar_try(at, parity)) {
+    uint64_t now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (start == 0)
+      start = now;
+    if (now - start > kWaitLimit || *reinterpret_cast<volatile int *>(failed)) {
+      *reinterpret_cast<volatile int *>(failed) = 1;
+      return false;
     }
   }
+  return true;
+}
+
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *failed) {
+  const uint32_t at = smem_at(bar);
+  return bar_try(at, parity) || bar_wait_long(at, parity, failed);
 }
 
 // Matrix descriptors, 128-byte swizzle. K-major (queries, keys): rows of 128
@@ -471,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       // their way.
       const uint32_t from_at = s_at + kSub * half;
       uint32_t x[2][16];
-      float top = -INFINITY;
+      float top = -INFINITY, slopes[4];
       tmem_load_start(from_at, x[0]);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -489,7 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         }
         best = max3(best, __uint_as_float(y[14]), __uint_as_float(y[15]));
         const float4 sc = load_scale(scale_at + g * 16);
-        top = fmaxf(top, fmaf(fmaxf(best, next), slope_of(sc.x), sc.y));
+        slopes[g] = slope_of(sc.x);
+        top = fmaxf(top, fmaf(fmaxf(best, next), slopes[g], sc.y));
       }
       // Both halves of a row have one reference.
       sm.tops[n & 1][st][half][row] = top;
@@ -515,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         if (!whole)
           hide(g, y);
         const float4 sc = load_scale(scale_at + g * 16);
-        const float slope = slope_of(sc.x), shift = sc.y - origin;
+        const float slope = slopes[g], shift = sc.y - origin;
         uint32_t high[8];
         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
