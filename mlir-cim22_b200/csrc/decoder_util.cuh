@@ -42,6 +42,53 @@ template <typename T> union Pack {
   __device__ Pack() : raw(make_uint4(0, 0, 0, 0)) {}
 };
 
+// A vector as f32, and back (each element rounded to nearest even).
+__device__ __forceinline__ void unpack(const Pack<float> &p, float (&x)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[i] = p.at[i];
+}
+__device__ __forceinline__ void unpack(const Pack<__nv_bfloat16> &p, float (&x)[8]) {
+  const uint32_t w[4] = {p.raw.x, p.raw.y, p.raw.z, p.raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const Pack<__half> &p, float (&x)[8]) {
+  const uint32_t w[4] = {p.raw.x, p.raw.y, p.raw.z, p.raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void pack(const float (&x)[4], Pack<float> &p) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    p.at[i] = x[i];
+}
+__device__ __forceinline__ void pack(const float (&x)[8], Pack<__nv_bfloat16> &p) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+  p.raw = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void pack(const float (&x)[8], Pack<__half> &p) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+  p.raw = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Elements e .. e + kVec - 1 of a row of `count` elements (those outside it
 // read as zero): one 16-byte load where they lie on such a boundary.
 template <typename T>
