@@ -544,8 +544,8 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
         0 if gate is None else FLOAT_TYPES[gate.dtype], _GATE_ACT[gate_activation],
         None if post is None else _norm_arg(post, x, dim, "post"),
         None if pre is None else _norm_arg(pre, x, dim, "pre"),
-        None if h is None else h.data_ptr(), 0 if h is None else _as_rows(h, x, "out"),
-        None if y is None else y.data_ptr(), 0 if y is None else _as_rows(y, x, "normed"))
+        None if h is None else h.data_ptr(), dim if out is None else _as_rows(out, x, "out"),
+        None if y is None else y.data_ptr(), dim if normed is None else _as_rows(normed, x, "normed"))
     launch("block_norm", x.get_device(), lib().cim22_cuda_block_norm, ctypes.byref(call))
     return h, y
 

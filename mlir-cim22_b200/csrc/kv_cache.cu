@@ -24,6 +24,43 @@ __device__ __forceinline__ int quantise(float x, float inverse) {
   return x == x ? static_cast<int>(q) : 0;
 }
 
+// The largest magnitude's bits so far, with a vector's (an infinity or NaN is
+// above every finite value's), in the words that max_bits takes them from.
+__device__ __forceinline__ uint32_t max_bits(uint32_t top, const Pack<float> &p) {
+  top = max(max(top, p.raw.x & 0x7fffffffu), p.raw.y & 0x7fffffffu);
+  return max(max(top, p.raw.z & 0x7fffffffu), p.raw.w & 0x7fffffffu);
+}
+template <typename T> __device__ __forceinline__ uint32_t max_bits(uint32_t top, const Pack<T> &p) {
+  top = __vimax3_u16x2(top, p.raw.x & 0x7fff7fffu, p.raw.y & 0x7fff7fffu);
+  return __vimax3_u16x2(top, p.raw.z & 0x7fff7fffu, p.raw.w & 0x7fff7fffu);
+}
+template <typename T> __device__ __forceinline__ float magnitude(uint32_t top) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(top);
+  } else {
+    const uint16_t most = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+    return to_f32(*reinterpret_cast<const T *>(&most));
+  }
+}
+
+// Codes of four values that the scale covers: |x * inverse| is below 127.5, so
+// 1.5 * 2^23 more is rounded to an integer whose low byte is the code.
+__device__ __forceinline__ uint32_t quantise4(const float *x, float inverse) {
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inverse), 12582912.0f));
+  return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+}
+
+// Four codes as f32: code + 128 as the low byte of 2^23 + u.
+__device__ __forceinline__ void code_values(uint32_t codes, float *y) {
+  codes ^= 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    y[i] = __uint_as_float(__byte_perm(codes, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
+}
+
 template <typename T> struct Codes; // kVec<T> codes
 template <> struct Codes<float> {
   using type = uint32_t;
@@ -49,7 +86,10 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ float top[kThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.z, head = blockIdx.y >> 1, side = blockIdx.y & 1;
+  // Neighbouring CTAs take the heads and sides of one block: their rows are
+  // neighbours in memory.
+  const int b = blockIdx.y, planes = 2 * v.heads, touch = blockIdx.x / planes;
+  const int plane = blockIdx.x - touch * planes, head = plane >> 1, side = plane & 1;
   const KvSequence s = kv_sequence(v, b);
   if (!s.ok) {
     if (threadIdx.x == 0 && blockIdx.x == 0)
@@ -57,16 +97,10 @@ __global__ void __launch_bounds__(kThreads)
     return;
   }
   const int begin = max(0, s.length - s.n);
-  const int ordinal = (begin >> v.block_log2) + static_cast<int>(blockIdx.x);
+  const int ordinal = (begin >> v.block_log2) + touch;
   const int64_t base = static_cast<int64_t>(ordinal) << v.block_log2;
   if (begin >= s.length || base >= s.length)
     return;
-  const int page = kv_page(v, b, ordinal);
-  if (page < 0) {
-    if (threadIdx.x == 0)
-      atomicOr(status, CIM22_STATUS_CACHE_INDEX);
-    return;
-  }
   const int lo = static_cast<int>(max(static_cast<int64_t>(begin), base) - base);
   const int hi = static_cast<int>(min(static_cast<int64_t>(s.length) - base,
                                       static_cast<int64_t>(1) << v.block_log2));
@@ -87,27 +121,38 @@ __global__ void __launch_bounds__(kThreads)
       x[p] = load_pack(rows + (row + lo + i) * stride, (c - i * parts.d) * V, v.dim);
     }
   }
+  // The page is looked up while the values are on their way.
+  const int page = kv_page(v, b, ordinal);
+  if (page < 0) {
+    if (threadIdx.x == 0)
+      atomicOr(status, CIM22_STATUS_CACHE_INDEX);
+    return;
+  }
   float *scale_at = v.scales + (static_cast<int64_t>(page) * v.heads + head) * 2 + side;
   const float old = lo > 0 ? *scale_at : 0.0f;
-  float amax = 0.0f;
-  bool wild = false;
+  uint32_t bits = 0;
 #pragma unroll
-  for (int p = 0; p < kPer; ++p) {
+  for (int p = 0; p < kPer; ++p)
+    bits = max_bits(bits, x[p]);
+  float amax = magnitude<T>(bits);
+  // Also orders every thread's read of the old scale before the new store.
+  const bool wild = __syncthreads_or(!(amax < INFINITY));
+  if (wild) { // the largest of the finite ones
+    amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float m = fabsf(to_f32(x[p].at[i]));
-      const bool finite = m < INFINITY; // false for NaN
-      wild |= !finite;
-      amax = finite ? fmaxf(amax, m) : amax;
-    }
+    for (int p = 0; p < kPer; ++p)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float m = fabsf(to_f32(x[p].at[i]));
+        amax = m < INFINITY ? fmaxf(amax, m) : amax;
+      }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1)
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if ((threadIdx.x & 31) == 0)
     top[threadIdx.x >> 5] = amax;
-  // Also orders every thread's read of the old scale before the new store.
-  wild = __syncthreads_or(wild);
+  __syncthreads();
   for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w)
     amax = fmaxf(amax, top[w]);
   const float scale = fmaxf(old, __fmul_rn(fmaxf(amax, kKvFloor), kKvInv127));
@@ -125,10 +170,19 @@ __global__ void __launch_bounds__(kThreads)
       union {
         C raw;
         int8_t at[V];
+        uint32_t words[V / 4];
       } q;
+      float y[V];
+      unpack(x[p], y);
+      if (wild) {
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        q.at[i] = static_cast<int8_t>(quantise(to_f32(x[p].at[i]), inverse));
+        for (int i = 0; i < V; ++i)
+          q.at[i] = static_cast<int8_t>(quantise(y[i], inverse));
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4)
+          q.words[i / 4] = quantise4(y + i, inverse);
+      }
       *reinterpret_cast<C *>(codes + lo * v.dim + c * V) = q.raw;
     }
   }
@@ -156,7 +210,10 @@ __global__ void __launch_bounds__(kThreads)
   using C = typename Codes<T>::type;
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.z, head = blockIdx.y >> 1, side = blockIdx.y & 1;
+  // Neighbouring CTAs take the heads and sides of one block: their rows are
+  // neighbours in memory.
+  const int b = blockIdx.y, planes = 2 * v.heads, touch = blockIdx.x / planes;
+  const int plane = blockIdx.x - touch * planes, head = plane >> 1, side = plane & 1;
   T *out = side ? values : k;
   const KvSequence s = kv_sequence(v, b);
   if (!s.ok) {
@@ -165,7 +222,7 @@ __global__ void __launch_bounds__(kThreads)
     return;
   }
   const int begin = max(0, s.length - s.n);
-  const int ordinal = (begin >> v.block_log2) + static_cast<int>(blockIdx.x);
+  const int ordinal = (begin >> v.block_log2) + touch;
   const int64_t base = static_cast<int64_t>(ordinal) << v.block_log2;
   if (!out || begin >= s.length || base >= s.length)
     return;
@@ -186,7 +243,7 @@ __global__ void __launch_bounds__(kThreads)
   for (int c0 = threadIdx.x; c0 < chunks; c0 += kUnroll * kThreads) {
     union {
       C raw;
-      int8_t at[V];
+      uint32_t words[V / 4];
     } q[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
@@ -197,10 +254,15 @@ __global__ void __launch_bounds__(kThreads)
       const int c = c0 + u * kThreads;
       if (c < chunks) {
         const int i = fdiv(c, parts);
-        Pack<T> o;
+        float y[V];
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+          code_values(q[u].words[j / 4], y + j);
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          o.at[j] = from_f32<T>(__fmul_rn(static_cast<float>(q[u].at[j]), scale));
+          y[j] = __fmul_rn(y[j], scale);
+        Pack<T> o;
+        pack(y, o);
         store_pack(out + ((row + lo + i) * v.heads + head) * v.dim, (c - i * parts.d) * V, v.dim, o);
       }
     }
@@ -208,10 +270,10 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Blocks that n consecutive tokens can touch.
-int touched(const KvView &v) {
+unsigned touched(const KvView &v) {
   const int block = 1 << v.block_log2;
   const int64_t most = std::min<int64_t>(v.most, static_cast<int64_t>(v.table_width) * block);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((most + 2 * block - 2) / block, v.table_width)));
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 2 * block - 2) / block, v.table_width)));
 }
 
 template <typename T>
@@ -226,14 +288,14 @@ cudaError_t launch_write(const KvView &v, const Rows &keys, const Rows &values, 
                       : per <= 4 ? kv_write_kernel<T, 4>
                       : per <= 8 ? kv_write_kernel<T, 8>
                                  : kv_write_kernel<T, 128 * 128 / kVec<T> / kThreads>;
-  return launch_pdl(kernel, dim3(touched(v), v.heads * 2, v.batch), dim3(threads), 0, stream, v,
+  return launch_pdl(kernel, dim3(touched(v) * v.heads * 2, v.batch), dim3(threads), 0, stream, v,
                     keys, values, make_fastdiv(parts), status);
 }
 
 template <typename T>
 cudaError_t launch_read(const KvView &v, void *k, void *values, int32_t *status,
                         cudaStream_t stream) {
-  return launch_pdl(kv_read_kernel<T>, dim3(touched(v), v.heads * 2, v.batch), dim3(kThreads), 0,
+  return launch_pdl(kv_read_kernel<T>, dim3(touched(v) * v.heads * 2, v.batch), dim3(kThreads), 0,
                     stream, v, static_cast<T *>(k), static_cast<T *>(values),
                     make_fastdiv(v.dim / kVec<T>), status);
 }
