@@ -89,70 +89,88 @@ __device__ __forceinline__ float row_sum(float v, int warps_log2, float *buffer,
   return v;
 }
 
-template <typename T, int kPer, int kMax>
+// Narrow rows (several to a CTA) and, with kScalar, rows off vector boundaries.
+// There a warp's loads and stores take 32 neighbouring elements: lanes that
+// each took their own eight would spread every weight load over eight lines.
+template <typename T, int kPer, int kMax, bool kScalar>
 __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a) {
   constexpr int V = kVec<T>;
   __shared__ float buffer[64];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int w = 1 << a.warps_log2;
+  const int w = 1 << a.warps_log2, part = warp & (w - 1);
   const int64_t row_at = static_cast<int64_t>(blockIdx.x) * ((blockDim.x >> 5) >> a.warps_log2) +
                          (warp >> a.warps_log2);
   const bool live = row_at < a.rows;
   const int64_t row = live ? row_at : a.rows - 1; // every thread reaches the barriers
-  const int thread = ((warp & (w - 1)) << 5) | lane;
-  const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-  const T *residual = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
-  // Vectors are aligned to x's 16-byte boundaries: the first starts `phase`
-  // elements before the row.
-  const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const float inverse = 1.0f / static_cast<float>(a.dim);
+  const int dim = static_cast<int>(a.dim);
+  const float inverse = 1.0f / static_cast<float>(dim);
   int slot = 0;
+  // Element i of the thread's p-th vector.
+  auto at = [&](int p, int i) {
+    return kScalar ? ((p * w + part) * V + i) * 32 + lane : ((p * w + part) * 32 + lane) * V + i;
+  };
+  auto load = [&](const T *from, int p, float (&x)[V]) {
+    if constexpr (kScalar) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        x[i] = at(p, i) < dim ? to_f32(from[at(p, i)]) : 0.0f;
+    } else {
+      unpack(load_pack(from, at(p, 0), dim), x);
+    }
+  };
+  auto load_weights = [&](const void *from, int type, int p, float (&x)[V]) {
+    if constexpr (kScalar) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int e = at(p, i);
+        x[i] = 0.0f;
+        if (e < dim)
+          x[i] = type == CIM22_FLOAT32 ? static_cast<const float *>(from)[e]
+                                       : to_f32(static_cast<const T *>(from)[e]);
+      }
+    } else {
+      load_params<V>(from, type, at(p, 0), dim, x);
+    }
+  };
 
-  Pack<T> raw[kPer], res[kPer];
-  float v[kPer][V];
+  const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+  float v[kPer][V], res[kPer][V];
 #pragma unroll
   for (int p = 0; p < kPer; ++p)
-    raw[p] = load_pack(x, static_cast<int64_t>(p * (w << 5) + thread) * V - phase, a.dim);
-  if (residual) {
+    load(x, p, v[p]);
+  if (a.residual) {
+    const T *residual = static_cast<const T *>(a.residual) + row * a.residual_stride;
 #pragma unroll
     for (int p = 0; p < kPer; ++p)
-      res[p] = load_pack(residual, static_cast<int64_t>(p * (w << 5) + thread) * V - phase, a.dim);
+      load(residual, p, res[p]);
   }
-#pragma unroll
-  for (int p = 0; p < kPer; ++p)
-    unpack(raw[p], v[p]);
 
   auto normalise = [&](const NormArg &n) {
-    float mean = 0.0f;
+    float mean = 0.0f, s = 0.0f;
     if (n.kind == CIM22_NORM_LAYER) {
-      float s = 0.0f;
 #pragma unroll
       for (int p = 0; p < kPer; ++p)
 #pragma unroll
         for (int i = 0; i < V; ++i)
           s += v[p][i]; // zero outside the row
       mean = row_sum(s, a.warps_log2, buffer, slot) * inverse;
+      s = 0.0f;
     }
-    float s = 0.0f;
 #pragma unroll
-    for (int p = 0; p < kPer; ++p) {
-      const int64_t e = static_cast<int64_t>(p * (w << 5) + thread) * V - phase;
+    for (int p = 0; p < kPer; ++p)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        v[p][i] = (e + i >= 0 && e + i < a.dim) ? v[p][i] - mean : 0.0f;
+        v[p][i] = at(p, i) < dim ? v[p][i] - mean : 0.0f;
         s = fmaf(v[p][i], v[p][i], s);
       }
-    }
-    const float power = row_sum(s, a.warps_log2, buffer, slot) * inverse;
-    const float scale = rsqrtf(power + n.eps);
+    const float scale = rsqrtf(row_sum(s, a.warps_log2, buffer, slot) * inverse + n.eps);
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
-      const int64_t e = static_cast<int64_t>(p * (w << 5) + thread) * V - phase;
       float g[V];
       if (n.weight) {
-        load_params<V>(n.weight, n.type, e, a.dim, g);
+        load_weights(n.weight, n.type, p, g);
 #pragma unroll
         for (int i = 0; i < V; ++i)
           v[p][i] *= scale * g[i];
@@ -162,7 +180,7 @@ __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a)
           v[p][i] *= scale;
       }
       if (n.bias) {
-        load_params<V>(n.bias, n.type, e, a.dim, g);
+        load_weights(n.bias, n.type, p, g);
 #pragma unroll
         for (int i = 0; i < V; ++i)
           v[p][i] += g[i];
@@ -173,17 +191,12 @@ __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a)
   if (a.post.kind != CIM22_NORM_NONE)
     normalise(a.post);
   if (a.gate) {
-    const int64_t at = a.gate_rows ? row / a.gate_rows * a.gate_stride : 0;
-    const char *gate = static_cast<const char *>(a.gate) + at * (a.gate_type == CIM22_FLOAT32 ? 4 : 2);
+    const int64_t from = a.gate_rows ? row / a.gate_rows * a.gate_stride : 0;
+    const char *gate = static_cast<const char *>(a.gate) + from * (a.gate_type == CIM22_FLOAT32 ? 4 : 2);
     if (a.gate_columns == 1) {
-      float g;
-      if (a.gate_type == CIM22_FLOAT32)
-        g = *reinterpret_cast<const float *>(gate);
-      else if (a.gate_type == CIM22_BFLOAT16)
-        g = to_f32(*reinterpret_cast<const __nv_bfloat16 *>(gate));
-      else
-        g = to_f32(*reinterpret_cast<const __half *>(gate));
-      g = gate_fn(g, a.gate_act);
+      const float g = gate_fn(a.gate_type == CIM22_FLOAT32 ? *reinterpret_cast<const float *>(gate)
+                                                           : to_f32(*reinterpret_cast<const T *>(gate)),
+                              a.gate_act);
 #pragma unroll
       for (int p = 0; p < kPer; ++p)
 #pragma unroll
@@ -193,23 +206,19 @@ __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a)
 #pragma unroll
       for (int p = 0; p < kPer; ++p) {
         float g[V];
-        load_params<V>(gate, a.gate_type, static_cast<int64_t>(p * (w << 5) + thread) * V - phase,
-                       a.dim, g);
+        load_weights(gate, a.gate_type, p, g);
 #pragma unroll
         for (int i = 0; i < V; ++i)
           v[p][i] *= gate_fn(g[i], a.gate_act);
       }
     }
   }
-  if (residual) {
+  if (a.residual) {
 #pragma unroll
-    for (int p = 0; p < kPer; ++p) {
-      float r[V];
-      unpack(res[p], r);
+    for (int p = 0; p < kPer; ++p)
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        v[p][i] = fmaf(a.residual_scale, r[i], v[p][i]);
-    }
+        v[p][i] = fmaf(a.residual_scale, res[p][i], v[p][i]);
   }
   auto put = [&](void *out, int64_t stride) {
     if (!live)
@@ -217,9 +226,16 @@ __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a)
     T *to = static_cast<T *>(out) + row * stride;
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
-      Pack<T> o;
-      pack(v[p], o);
-      store_pack(to, static_cast<int64_t>(p * (w << 5) + thread) * V - phase, a.dim, o);
+      if constexpr (kScalar) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (at(p, i) < dim)
+            to[at(p, i)] = from_f32<T>(v[p][i]);
+      } else {
+        Pack<T> o;
+        pack(v[p], o);
+        store_pack(to, at(p, 0), dim, o);
+      }
     }
   };
   if (a.h)
@@ -507,9 +523,9 @@ cudaError_t launch_rows(const BlockNormArgs &a, int threads, cudaStream_t stream
 template <typename T>
 cudaError_t launch_block_norm(BlockNormArgs a, cudaStream_t stream) {
   constexpr int V = kVec<T>;
-  // Narrow rows share a CTA in the kernel below.
-  if (whole_vectors<T>(a) && a.dim > 64 * V) {
-    const int64_t vectors = a.dim / V;
+  const int64_t vectors = (a.dim + V - 1) / V;
+  const bool whole = whole_vectors<T>(a);
+  if (whole && vectors > 64) {
     if (vectors <= 256)
       return launch_rows<T, 1, true, 256>(a, static_cast<int>(round_up(vectors, 32)), stream);
     if (vectors <= 512)
@@ -526,28 +542,22 @@ cudaError_t launch_block_norm(BlockNormArgs a, cudaStream_t stream) {
       return launch_rows<T, 8, false, 512>(a, 512, stream);
     }
   }
-  const bool aligned = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.x_stride % V == 0;
-  const int64_t vectors = (a.dim + (aligned ? 0 : V - 1) + V - 1) / V;
   // Vectors a thread and warps a row: the fewest warps that hold the row.
   int per = 1, log2w = 0;
-  while (per < 4 && (int64_t{32} * per) < vectors)
+  while (per < 4 && int64_t{32} * per < vectors)
     per *= 2;
   while ((int64_t{32} * per << log2w) < vectors)
     ++log2w;
-  if (log2w > 5) { // the widest rows, off a vector boundary: one vector too many
-    per = 8;
-    log2w = 5;
-  }
   a.warps_log2 = log2w;
   const int warps = std::max(8, 1 << log2w);
-  const int64_t rows_per = warps >> log2w;
-  const int64_t grid = (a.rows + rows_per - 1) / rows_per;
-  const auto kernel = per == 1       ? block_norm_kernel<T, 1, 256>
-                      : per == 2     ? block_norm_kernel<T, 2, 256>
-                      : per == 8     ? block_norm_kernel<T, 8, 1024>
-                      : warps <= 8   ? block_norm_kernel<T, 4, 256>
-                      : warps <= 16  ? block_norm_kernel<T, 4, 512>
-                                     : block_norm_kernel<T, 4, 1024>;
+  const int64_t grid = (a.rows + (warps >> log2w) - 1) / (warps >> log2w);
+  constexpr int kWidest = V == 8 ? 512 : 1024; // threads of the widest row
+  const auto kernel = whole        ? per == 1 ? block_norm_kernel<T, 1, 256, false>
+                                              : block_norm_kernel<T, 2, 256, false>
+                      : per == 1   ? block_norm_kernel<T, 1, 256, true>
+                      : per == 2   ? block_norm_kernel<T, 2, 256, true>
+                      : warps <= 8 ? block_norm_kernel<T, 4, 256, true>
+                                   : block_norm_kernel<T, 4, kWidest, true>;
   return launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(warps * 32), 0, stream, a);
 }
 

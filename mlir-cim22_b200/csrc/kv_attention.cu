@@ -50,13 +50,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// Code + 1152 as f16: what codes_to_half gives before its subtraction.
-__device__ __forceinline__ void codes_to_half_raised(uint32_t w, uint32_t &lo, uint32_t &hi) {
-  w ^= 0x80808080u;
-  lo = __byte_perm(w, 0x64646464u, 0x4140);
-  hi = __byte_perm(w, 0x64646464u, 0x4342);
-}
-
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
@@ -113,7 +106,6 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   constexpr int kRounds = kRing<kCh, kParts, kQ> / kG; // rounds in the ring
   constexpr int kBytes = kGroupBytes<kCh>;
   constexpr int kRows = 8 * kQ;
-  constexpr bool kRaised = kParts == 1; // keys enter with 1152 added
   extern __shared__ uint8_t raw[];
   uint8_t *smem = raw + ((1024u - (smem_at(raw) & 1023u)) & 1023u);
   __shared__ uint64_t full[kWarps][kRounds];
@@ -232,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
   // Query rows f0 + 8 t + g as B fragments (lane (g, c) holds the elements
   // whose codes lane (., c) holds); results come out for rows 2c and 2c + 1.
   uint32_t qb[kQ][kParts][kCh * 4][2];
-  float coef[kQ][2], start[kQ][2];
+  float coef[kQ][2];
   int pos[kQ][2];
 #pragma unroll
   for (int t = 0; t < kQ; ++t) {
@@ -246,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
 #pragma unroll
     for (int o = 1; o < 4; o *= 2)
       amax = nan_max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    float factor, inverse, sum = 0.0f;
+    float factor, inverse;
     row_factor(amax, factor, inverse);
     // A row with NaN or infinity gives NaN wherever it sees a key.
     const bool wild = !(amax < INFINITY);
@@ -256,20 +248,14 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
       const float y0 = wild ? 0.0f : x[e] * factor, y1 = wild ? 0.0f : x[e + 1] * factor;
       const uint32_t h = pack_half(y0, y1);
       const float2 back = unpack_half(h);
-      sum += back.x + back.y;
       // Elements 4x .. 4x + 3 of a lane are columns 2c, 2c + 1, 2c + 8, 2c + 9.
       qb[t][0][e / 4][(e & 2) / 2] = h;
       if constexpr (kParts == 2)
         qb[t][1][e / 4][(e & 2) / 2] = pack_half(y0 - back.x, y1 - back.y);
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       coef[t][r] = __shfl_sync(0xffffffffu, mine, (2 * c + r) * 4);
-      // The raised keys add 1152 times the row's sum. Its roundings stay 30
-      // times below half a step of bf16 or f16 in the scores.
-      start[t][r] = kRaised ? -1152.0f * __shfl_sync(0xffffffffu, sum, (2 * c + r) * 4) : 0.0f;
       const int fr = f0 + 8 * t + 2 * c + r;
       pos[t][r] = fr < rows ? offset + fr / a.group : -0x40000000;
     }
@@ -336,8 +322,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     for (int u = 0; u < kG; ++u)
 #pragma unroll
       for (int t = 0; t < kQ; ++t) {
-        sc[u][t][0] = sc[u][t][2] = start[t][0];
-        sc[u][t][1] = sc[u][t][3] = start[t][1];
+        sc[u][t][0] = sc[u][t][1] = sc[u][t][2] = sc[u][t][3] = 0.0f;
       }
 #pragma unroll
     for (int ch = 0; ch < kCh; ++ch) {
@@ -355,13 +340,8 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
 #pragma unroll
         for (int u = 0; u < kG; ++u) {
           uint32_t f[4];
-          if constexpr (kRaised) {
-            codes_to_half_raised(w[u][0][x], f[0], f[2]);
-            codes_to_half_raised(w[u][1][x], f[1], f[3]);
-          } else {
-            codes_to_half(w[u][0][x], f[0], f[2]);
-            codes_to_half(w[u][1][x], f[1], f[3]);
-          }
+          codes_to_half(w[u][0][x], f[0], f[2]);
+          codes_to_half(w[u][1][x], f[1], f[3]);
 #pragma unroll
           for (int t = 0; t < kQ; ++t) {
             if constexpr (kParts == 2)
@@ -723,7 +703,8 @@ struct Plan {
   int splits;  // parts of the key axis,
   int cluster; // so many of them joined within the kernel
   int64_t tiles;
-  size_t bytes; // of the partial results
+  size_t bytes; // of the workspace: the parts' results, then
+  size_t carry; // what f32 prompts carry from tile to tile (0: nothing)
 };
 
 // Up to kDecodeRows query rows a sequence and kv head go to the decode kernel.
@@ -752,6 +733,12 @@ Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   p.bytes = parts == 1 ? 0
                        : static_cast<size_t>(parts) * v.rows * t.q_heads *
                              (static_cast<size_t>(v.dim) * 4 + 8);
+  // More than two tiles of 128 keys for each of a CTA's two streams.
+  if (p.prompt && t.type == CIM22_FLOAT32 && (longest + p.splits - 1) / p.splits > 512) {
+    p.bytes = (p.bytes + 15) / 16 * 16;
+    p.carry = static_cast<size_t>(p.splits) * 2 * v.rows * t.q_heads * (v.dim > 64 ? 128 : 64) * 4;
+    p.bytes += p.carry;
+  }
   return p;
 }
 
@@ -883,8 +870,10 @@ int cim22_cuda_kv_attend(const cim22_kv_cache *cache, const cim22_kv_sequences *
   a.splits = plan.splits;
   a.cluster = plan.cluster;
   a.part_o = static_cast<float *>(workspace);
-  a.part_ml = plan.bytes ? reinterpret_cast<float2 *>(a.part_o + static_cast<size_t>(plan.splits / plan.cluster) * v.rows * a.q_heads * v.dim)
+  a.part_ml = plan.splits > plan.cluster ? reinterpret_cast<float2 *>(a.part_o + static_cast<size_t>(plan.splits / plan.cluster) * v.rows * a.q_heads * v.dim)
                          : nullptr;
+  a.carry = plan.carry ? reinterpret_cast<float *>(static_cast<char *>(workspace) + (plan.bytes - plan.carry))
+                       : nullptr;
   a.status = status;
   const auto s = static_cast<cudaStream_t>(stream);
   const cudaError_t e =

@@ -20,6 +20,9 @@ struct KvAttendArgs {
   int cluster;    // so many neighbouring ones joined within the kernel
   float *part_o;   // [splits / cluster][rows * q_heads][dim], relative to 2^m,
   float2 *part_ml; // [splits / cluster][rows * q_heads] (m, l), when not one
+  // For prompts of f32 queries, or null: what each stream has taken out of its
+  // accumulators, [splits][2][kv_heads][64 or 128][rows * group].
+  float *carry;
   int32_t *status;
 };
 

@@ -37,6 +37,11 @@ namespace {
 constexpr int kThreads = 768, kM = 128, kTile = 128; // query rows a stream, keys a tile
 constexpr int kSub = 64, kIndex = 8; // tokens converted at a time, and indexed ahead
 constexpr int kPanel = 128 * 128;    // bytes: 128 rows of 64 f16
+// The products' accumulation does not round to nearest: f32 outputs lost half
+// their accuracy to it over 1,500 keys (1.25e-6 relative; 4.8e-6 over 8,192). With
+// two parts a stream's sum is therefore taken out of the accumulators every
+// kFlush tiles and added to what it carries in memory, rounding to nearest.
+constexpr int kFlush = 2;
 constexpr uint64_t kWaitLimit = 2000000000ull; // ns
 
 template <int kCh> struct alignas(1024) PromptSmem {
@@ -424,6 +429,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     const int row_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     const float coef = sm.coef[kShare ? row : st * kM + row];
     float m = kNone, l = 0.0f;
+    // What the stream carries: [split][stream][kv head][element][packed row],
+    // to be multiplied by `carried`.
+    const int64_t plane = v.rows * a.group;
+    float *carry = kParts == 2 && a.carry
+                       ? a.carry + ((static_cast<int64_t>(split) * 2 + st) * v.heads + head) * kD * plane +
+                             s.row0 * a.group + (live ? f : 0)
+                       : nullptr;
+    float carried = 0.0f; // nothing yet
     const int mine = kShare ? (count - st + 1) / 2 : count;
     bool ok = true;
 #pragma unroll 1
@@ -458,7 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         const float shrink = grown ? exp2_approx(m - to) : 1.0f; // 0 for the first
         m = grown ? to : m;
         l *= shrink;
-        if (n > 0) {
+        carried *= shrink;
+        if (n > 0 && !(carry && n % kFlush == 0)) {
           ok = bar_wait(&sm.o_full[st], (n - 1) & 1, failed) && ok;
           __syncwarp();
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -503,6 +517,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       sm.tops[n & 1][st][half][row] = top;
       asm volatile("bar.sync %0, 64;" ::"r"(2 + st * 4 + (warp & 3)) : "memory");
       top = fmaxf(top, sm.tops[n & 1][st][half ^ 1][row]);
+      if (kParts == 2 && carry && n > 0 && n % kFlush == 0) {
+        ok = bar_wait(&sm.o_full[st], (n - 1) & 1, failed) && ok;
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+        for (int d = half * (kD / 2); d < (half + 1) * (kD / 2); d += 8) {
+          uint32_t y[8];
+          tmem_load8(o_at + d, y);
+          if (live) {
+            float old[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              old[i] = n > kFlush ? carry[(d + i) * plane] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              carry[(d + i) * plane] = fmaf(old[i], carried, __uint_as_float(y[i]));
+          }
+        }
+        carried = 1.0f;
+      }
       const bool grown = top > (m == kNone ? -INFINITY : m + kGrowth<kParts>);
       if (__any_sync(0xffffffffu, grown))
         refer(grown, top - kTop<kParts>);
@@ -576,8 +610,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
             uint32_t x[32];
             tmem_load(o_at + 32 * c, x);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              joined[(32 * c + i) * kM + row] = __uint_as_float(x[i]);
+            for (int i = 0; i < 32; ++i) {
+              float o = __uint_as_float(x[i]);
+              if (carry && mine > kFlush && live)
+                o = fmaf(carry[(32 * c + i) * plane], carried, o);
+              joined[(32 * c + i) * kM + row] = o;
+            }
           }
         }
       }
@@ -606,7 +644,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
           // Where a stream had no keys its accumulators hold nothing.
-          float o = share == 0.0f ? 0.0f : __uint_as_float(x[k]) * share;
+          float o = __uint_as_float(x[k]);
+          if (kParts == 2 && carry && mine > kFlush && live)
+            o = fmaf(carry[(32 * c + k) * plane], carried, o);
+          o = share == 0.0f ? 0.0f : o * share;
           if constexpr (kShare)
             if (other != 0.0f)
               o = fmaf(joined[(32 * c + k) * kM + row], other, o);
@@ -763,6 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         const int tile = kShare ? 2 * n + st : n, slot = kShare ? st : u;
         if (tile >= count || !ready(1, tile, slot) || !wait(&sm.p_full[st], n & 1))
           return;
+        const bool fresh = n == 0 || (kParts == 2 && a.carry && n % kFlush == 0);
         if (elect()) {
 #pragma unroll
           for (int part = 0; part < kParts; ++part)
@@ -770,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
             for (int i = 0; i < kTile / 16; ++i)
               mma_ts(tmem + 2 * kTile + st * kD,
                      tmem + st * kTile + ((i / 2) * 32 + (i % 2) * 8 + (kParts - 1 - part) * 16),
-                     v_desc + (slot * kSlot + i * (2048 / 16)), kO, n > 0 || part + i > 0);
+                     v_desc + (slot * kSlot + i * (2048 / 16)), kO, !fresh || part + i > 0);
           commit(&sm.o_full[st]);
           if (kShare || st == 1)
             commit(&sm.kv_empty[1][slot]);
