@@ -813,7 +813,8 @@ int cim22_cuda_block_norm(const cim22_block_norm *description, void *stream);
 
 /* A paged key/value cache in 8 bits: int8 codes [pages][kv_heads][2][block]
  * [head_dim] (0 = key, 1 = value) and one f32 scale [pages][kv_heads][2] for
- * each block of tokens, head and side; a code q stands for q * scale. Token p
+ * each block of tokens, head and side (never negative); a code q stands for
+ * q * scale. Token p
  * of sequence b lies in page table[b * table_stride + p / block]. Pages may
  * be shared by sequences that only read them.
  *
@@ -869,7 +870,7 @@ int cim22_cuda_kv_read(const cim22_kv_cache *cache, const cim22_kv_sequences *se
  * sits at position lengths[b] - n_b + i; causal: it sees positions up to its
  * own, otherwise all lengths[b]; window > 0: only positions above its own
  * minus window. A query that sees nothing gives zeros and lse = -inf. out is
- * contiguous [rows][q_heads][head_dim] of q's type; lse (or NULL) is f32
+ * contiguous [rows][q_heads][head_dim] of q's type and does not overlap q; lse (or NULL) is f32
  * [rows][q_heads], the natural logarithm of the sum of exp(score). */
 typedef struct cim22_kv_attention {
   int32_t type;

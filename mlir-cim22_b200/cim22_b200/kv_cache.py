@@ -14,7 +14,11 @@ tensors therefore serve the write of a step's keys and values and the
 attention of its queries. Lengths, starts and table live on the device, so a
 step can be captured into a CUDA graph and replayed with new contents.
 ``most`` bounds a sequence's rows in the call and ``longest`` its length; both
-are host numbers that size the launch (a graph's have to cover every replay).
+are host numbers that size the launch (a graph's ``most`` has to cover every
+replay; any ``longest`` gives the right results). Under capture, and to avoid a
+synchronization in every call, pass ``status``: without it each call makes a
+status word of its own and reads it back. A ``workspace`` belongs to calls that
+run one after another, graphs among them.
 """
 
 from __future__ import annotations
@@ -45,7 +49,8 @@ class Int8KVCache:
     @classmethod
     def over(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Int8KVCache":
         """A cache over existing tensors: int8 codes [pages, kv_heads, 2, block,
-        head_dim] and f32 scales [pages, kv_heads, 2], both contiguous."""
+        head_dim] and f32 scales [pages, kv_heads, 2] (never negative), both
+        contiguous."""
         if codes.dim() != 5 or codes.shape[2] != 2:
             raise ValueError("codes must be [pages, kv_heads, 2, block, head_dim]")
         cls._shape_check(codes.shape[0], codes.shape[1], codes.shape[4], codes.shape[3])
@@ -195,7 +200,7 @@ class Int8KVCache:
         a sequence's n sits at position lengths[b] - n + i. causal: it sees
         positions up to its own; window > 0: only the last window of them. A
         query that sees nothing gives zeros. scale defaults to
-        head_dim ** -0.5. Returns out [rows, q_heads, head_dim] of q's type, or
+        head_dim ** -0.5; out must not overlap q. Returns out [rows, q_heads, head_dim] of q's type, or
         (out, lse) with the f32 logarithm of each row's sum of exponentials.
         longest: the longest of lengths (default: what the table can hold)."""
         if q.dim() != 3:
@@ -219,6 +224,8 @@ class Int8KVCache:
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device \
                 or not out.is_contiguous():
             raise TypeError("out must be contiguous, of q's shape and type")
+        elif out.data_ptr() == q.data_ptr() and q.numel():
+            raise ValueError("out must not be q")
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) \
             if return_lse else None
         call = abi.KvAttention(FLOAT_TYPES[q.dtype], heads, q.data_ptr(), q.stride(0),

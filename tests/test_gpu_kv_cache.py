@@ -243,6 +243,48 @@ def test_long_axis_is_split_and_joined(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [48, 128])
+def test_a_chunk_against_a_long_context(dtype, dim):
+    """Many tiles of keys for each of a CTA's two query streams (f32 takes its
+    sums out of the accumulators between them), one part and several."""
+    s = Setup([2900], 1, dim, 32)
+    s.fill()
+    s.check_attend([40], dtype, group=2, longest=1024)
+    s.check_attend([40], dtype, group=2)
+    s.check_attend([150], dtype, group=2, longest=1024, window=1500)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_large_score_late_in_the_context(dtype):
+    """References are set again in the middle of the keys, for some rows only."""
+    s = Setup([700], 1, 64, 64)
+    k, v = s.rows(700, 1, torch.float32), s.rows(700, 1, torch.float32)
+    k[300] *= 12
+    k[600] *= 40
+    s.host.write(k, v, s.table, [700], [0, 700])
+    table, at, first = s.device([700], [0, 700])
+    s.cache.write(k.cuda(), v.cuda(), table, at, first, status=s.status)
+    s.check_attend([1], dtype, group=8, starts=None)
+    s.check_attend([90], dtype, group=2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_an_empty_cache(dtype):
+    cache = Int8KVCache(0, 1, 32, 16)
+    status = StatusWord(torch.device("cuda", 0))
+    table = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    at = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for n in (1, 40):
+        first = torch.tensor([0, n, 2 * n], dtype=torch.int32, device="cuda")
+        q = torch.ones(2 * n, 2, 32, dtype=dtype, device="cuda")
+        out, lse = cache.attend(q, table, at, first, return_lse=True, status=status)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    status.raise_if_set()
+    none = cache.attend(q[:0], table[:0], at[:0], status=status)
+    assert none.shape == (0, 2, 32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_scales_that_differ_by_blocks(dtype):
     """Value scales 1e-6 to 1e6 and key scales apart: probabilities carry the
     value scale in their exponent."""
@@ -257,8 +299,9 @@ def test_scales_that_differ_by_blocks(dtype):
     s.cache.write(k.cuda(), v.cuda(), table, at, first, status=s.status)
     s.check_attend([128], dtype, group=1)
     s.check_attend([1], dtype, group=1, starts=None)
-    s.check_attend([3], dtype, group=1, scale=-0.3)
-    s.check_attend([3], dtype, group=1, scale=0.0)
+    for new in (3, 128):
+        s.check_attend([new], dtype, group=1, scale=-0.3)
+        s.check_attend([new], dtype, group=1, scale=0.0)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -325,12 +368,13 @@ def bad_descriptions(s):
 @pytest.mark.parametrize("which", ["page past the cache", "negative page", "length past the table",
                                    "negative length", "starts run backwards",
                                    "starts past the rows"])
-def test_bad_descriptions_are_reported_not_followed(which):
+@pytest.mark.parametrize("group", [2, 8])
+def test_bad_descriptions_are_reported_not_followed(which, group):
     s = Setup([12, 9], 1, 16, 16)
     s.fill()
     s.status.raise_if_set()
     table, at, first = bad_descriptions(s)[which]
-    q = s.rows(9, 2, torch.float32).cuda()
+    q = s.rows(9, group, torch.float32).cuda()
     k = s.rows(9, 1, torch.float32).cuda()
     calls = [lambda: s.cache.attend(q, table, at, first, status=s.status),
              lambda: s.cache.read(table, at, first, tokens=9, status=s.status),
@@ -415,6 +459,32 @@ def test_captured_step_takes_new_contents():
     s.status.raise_if_set()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_captured_prompt_takes_new_contents(dtype):
+    s = Setup([300, 90], 2, 128, 64)
+    s.fill()
+    table, at, first = s.device(s.lengths, [0, 70, 120])
+    workspace = Workspace(torch.device("cuda", 0))
+    q = s.rows(120, 4, dtype).cuda()
+
+    def step():
+        return s.cache.attend(q, table, at, first, most=70, longest=300, workspace=workspace,
+                              status=s.status)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for n in (300, 250, 71):
+        q.copy_(s.rows(120, 4, dtype))
+        at[0] = n
+        graph.replay()
+        assert torch.equal(out, s.cache.attend(q, table, at, first, most=70, longest=300,
+                                               status=s.status))
+    s.status.raise_if_set()
+
+
 def test_results_repeat_and_do_not_hang_on_streams():
     s = Setup([900, 40, 300], 2, 128, 64)
     s.fill()
@@ -446,6 +516,7 @@ def test_results_repeat_and_do_not_hang_on_streams():
     lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st[:2]),
     lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st, out=q.half()),
     lambda s, q, k, t, n, st: s.cache.attend(q.cpu(), t, n, st),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st, out=q),
     lambda s, q, k, t, n, st: s.cache.write(k, k.half(), t, n, st),
     lambda s, q, k, t, n, st: s.cache.write(k, k[:8], t, n, st),
     lambda s, q, k, t, n, st: s.cache.write(q, q, t, n, st),
