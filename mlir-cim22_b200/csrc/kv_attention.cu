@@ -707,8 +707,15 @@ struct Plan {
   size_t carry; // what f32 prompts carry from tile to tile (0: nothing)
 };
 
-// Up to kDecodeRows query rows a sequence and kv head go to the decode kernel.
-constexpr int64_t kDecodeRows = 32;
+// Up to kDecodeRows query rows a sequence and kv head go to the decode kernel
+// (decode | prompt, head_dim 128, bf16, 8 kv heads, L2 flushed: 32 sequences of
+// 4,096 with 32 rows 145 | 197 us, 48 rows 195 | 199, 64 rows 244 | 197; one of
+// 32,768 46 | 63, 58 | 65, 75 | 65). So do more rows where all of its tiles of 16
+// have a place at once and come to kDecodeWork keys (one sequence of 2,000 with
+// 256 rows 32 | 54 us; 4 of 1,000 with 128 rows 33 | 39; twice the work, 4 of
+// 2,000 with 128 rows, 49 | 48; more tiles than places, 16 of 300 with 64 rows,
+// 37 | 27): the prompt kernel starts with some 25 us of filling and joining.
+constexpr int64_t kDecodeRows = 32, kDecodeWork = 1 << 18;
 
 Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   Plan p{};
@@ -716,13 +723,17 @@ Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   const int64_t rows = std::min<int64_t>(v.most, v.rows) * group;
   const int64_t held = static_cast<int64_t>(v.table_width) << v.block_log2;
   const int64_t longest = std::max<int64_t>(1, std::min(t.longest, held));
-  p.prompt = rows > kDecodeRows;
+  const int64_t tiles16 = (rows + 15) / 16 * v.heads * v.batch;
+  const int resident = t.type == CIM22_FLOAT32 && rows > 8 ? 2 : 3;
+  p.prompt =
+      rows > kDecodeRows && (tiles16 > 148 * resident || tiles16 * longest > kDecodeWork);
+  // One query tile a CTA up to 128 rows: 32 sequences of 4,096 with 64 rows 199
+  // us, as two half-empty tiles 285; 192 rows the other way round, 363 and 260.
   p.share = p.prompt && (t.type == CIM22_FLOAT32 || rows <= 128);
   if (!p.prompt) {
     p.few = rows <= 8;
     p.tiles = (rows + (p.few ? 7 : 15)) / (p.few ? 8 : 16);
-    decode_parts(v, p.tiles, longest, t.type == CIM22_FLOAT32 && !p.few ? 2 : 3, p.splits,
-                 p.cluster);
+    decode_parts(v, p.tiles, longest, resident, p.splits, p.cluster);
   } else {
     p.tiles = (rows + (p.share ? 127 : 255)) / (p.share ? 128 : 256);
     const int64_t items = p.tiles * v.heads * v.batch;
@@ -849,7 +860,7 @@ int cim22_cuda_kv_attend(const cim22_kv_cache *cache, const cim22_kv_sequences *
     set_last_error("cim22_cuda_kv_attend: workspace too small or not 16-byte aligned");
     return bad;
   }
-  if (plan.tiles * v.heads > 65535) {
+  if (plan.tiles * v.heads > 0x7fffffff) { // (decode's fit its axis by the choice above)
     set_last_error("cim22_cuda_kv_attend: too many query rows");
     return bad;
   }

@@ -329,10 +329,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   }
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.z, split = blockIdx.x;
-  const int head = blockIdx.y % v.heads;
+  const int b = blockIdx.z, split = blockIdx.y;
+  const int head = blockIdx.x % v.heads;
   // The last tiles of a causal prompt see the most keys: they start first.
-  const int f0 = (tiles - 1 - static_cast<int>(blockIdx.y) / v.heads) * kRows;
+  const int f0 = (tiles - 1 - static_cast<int>(blockIdx.x / v.heads)) * kRows;
   const KvSequence s = kv_sequence(v, b);
   if (!s.ok) {
     if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0)
@@ -905,7 +905,7 @@ cudaError_t launch_prompt(const KvAttendArgs &a, int tiles, cudaStream_t stream)
   static DynamicSmem allowed;
   if (const cudaError_t e = allowed.allow(kernel, bytes); e != cudaSuccess)
     return e;
-  return launch_pdl(kernel, dim3(a.splits, static_cast<unsigned>(tiles * a.v.heads), a.v.batch),
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles) * a.v.heads, a.splits, a.v.batch),
                     dim3(kThreads), bytes, stream, a, tiles);
 }
 

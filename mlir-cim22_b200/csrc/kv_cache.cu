@@ -269,11 +269,19 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Blocks that n consecutive tokens can touch.
-unsigned touched(const KvView &v) {
+// CTAs for the heads and sides of the blocks that a sequence's rows can touch.
+int64_t planes_touched(const KvView &v) {
   const int block = 1 << v.block_log2;
   const int64_t most = std::min<int64_t>(v.most, static_cast<int64_t>(v.table_width) * block);
-  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 2 * block - 2) / block, v.table_width)));
+  const int64_t touched = std::min<int64_t>((most + 2 * block - 2) / block, v.table_width);
+  return std::max<int64_t>(1, touched) * v.heads * 2;
+}
+
+bool too_many(const char *what, const KvView &v) {
+  if (planes_touched(v) <= 0x7fffffff)
+    return false;
+  set_last_error(std::string(what) + ": too many rows a sequence for one call");
+  return true;
 }
 
 template <typename T>
@@ -288,14 +296,14 @@ cudaError_t launch_write(const KvView &v, const Rows &keys, const Rows &values, 
                       : per <= 4 ? kv_write_kernel<T, 4>
                       : per <= 8 ? kv_write_kernel<T, 8>
                                  : kv_write_kernel<T, 128 * 128 / kVec<T> / kThreads>;
-  return launch_pdl(kernel, dim3(touched(v) * v.heads * 2, v.batch), dim3(threads), 0, stream, v,
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(planes_touched(v)), v.batch), dim3(threads), 0, stream, v,
                     keys, values, make_fastdiv(parts), status);
 }
 
 template <typename T>
 cudaError_t launch_read(const KvView &v, void *k, void *values, int32_t *status,
                         cudaStream_t stream) {
-  return launch_pdl(kv_read_kernel<T>, dim3(touched(v) * v.heads * 2, v.batch), dim3(kThreads), 0,
+  return launch_pdl(kv_read_kernel<T>, dim3(static_cast<unsigned>(planes_touched(v)), v.batch), dim3(kThreads), 0,
                     stream, v, static_cast<T *>(k), static_cast<T *>(values),
                     make_fastdiv(v.dim / kVec<T>), status);
 }
@@ -325,6 +333,8 @@ int cim22_cuda_kv_write(const cim22_kv_cache *cache, const cim22_kv_sequences *s
   }
   if (view.batch == 0 || view.rows == 0)
     return 0;
+  if (too_many("cim22_cuda_kv_write", view))
+    return bad;
   const Rows keys{k, k_row_stride, k_head_stride}, values{v, v_row_stride, v_head_stride};
   const auto s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = type == CIM22_FLOAT32    ? launch_write<float>(view, keys, values, status, s)
@@ -345,6 +355,8 @@ int cim22_cuda_kv_read(const cim22_kv_cache *cache, const cim22_kv_sequences *se
   }
   if (view.batch == 0 || view.rows == 0 || (!k && !v))
     return 0;
+  if (too_many("cim22_cuda_kv_read", view))
+    return bad;
   const auto s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = type == CIM22_FLOAT32    ? launch_read<float>(view, k, v, status, s)
                         : type == CIM22_BFLOAT16 ? launch_read<__nv_bfloat16>(view, k, v, status, s)

@@ -60,6 +60,21 @@ def test_write_and_read_refuse(c, s):
     assert native.last_error().startswith("cim22_cuda_kv_read: ")
 
 
+def test_launches_past_the_grid_are_refused():
+    lib = native.lib()
+    wide = ctypes.byref(cache(kv_heads=32767))
+    long = ctypes.byref(sequences(rows=2 ** 30, most=2 ** 30, table_width=2 ** 20,
+                                  table_stride=2 ** 20))
+    assert lib.cim22_cuda_kv_write(wide, long, abi.FLOAT16, HERE, 64, 32, HERE, 64, 32, HERE,
+                                   None) != 0
+    assert "too many rows" in native.last_error()
+    assert lib.cim22_cuda_kv_read(wide, long, abi.FLOAT16, HERE, HERE, HERE, None) != 0
+    assert "too many rows" in native.last_error()
+    call = ctypes.byref(attention(type=abi.FLOAT16, q_heads=32767))
+    assert lib.cim22_cuda_kv_attend(wide, long, call, HERE, 1 << 40, HERE, None) != 0
+    assert "too many query rows" in native.last_error()
+
+
 def test_null_and_unknown_arguments_are_refused():
     lib = native.lib()
     c, s, a = cache(), sequences(), attention()

@@ -83,10 +83,17 @@ class Setup:
         for n in new:
             first.append(first[-1] + n)
         table, at, dev_starts = self.device(self.lengths, first if starts == "rows" else None)
-        out, lse = self.cache.attend(q.cuda(), table, at, dev_starts, causal=causal,
-                                     window=window, scale=scale, return_lse=True,
-                                     status=self.status, **kw)
-        self.status.raise_if_set()
+        # Rows behind the last sequence choose the kernel: as given, more than
+        # the decode kernel takes, and enough that the keys are not split.
+        runs = []
+        for least in (0, 7200, 38000) if starts == "rows" else (0,):
+            pad = max(0, least // (heads * len(new)) + 1 - total) if least else 0
+            more = torch.cat([q, torch.full((pad, heads, self.dim), math.nan, dtype=dtype)])
+            out, lse = self.cache.attend(more.cuda(), table, at, dev_starts, causal=causal,
+                                         window=window, scale=scale, return_lse=True,
+                                         status=self.status, **kw)
+            self.status.raise_if_set()
+            runs.append((out[:total], lse[:total]))
         parts = 2 if dtype == torch.float32 else 1
         step = 2.0 ** -22  # one product or sum of the tensor cores, truncation allowed for
         # A probability is off by half a step of f16 (one part) or of its two
@@ -103,8 +110,6 @@ class Setup:
             want, want_lse, size, reach, peak = ref.attend(
                 q[first[b]:first[b + 1]], k, v, keys - n, s, causal, window,
                 self.host.value_scales(self.table[b], keys))
-            got = out[first[b]:first[b + 1]].double().cpu()
-            got_lse = lse[first[b]:first[b + 1]].double().cpu()
             # Score error: the contraction's steps, the queries' parts and the
             # exponent's own rounding (arguments below 128).
             delta = (parts * (self.dim / 16) + 6) * step * reach + 130 * 2.0 ** -24
@@ -113,14 +118,18 @@ class Setup:
                 2 * p_err + 2 * delta + steps)[..., None] + floor * peak[..., None]
             if dtype == torch.float16:
                 tol = tol + 2.0 ** -25
-            off = (got - want).abs()
-            assert bool((off <= tol).all()), (b, float((off / tol.clamp(min=1e-300)).max()))
             seen = torch.isfinite(want_lse)
-            assert torch.equal(seen, torch.isfinite(got_lse))
-            assert bool((got_lse[~seen] == -math.inf).all())
             lse_tol = delta + steps + 2.0 ** -23 * want_lse.abs()
-            assert bool(((got_lse - want_lse).abs() <= lse_tol)[seen].all())
-        return out
+            for run, (out, lse) in enumerate(runs):
+                got = out[first[b]:first[b + 1]].double().cpu()
+                got_lse = lse[first[b]:first[b + 1]].double().cpu()
+                off = (got - want).abs()
+                assert bool((off <= tol).all()), (
+                    run, b, float((off / tol.clamp(min=1e-300)).max()))
+                assert torch.equal(seen, torch.isfinite(got_lse))
+                assert bool((got_lse[~seen] == -math.inf).all())
+                assert bool(((got_lse - want_lse).abs() <= lse_tol)[seen].all())
+        return runs[0][0]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -185,7 +194,7 @@ def test_values_of_all_sizes_and_not_finite():
 def test_rows_of_a_fused_projection(dtype):
     """Strided views, rows off a 16-byte boundary too."""
     s = Setup([37, 20], 2, 32, 16)
-    for base, pad in ((0, 0), (3, 1)):
+    for base, pad, more in ((0, 0, 0), (3, 1, 0), (0, 0, 4000), (3, 1, 4000)):
         flat = torch.randn(57 * (6 * 32 + pad) + 8, generator=s.g).to(dtype)
         fused = flat.as_strided((57, 6, 32), (6 * 32 + pad, 32, 1), base)
         k, v = fused[:, 2:4], fused[:, 4:6]
@@ -194,9 +203,14 @@ def test_rows_of_a_fused_projection(dtype):
         table, at, first = s.device(s.lengths, [0, 37, 57])
         s.cache.write(dev[:, 2:4], dev[:, 4:6], table, at, first, status=s.status)
         s.check_read(dtype)
-        want = s.cache.attend(dev[:, 0:2].contiguous(), table, at, first, status=s.status)
-        got = s.cache.attend(dev[:, 0:2], table, at, first, status=s.status)
-        assert torch.equal(got, want)
+        q = dev[:, 0:2]
+        if more: # rows behind the last sequence: the prompt kernel
+            q = torch.empty(base + (57 + more) * (6 * 32 + pad), dtype=dtype, device="cuda"
+                            ).as_strided((57 + more, 2, 32), (6 * 32 + pad, 32, 1), base)
+            q[:57] = dev[:, 0:2]
+        want = s.cache.attend(q.contiguous(), table, at, first, status=s.status)
+        got = s.cache.attend(q, table, at, first, status=s.status)
+        assert torch.equal(got[:57], want[:57])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -255,6 +269,14 @@ def test_a_chunk_against_a_long_context(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_chunks_of_many_sequences(dtype):
+    """One tile of at most 128 query rows for both streams of a CTA."""
+    s = Setup([700, 704, 513, 130, 700, 0, 64, 129], 16, 32, 32)
+    s.fill()
+    s.check_attend([40, 33, 40, 40, 1, 0, 40, 17], dtype, group=1, most=40)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_a_large_score_late_in_the_context(dtype):
     """References are set again in the middle of the keys, for some rows only."""
     s = Setup([700], 1, 64, 64)
@@ -274,7 +296,7 @@ def test_an_empty_cache(dtype):
     status = StatusWord(torch.device("cuda", 0))
     table = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
     at = torch.zeros(2, dtype=torch.int32, device="cuda")
-    for n in (1, 40):
+    for n in (1, 40, 3000):
         first = torch.tensor([0, n, 2 * n], dtype=torch.int32, device="cuda")
         q = torch.ones(2 * n, 2, 32, dtype=dtype, device="cuda")
         out, lse = cache.attend(q, table, at, first, return_lse=True, status=status)
@@ -282,6 +304,26 @@ def test_an_empty_cache(dtype):
     status.raise_if_set()
     none = cache.attend(q[:0], table[:0], at[:0], status=status)
     assert none.shape == (0, 2, 32)
+
+
+def test_more_query_tiles_than_one_grid_axis_holds():
+    """32,767 kv heads x 3 tiles of 128 rows; a head's results are those it has
+    in a cache by itself."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    codes = torch.randint(-127, 128, (1, 32767, 2, 16, 16), generator=g, device="cuda",
+                          dtype=torch.int8)
+    scales = torch.rand(1, 32767, 2, generator=g, device="cuda") * 0.02 + 0.01
+    q = torch.randn(257, 1, 16, generator=g, device="cuda")
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    at = torch.tensor([16], dtype=torch.int32, device="cuda")
+    first = torch.tensor([0, 257], dtype=torch.int32, device="cuda")
+    out = Int8KVCache.over(codes, scales).attend(q.expand(257, 32767, 16), table, at, first,
+                                                 causal=False)
+    more = torch.cat([q, torch.zeros(8000, 1, 16, device="cuda")])  # the same kernel's
+    for h in (0, 1, 21844, 21845, 32766):
+        one = Int8KVCache.over(codes[:, h:h + 1].contiguous(), scales[:, h:h + 1].contiguous())
+        assert torch.equal(out[:, h:h + 1],
+                           one.attend(more, table, at, first, causal=False)[:257])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -316,10 +358,11 @@ def test_queries_of_all_sizes(dtype):
     s.check_attend([40], dtype, q=q)
 
 
-def test_not_finite_queries_stay_in_their_rows():
+@pytest.mark.parametrize("rows", [20, 4000])
+def test_not_finite_queries_stay_in_their_rows(rows):
     s = Setup([40], 1, 32, 16)
     s.fill()
-    q = s.rows(20, 2, torch.float32)
+    q = s.rows(rows, 2, torch.float32)
     clean = q.clone()
     q[3, 0, 5], q[7, 1, 0] = math.nan, math.inf
     table, at, first = s.device([40], [0, 20])
@@ -328,17 +371,18 @@ def test_not_finite_queries_stay_in_their_rows():
     assert bool(torch.isnan(got[3, 0]).all()) and bool(torch.isnan(got[7, 1]).all())
     keep = torch.ones(20, 2, dtype=torch.bool)
     keep[3, 0] = keep[7, 1] = False
-    assert torch.equal(got.cpu()[keep], want.cpu()[keep])
+    assert torch.equal(got[:20].cpu()[keep], want[:20].cpu()[keep])
 
 
 def test_rows_behind_the_last_sequence_are_left():
     s = Setup([20, 9], 1, 16, 16)
     s.fill()
-    q = s.rows(15, 2, torch.float32).cuda()
     table, at, first = s.device(s.lengths, [0, 6, 9])
-    out = torch.full((15, 2, 16), 5.0, device="cuda")
-    s.cache.attend(q, table, at, first, out=out, status=s.status)
-    assert bool((out[9:] == 5).all()) and not bool((out[:9] == 5).any())
+    for rows in (15, 3000):
+        q = s.rows(rows, 2, torch.float32).cuda()
+        out = torch.full((rows, 2, 16), 5.0, device="cuda")
+        s.cache.attend(q, table, at, first, out=out, status=s.status)
+        assert bool((out[9:] == 5).all()) and not bool((out[:9] == 5).any())
     k = torch.full((15, 1, 16), 5.0, device="cuda")
     v = k.clone()
     s.cache.read(table, at, first, out=(k, v), status=s.status)
@@ -359,7 +403,7 @@ def bad_descriptions(s):
     back = first.clone()
     back[1] = -3
     past = first.clone()
-    past[2] = 10
+    past[2] = 2001
     return {"page past the cache": (high, at, first), "negative page": (low, at, first),
             "length past the table": (table, long, first), "negative length": (table, negative, first),
             "starts run backwards": (table, at, back), "starts past the rows": (table, at, past)}
@@ -368,13 +412,13 @@ def bad_descriptions(s):
 @pytest.mark.parametrize("which", ["page past the cache", "negative page", "length past the table",
                                    "negative length", "starts run backwards",
                                    "starts past the rows"])
-@pytest.mark.parametrize("group", [2, 8])
-def test_bad_descriptions_are_reported_not_followed(which, group):
+@pytest.mark.parametrize("rows", [9, 2000])
+def test_bad_descriptions_are_reported_not_followed(which, rows):
     s = Setup([12, 9], 1, 16, 16)
     s.fill()
     s.status.raise_if_set()
     table, at, first = bad_descriptions(s)[which]
-    q = s.rows(9, group, torch.float32).cuda()
+    q = s.rows(rows, 2, torch.float32).cuda()
     k = s.rows(9, 1, torch.float32).cuda()
     calls = [lambda: s.cache.attend(q, table, at, first, status=s.status),
              lambda: s.cache.read(table, at, first, tokens=9, status=s.status),
@@ -460,16 +504,17 @@ def test_captured_step_takes_new_contents():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_captured_prompt_takes_new_contents(dtype):
-    s = Setup([300, 90], 2, 128, 64)
+@pytest.mark.parametrize("longest", [300, 40000])
+def test_captured_prompt_takes_new_contents(dtype, longest):
+    s = Setup([300, 90], 2, 128, 64, width=700)
     s.fill()
     table, at, first = s.device(s.lengths, [0, 70, 120])
     workspace = Workspace(torch.device("cuda", 0))
     q = s.rows(120, 4, dtype).cuda()
 
     def step():
-        return s.cache.attend(q, table, at, first, most=70, longest=300, workspace=workspace,
-                              status=s.status)
+        return s.cache.attend(q, table, at, first, most=70, longest=longest,
+                              workspace=workspace, status=s.status)
 
     step()
     torch.cuda.synchronize()
@@ -480,7 +525,7 @@ def test_captured_prompt_takes_new_contents(dtype):
         q.copy_(s.rows(120, 4, dtype))
         at[0] = n
         graph.replay()
-        assert torch.equal(out, s.cache.attend(q, table, at, first, most=70, longest=300,
+        assert torch.equal(out, s.cache.attend(q, table, at, first, most=70, longest=longest,
                                                status=s.status))
     s.status.raise_if_set()
 
