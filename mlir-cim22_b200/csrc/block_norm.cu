@@ -38,27 +38,6 @@ struct BlockNormArgs {
   int warps_log2; // warps a row, log2
 };
 
-// kVec parameter values at element e as f32 (`fill` outside the row).
-template <int N>
-__device__ __forceinline__ void load_params(const void *base, int type, int64_t e, int64_t count,
-                                            float (&out)[N]) {
-  if (type == CIM22_FLOAT32) {
-#pragma unroll
-    for (int c = 0; c < N; c += 4) {
-      const Pack<float> p = load_pack(static_cast<const float *>(base), e + c, count);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        out[c + i] = p.at[i];
-    }
-  } else if constexpr (N == 8) {
-    if (type == CIM22_BFLOAT16) {
-      unpack(load_pack(static_cast<const __nv_bfloat16 *>(base), e, count), out);
-    } else {
-      unpack(load_pack(static_cast<const __half *>(base), e, count), out);
-    }
-  }
-}
-
 __device__ __forceinline__ float gate_fn(float g, int act) {
   if (act == CIM22_GATE_SIGMOID)
     return 1.0f / (1.0f + expf(-g));
@@ -89,10 +68,11 @@ __device__ __forceinline__ float row_sum(float v, int warps_log2, float *buffer,
   return v;
 }
 
-// Narrow rows (several to a CTA) and, with kScalar, rows off vector boundaries.
-// There a warp's loads and stores take 32 neighbouring elements: lanes that
-// each took their own eight would spread every weight load over eight lines.
-template <typename T, int kPer, int kMax, bool kScalar>
+// Rows off vector boundaries, several to a CTA where they are narrow. A warp's
+// loads and stores take 32 neighbouring elements (lanes that each took their
+// own eight spread every weight load over eight lines: 3,001 x 1,001 f16, 31 us
+// against 19).
+template <typename T, int kPer, int kMax>
 __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a) {
   constexpr int V = kVec<T>;
   __shared__ float buffer[64];
@@ -107,31 +87,21 @@ __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a)
   const int dim = static_cast<int>(a.dim);
   const float inverse = 1.0f / static_cast<float>(dim);
   int slot = 0;
-  // Element i of the thread's p-th vector.
-  auto at = [&](int p, int i) {
-    return kScalar ? ((p * w + part) * V + i) * 32 + lane : ((p * w + part) * 32 + lane) * V + i;
-  };
+  // The thread's element i of its p-th group.
+  auto at = [&](int p, int i) { return ((p * w + part) * V + i) * 32 + lane; };
   auto load = [&](const T *from, int p, float (&x)[V]) {
-    if constexpr (kScalar) {
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        x[i] = at(p, i) < dim ? to_f32(from[at(p, i)]) : 0.0f;
-    } else {
-      unpack(load_pack(from, at(p, 0), dim), x);
-    }
+    for (int i = 0; i < V; ++i)
+      x[i] = at(p, i) < dim ? to_f32(from[at(p, i)]) : 0.0f;
   };
   auto load_weights = [&](const void *from, int type, int p, float (&x)[V]) {
-    if constexpr (kScalar) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = at(p, i);
-        x[i] = 0.0f;
-        if (e < dim)
-          x[i] = type == CIM22_FLOAT32 ? static_cast<const float *>(from)[e]
-                                       : to_f32(static_cast<const T *>(from)[e]);
-      }
-    } else {
-      load_params<V>(from, type, at(p, 0), dim, x);
+    for (int i = 0; i < V; ++i) {
+      const int e = at(p, i);
+      x[i] = 0.0f;
+      if (e < dim)
+        x[i] = type == CIM22_FLOAT32 ? static_cast<const float *>(from)[e]
+                                     : to_f32(static_cast<const T *>(from)[e]);
     }
   };
 
@@ -226,16 +196,10 @@ __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a)
     T *to = static_cast<T *>(out) + row * stride;
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
-      if constexpr (kScalar) {
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (at(p, i) < dim)
-            to[at(p, i)] = from_f32<T>(v[p][i]);
-      } else {
-        Pack<T> o;
-        pack(v[p], o);
-        store_pack(to, at(p, 0), dim, o);
-      }
+      for (int i = 0; i < V; ++i)
+        if (at(p, i) < dim)
+          to[at(p, i)] = from_f32<T>(v[p][i]);
     }
   };
   if (a.h)
@@ -281,12 +245,13 @@ __device__ __forceinline__ uint4 load_stream(const void *at) {
   return v;
 }
 
-// Rows of whole, aligned vectors: the case of every ordinary width. Each CTA
+// Rows of whole, aligned vectors: every ordinary width. Each CTA
 // keeps to its columns over many rows, so that it loads the weights once (kHold:
 // into registers) and has the next row's streams on their way while it reduces
 // this one. Measured on 32,768 x 4096 bf16 (two norms, a gate value a row): 237
-// us, 4.5 TB/s, against 410 us of the kernel above, which tests every element's
-// place and reads the weights for each row. What bounds it is the latency of a
+// us, 4.5 TB/s, against 410 us of a CTA for each few rows, which tests every element's
+// place and reads the weights each time (262,144 x 512: 195 and 265, x 64: 85
+// and 178). What bounds it is the latency of a
 // row's two reductions at 16 resident warps: with the weights left in memory 24
 // warps fit and take 283 us, 512 threads a row 310 us.
 template <typename T, int kPer, bool kHold, int kMax>
@@ -524,8 +489,7 @@ template <typename T>
 cudaError_t launch_block_norm(BlockNormArgs a, cudaStream_t stream) {
   constexpr int V = kVec<T>;
   const int64_t vectors = (a.dim + V - 1) / V;
-  const bool whole = whole_vectors<T>(a);
-  if (whole && vectors > 64) {
+  if (whole_vectors<T>(a)) {
     if (vectors <= 256)
       return launch_rows<T, 1, true, 256>(a, static_cast<int>(round_up(vectors, 32)), stream);
     if (vectors <= 512)
@@ -552,12 +516,10 @@ cudaError_t launch_block_norm(BlockNormArgs a, cudaStream_t stream) {
   const int warps = std::max(8, 1 << log2w);
   const int64_t grid = (a.rows + (warps >> log2w) - 1) / (warps >> log2w);
   constexpr int kWidest = V == 8 ? 512 : 1024; // threads of the widest row
-  const auto kernel = whole        ? per == 1 ? block_norm_kernel<T, 1, 256, false>
-                                              : block_norm_kernel<T, 2, 256, false>
-                      : per == 1   ? block_norm_kernel<T, 1, 256, true>
-                      : per == 2   ? block_norm_kernel<T, 2, 256, true>
-                      : warps <= 8 ? block_norm_kernel<T, 4, 256, true>
-                                   : block_norm_kernel<T, 4, kWidest, true>;
+  const auto kernel = per == 1     ? block_norm_kernel<T, 1, 256>
+                      : per == 2   ? block_norm_kernel<T, 2, 256>
+                      : warps <= 8 ? block_norm_kernel<T, 4, 256>
+                                   : block_norm_kernel<T, 4, kWidest>;
   return launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(warps * 32), 0, stream, a);
 }
 

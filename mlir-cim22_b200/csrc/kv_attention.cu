@@ -738,7 +738,12 @@ Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
     p.tiles = (rows + (p.share ? 127 : 255)) / (p.share ? 128 : 256);
     const int64_t items = p.tiles * v.heads * v.batch;
     p.cluster = 1;
-    p.splits = static_cast<int>(std::max<int64_t>(1, std::min({148 / std::max<int64_t>(1, items), (longest + 1023) / 1024, int64_t{64}})));
+    // Parts of 1,024 keys, or of 512 where there are few rows to join (one
+    // sequence of 4,000 with 256 rows 52 -> 44 us, 1,000 with 2,048 45 -> 62).
+    const int64_t least = rows <= 256 ? 512 : 1024;
+    p.splits = static_cast<int>(std::max<int64_t>(
+        1, std::min({148 / std::max<int64_t>(1, items), (longest + least - 1) / least,
+                     int64_t{64}})));
   }
   const int parts = p.splits / p.cluster;
   p.bytes = parts == 1 ? 0
