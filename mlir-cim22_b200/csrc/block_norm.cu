@@ -71,7 +71,8 @@ __device__ __forceinline__ float row_sum(float v, int warps_log2, float *buffer,
 // Rows off vector boundaries, several to a CTA where they are narrow. A warp's
 // loads and stores take 32 neighbouring elements (lanes that each took their
 // own eight spread every weight load over eight lines: 3,001 x 1,001 f16, 31 us
-// against 19).
+// against 19). Bound by the issue of 2-byte accesses: 20,000 x 1,001 f16 with a
+// gate value an element 98 us, 2.05 TB/s.
 template <typename T, int kPer, int kMax>
 __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a) {
   constexpr int V = kVec<T>;
@@ -115,6 +116,19 @@ __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a)
 #pragma unroll
     for (int p = 0; p < kPer; ++p)
       load(residual, p, res[p]);
+  }
+
+  // A gate row of x's type is on its way while post reduces.
+  T gates[kPer][V];
+  const bool early = a.gate && a.gate_columns != 1 && a.gate_type == a.type;
+  if (early) {
+    const T *gate = static_cast<const T *>(a.gate) + (a.gate_rows ? row / a.gate_rows * a.gate_stride : 0);
+#pragma unroll
+    for (int p = 0; p < kPer; ++p)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (at(p, i) < dim)
+          gates[p][i] = gate[at(p, i)];
   }
 
   auto normalise = [&](const NormArg &n) {
@@ -176,7 +190,13 @@ __global__ void __launch_bounds__(kMax) block_norm_kernel(const BlockNormArgs a)
 #pragma unroll
       for (int p = 0; p < kPer; ++p) {
         float g[V];
-        load_weights(gate, a.gate_type, p, g);
+        if (early) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            g[i] = at(p, i) < dim ? to_f32(gates[p][i]) : 0.0f;
+        } else {
+          load_weights(gate, a.gate_type, p, g);
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i)
           v[p][i] *= gate_fn(g[i], a.gate_act);
@@ -494,22 +514,20 @@ cudaError_t launch_block_norm(BlockNormArgs a, cudaStream_t stream) {
       return launch_rows<T, 1, true, 256>(a, static_cast<int>(round_up(vectors, 32)), stream);
     if (vectors <= 512)
       return launch_rows<T, 2, true, 256>(a, 256, stream);
+    if (vectors <= 1024) // (512 x 4096 f32, two layer norms: 13.9 us; 256 threads 18.4)
+      return launch_rows<T, 2, true, 512>(a, 512, stream);
     if constexpr (V == 8) {
-      if (vectors <= 1024)
-        return launch_rows<T, 2, true, 512>(a, 512, stream);
       return launch_rows<T, 4, false, 512>(a, 512, stream);
     } else {
-      if (vectors <= 1024)
-        return launch_rows<T, 4, true, 256>(a, 256, stream);
       if (vectors <= 2048)
         return launch_rows<T, 4, true, 512>(a, 512, stream);
       return launch_rows<T, 8, false, 512>(a, 512, stream);
     }
   }
-  // Vectors a thread and warps a row: the fewest warps that hold the row.
-  int per = 1, log2w = 0;
-  while (per < 4 && int64_t{32} * per < vectors)
-    per *= 2;
+  // Groups of V elements a thread and warps a row: two groups, and four only
+  // where the row needs them (20,000 x 1,001 f16: 98 us; four 137, one 106).
+  const int per = vectors <= 32 ? 1 : vectors <= (V == 8 ? 1024 : 2048) ? 2 : 4;
+  int log2w = 0;
   while ((int64_t{32} * per << log2w) < vectors)
     ++log2w;
   a.warps_log2 = log2w;
@@ -517,9 +535,9 @@ cudaError_t launch_block_norm(BlockNormArgs a, cudaStream_t stream) {
   const int64_t grid = (a.rows + (warps >> log2w) - 1) / (warps >> log2w);
   constexpr int kWidest = V == 8 ? 512 : 1024; // threads of the widest row
   const auto kernel = per == 1     ? block_norm_kernel<T, 1, 256>
-                      : per == 2   ? block_norm_kernel<T, 2, 256>
-                      : warps <= 8 ? block_norm_kernel<T, 4, 256>
-                                   : block_norm_kernel<T, 4, kWidest>;
+                      : per == 4   ? block_norm_kernel<T, 4, kWidest>
+                      : warps <= 8 ? block_norm_kernel<T, 2, 256>
+                                   : block_norm_kernel<T, 2, kWidest>;
   return launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(warps * 32), 0, stream, a);
 }
 
