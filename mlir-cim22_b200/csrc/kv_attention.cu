@@ -587,9 +587,10 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     cluster_sync(); // no CTA leaves while others read its memory
 }
 
-// Joins the parts of the key axis: a CTA a row and head, its warps take parts
-// in turn.
-template <typename T>
+// Joins the parts of the key axis. kWarps 4: a CTA a row and head, its warps
+// take parts in turn; 1, for up to 8 parts: a warp a row (2 parts of 8,192 rows:
+// 10 us less; one row of 32 parts 2 us more).
+template <typename T, int kWarps>
 __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
   __shared__ float2 warp_ml[4];
   __shared__ float4 warp_o[4][32];
@@ -598,19 +599,19 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
   const KvView &v = a.v;
   const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const KvSequence s = kv_sequence(v, b);
-  const int64_t f = blockIdx.x;
+  const int64_t f = kWarps == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + warp : blockIdx.x;
   if (!s.ok || f >= static_cast<int64_t>(s.n) * a.q_heads)
     return;
   const int64_t at = s.row0 * a.q_heads + f, step = v.rows * a.q_heads;
   float m = kNone, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int kAhead = 4;
   const int parts = a.splits / a.cluster;
-  for (int x0 = warp; x0 < parts; x0 += 4 * kAhead) {
+  for (int x0 = kWarps == 1 ? 0 : warp; x0 < parts; x0 += kWarps * kAhead) {
     float2 ml[kAhead];
     float4 p[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int64_t x = x0 + 4 * u;
+      const int64_t x = x0 + kWarps * u;
       ml[u] = make_float2(kNone, 0.0f);
       p[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (x < parts) {
@@ -639,35 +640,39 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
       acc[3] = fmaf(p[u].w, share, acc[3]);
     }
   }
-  if (lane == 0)
-    warp_ml[warp] = make_float2(m, sum);
-  warp_o[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-  __syncthreads();
-  if (warp > 0)
-    return;
-  float top = kNone;
+  float top = m;
+  if constexpr (kWarps > 1) {
+    if (lane == 0)
+      warp_ml[warp] = make_float2(m, sum);
+    warp_o[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    if (warp > 0)
+      return;
+    top = kNone;
 #pragma unroll
-  for (int x = 0; x < 4; ++x)
-    top = fmaxf(top, warp_ml[x].x);
-  sum = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+    for (int x = 0; x < 4; ++x)
+      top = fmaxf(top, warp_ml[x].x);
+    sum = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const float2 ml = warp_ml[x];
-    const float4 p = warp_o[x][lane];
-    const float share = exp2_approx(ml.x - top);
-    sum = fmaf(ml.y, share, sum);
-    acc[0] = fmaf(p.x, share, acc[0]);
-    acc[1] = fmaf(p.y, share, acc[1]);
-    acc[2] = fmaf(p.z, share, acc[2]);
-    acc[3] = fmaf(p.w, share, acc[3]);
+    for (int x = 0; x < 4; ++x) {
+      const float2 ml = warp_ml[x];
+      const float4 p = warp_o[x][lane];
+      const float share = exp2_approx(ml.x - top);
+      sum = fmaf(ml.y, share, sum);
+      acc[0] = fmaf(p.x, share, acc[0]);
+      acc[1] = fmaf(p.y, share, acc[1]);
+      acc[2] = fmaf(p.z, share, acc[2]);
+      acc[3] = fmaf(p.w, share, acc[3]);
+    }
   }
   const bool some = top > kNone || sum != sum;
   const float share = some ? 1.0f / sum : 0.0f;
   if (4 * lane < v.dim) {
+    const float o[4] = {acc[0] * share, acc[1] * share, acc[2] * share, acc[3] * share};
     T *out = static_cast<T *>(a.out) + at * v.dim + 4 * lane;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      out[j] = from_f32<T>(acc[j] * share);
+      out[j] = from_f32<T>(o[j]);
   }
   if (a.lse && lane == 0)
     a.lse[at] = some ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
@@ -694,6 +699,36 @@ void decode_parts(const KvView &v, int64_t tiles, int64_t longest, int resident,
   else
     cluster = items * splits <= 148 ? 8 : 2;
   splits = splits / cluster * cluster;
+}
+
+// The same for prompts, where a CTA fills an SM: the number that takes the least
+// time, counted in tiles of 128 keys (2.8 us, 2.1 with head_dim 64). A round of
+// CTAs lasts as long as its tiles and some five more for filling and emptying;
+// joining takes two and the parts' way through memory. (3 sequences of 6,000,
+// window 4,096, 700 new tokens, 24 heads of 64: 216 CTAs 223 us, halved 199; one
+// of 1,000, 8 heads of 128: 49 us, in 4 parts 39.)
+int prompt_parts(const KvView &v, int64_t tiles, int64_t tile_rows, int64_t group, int64_t longest,
+                 int64_t window) {
+  const int64_t items =
+      v.heads * std::min<int64_t>(tiles * v.batch, v.rows * group / tile_rows + v.batch);
+  const int64_t span =
+      ((window ? std::min(longest, window + tile_rows / group) : longest) + 127) / 128;
+  const double join = static_cast<double>(items * tile_rows * v.dim) * 8.0 / 12.5e6;
+  int64_t best = 1;
+  double least = 0.0;
+  for (int64_t parts = 1; parts <= std::min<int64_t>(64, span); ++parts) {
+    const int64_t rounds = (items * parts + 147) / 148;
+    if (parts > 1 && rounds > 6)
+      break;
+    const double cost =
+        static_cast<double>(rounds) * static_cast<double>((span + parts - 1) / parts + 5) +
+        (parts > 1 ? 2.0 + join * static_cast<double>(parts) : 0.0);
+    if (parts == 1 || cost < (best == 1 ? 0.96 : 1.0) * least) {
+      least = cost;
+      best = parts;
+    }
+  }
+  return static_cast<int>(best);
 }
 
 struct Plan {
@@ -736,14 +771,8 @@ Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
     decode_parts(v, p.tiles, longest, resident, p.splits, p.cluster);
   } else {
     p.tiles = (rows + (p.share ? 127 : 255)) / (p.share ? 128 : 256);
-    const int64_t items = p.tiles * v.heads * v.batch;
     p.cluster = 1;
-    // Parts of 1,024 keys, or of 512 where there are few rows to join (one
-    // sequence of 4,000 with 256 rows 52 -> 44 us, 1,000 with 2,048 45 -> 62).
-    const int64_t least = rows <= 256 ? 512 : 1024;
-    p.splits = static_cast<int>(std::max<int64_t>(
-        1, std::min({148 / std::max<int64_t>(1, items), (longest + least - 1) / least,
-                     int64_t{64}})));
+    p.splits = prompt_parts(v, p.tiles, p.share ? 128 : 256, group, longest, t.window);
   }
   const int parts = p.splits / p.cluster;
   p.bytes = parts == 1 ? 0
@@ -822,8 +851,11 @@ cudaError_t launch_attend(const KvAttendArgs &a, int type, const Plan &plan, cud
                   : launch_decode<T, kParts, 2>(a, plan.tiles, stream);
   if (e == cudaSuccess && a.splits > a.cluster) {
     const int64_t rows = std::min<int64_t>(a.v.most, a.v.rows) * a.q_heads;
-    e = launch_pdl(kv_join_kernel<T>, dim3(static_cast<unsigned>(rows), 1, a.v.batch), dim3(128),
-                   0, stream, a);
+    e = a.splits / a.cluster <= 8
+            ? launch_pdl(kv_join_kernel<T, 1>, dim3(static_cast<unsigned>((rows + 3) / 4), 1, a.v.batch),
+                         dim3(128), 0, stream, a)
+            : launch_pdl(kv_join_kernel<T, 4>, dim3(static_cast<unsigned>(rows), 1, a.v.batch),
+                         dim3(128), 0, stream, a);
   }
   return e;
 }
