@@ -7,6 +7,7 @@ kernel of libcim22_cuda.so. Tensors must be contiguous CUDA tensors.
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -448,10 +449,20 @@ _GATE_ACT = {None: abi.GATE_NONE, "none": abi.GATE_NONE, "sigmoid": abi.GATE_SIG
              "tanh": abi.GATE_TANH}
 
 
+# abi.BlockNorm and behind it its two abi.Norm, packed in one step: filling the
+# ctypes structures took 2 us more, a sixth of a small call.
+_BLOCK_NORM = struct.Struct("@iqqqqqqfqqqqiiqqqqqqifqqi4xifqqi4x")
+_BlockNormBytes = ctypes.c_char * _BLOCK_NORM.size
+_NORM_AT = ctypes.sizeof(abi.BlockNorm), ctypes.sizeof(abi.BlockNorm) + ctypes.sizeof(abi.Norm)
+assert _BLOCK_NORM.size == _NORM_AT[1] + ctypes.sizeof(abi.Norm)
+_NO_NORM = 0, 0.0, 0, 0, 0
+
+
 def _as_rows(t: torch.Tensor, like: torch.Tensor, name: str) -> int:
     """The row stride of a tensor taken as rows of its last axis: any 2-D tensor
     whose last axis is contiguous, or a contiguous one."""
-    if t.get_device() != like.get_device() or t.dtype != like.dtype or t.shape != like.shape:
+    if t is not like and (t.dtype != like.dtype or t.get_device() != like.get_device()
+                          or t.shape != like.shape):
         raise TypeError(f"{name} must have x's shape, type and device")
     if t.is_contiguous():
         return t.shape[-1]
@@ -460,40 +471,47 @@ def _as_rows(t: torch.Tensor, like: torch.Tensor, name: str) -> int:
     raise TypeError(f"{name} must be contiguous, or rows with a contiguous last axis")
 
 
-def _norm_arg(norm: Norm, x: torch.Tensor, dim: int, name: str):
-    if norm.kind not in _NORM_KIND:
+def _norm_arg(norm: Norm, x: torch.Tensor, dim: int, name: str) -> tuple:
+    """abi.Norm's fields."""
+    kind = _NORM_KIND.get(norm.kind)
+    if kind is None:
         raise ValueError(f"{name} norm must be \"rms\" or \"layer\"")
     weight, bias = norm.weight, norm.bias
     dtype = x.dtype
-    for field, t in (("weight", weight), ("bias", bias)):
+    for t in (weight, bias):
         if t is None:
             continue
-        if t.get_device() != x.get_device() or t.dtype not in (torch.float32, x.dtype) \
-                or t.dim() != 1 or t.shape[0] != dim or not t.is_contiguous():
-            raise TypeError(f"{name} {field} must be a contiguous [dim] tensor on x's device, "
-                            "f32 or of x's type")
+        if t.dtype not in (torch.float32, x.dtype) or t.get_device() != x.get_device() \
+                or t.dim() != 1 or t.numel() != dim or not t.is_contiguous():
+            raise TypeError(f"{name} weight and bias must be contiguous [dim] tensors on x's "
+                            "device, f32 or of x's type")
         dtype = t.dtype
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"{name} weight and bias must have one type")
-    return ctypes.pointer(abi.Norm(_NORM_KIND[norm.kind], norm.eps,
-                                   None if weight is None else weight.data_ptr(),
-                                   None if bias is None else bias.data_ptr(),
-                                   FLOAT_TYPES[dtype]))
+    return (kind, norm.eps, 0 if weight is None else weight.data_ptr(),
+            0 if bias is None else bias.data_ptr(), FLOAT_TYPES[dtype])
 
 
-def _gate_rows(gate: torch.Tensor, x: torch.Tensor, rows: int, dim: int) -> int:
-    """Consecutive rows that share a gate row; 0 for a single gate row."""
+def _gate_rows(gate: torch.Tensor, x: torch.Tensor, rows: int, dim: int) -> tuple[int, int]:
+    """Consecutive rows that share a gate row (0 for a single gate row), and the
+    gate's columns."""
     if gate.get_device() != x.get_device() or gate.dtype not in (torch.float32, x.dtype) \
             or not gate.is_contiguous():
         raise TypeError("gate must be a contiguous tensor on x's device, f32 or of x's type")
-    if gate.dim() == 1 and gate.shape[0] == dim:
-        return 0
+    if gate.dim() == 1 and gate.numel() == dim:
+        return 0, dim
     if gate.dim() >= 2 and gate.shape[-1] in (1, dim):
-        lead = gate.numel() // gate.shape[-1]
+        columns = gate.shape[-1]
+        lead = gate.numel() // columns
         if rows == 0 or lead and rows % lead == 0:
-            return rows // lead if lead > 1 else 0
+            return rows // lead if lead > 1 else 0, columns
     raise ValueError("gate must be [dim], or [groups, dim] or [groups, 1] with groups dividing "
                      "the rows")
+
+
+def _empty_rows(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else \
+        torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def block_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
@@ -524,29 +542,32 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     rows = x.numel() // dim
     if gate_activation not in _GATE_ACT:
         raise ValueError("gate activation must be None, sigmoid or tanh")
-    gate_rows = 0 if gate is None else _gate_rows(gate, x, rows, dim)
+    gate_rows = gate_columns = 0
+    if gate is not None:
+        gate_rows, gate_columns = _gate_rows(gate, x, rows, dim)
     h = y = None
     if out is not None or residual is not None or post is not None or gate is not None:
-        h = torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else out
+        h = _empty_rows(x) if out is None else out
     if pre is not None:
-        y = torch.empty_like(x, memory_format=torch.contiguous_format) if normed is None \
-            else normed
+        y = _empty_rows(x) if normed is None else normed
     elif normed is not None:
         raise ValueError("normed is an output of pre: it needs one")
     if h is None and y is None:
         raise ValueError("nothing to compute: give a residual, post, gate or pre")
-    call = abi.BlockNorm(
-        FLOAT_TYPES[x.dtype], rows, dim, x.data_ptr(), _as_rows(x, x, "x"),
-        None if residual is None else residual.data_ptr(),
+    call = _BlockNormBytes()
+    at = ctypes.addressof(call)
+    _BLOCK_NORM.pack_into(
+        call, 0, FLOAT_TYPES[x.dtype], rows, dim, x.data_ptr(), _as_rows(x, x, "x"),
+        0 if residual is None else residual.data_ptr(),
         0 if residual is None else _as_rows(residual, x, "residual"), residual_scale,
-        None if gate is None else gate.data_ptr(), 0 if gate is None else gate.shape[-1],
-        gate_rows, 0 if gate is None else gate.shape[-1],
+        0 if gate is None else gate.data_ptr(), gate_columns, gate_rows, gate_columns,
         0 if gate is None else FLOAT_TYPES[gate.dtype], _GATE_ACT[gate_activation],
-        None if post is None else _norm_arg(post, x, dim, "post"),
-        None if pre is None else _norm_arg(pre, x, dim, "pre"),
-        None if h is None else h.data_ptr(), dim if out is None else _as_rows(out, x, "out"),
-        None if y is None else y.data_ptr(), dim if normed is None else _as_rows(normed, x, "normed"))
-    launch("block_norm", x.get_device(), lib().cim22_cuda_block_norm, ctypes.byref(call))
+        0 if post is None else at + _NORM_AT[0], 0 if pre is None else at + _NORM_AT[1],
+        0 if h is None else h.data_ptr(), dim if out is None else _as_rows(out, x, "out"),
+        0 if y is None else y.data_ptr(), dim if normed is None else _as_rows(normed, x, "normed"),
+        *(_NO_NORM if post is None else _norm_arg(post, x, dim, "post")),
+        *(_NO_NORM if pre is None else _norm_arg(pre, x, dim, "pre")))
+    launch("block_norm", x.get_device(), lib().cim22_cuda_block_norm, call)
     return h, y
 
 

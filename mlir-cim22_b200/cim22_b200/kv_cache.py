@@ -25,14 +25,22 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
 from . import abi
 from .cim_ops import FLOAT_TYPES, StatusWord, Workspace, launch
-from .native import lib
+from .native import CudaError, lib
 
 BLOCKS = (16, 32, 64, 128)
+
+# abi.KvSequences and abi.KvAttention: packing them takes half the time of
+# filling the ctypes structures.
+_SEQUENCES = struct.Struct("@iqqiqqqi4x")
+_ATTENTION = struct.Struct("@iiqqqqqfiiq")
+assert _SEQUENCES.size == ctypes.sizeof(abi.KvSequences)
+assert _ATTENTION.size == ctypes.sizeof(abi.KvAttention)
 
 
 class Int8KVCache:
@@ -80,27 +88,30 @@ class Int8KVCache:
         self.codes, self.scales = codes, scales
         self.pages, self.kv_heads, _, self.block, self.head_dim = codes.shape
         self.device, self._index = codes.device, codes.get_device()
-        self._view = abi.KvCache(codes=codes.data_ptr(), scales=scales.data_ptr(),
-                                 pages=self.pages, kv_heads=self.kv_heads, block=self.block,
-                                 head_dim=self.head_dim)
+        self._view = bytes(abi.KvCache(codes=codes.data_ptr(), scales=scales.data_ptr(),
+                                       pages=self.pages, kv_heads=self.kv_heads,
+                                       block=self.block, head_dim=self.head_dim))
 
     # ------------------------------------------------------------- descriptions
 
     def _int32(self, t: torch.Tensor, count: int, name: str) -> None:
-        if t.get_device() != self._index or t.dtype != torch.int32 or t.dim() != 1 \
-                or t.shape[0] != count or not t.is_contiguous():
+        if t.dtype != torch.int32 or t.get_device() != self._index or t.dim() != 1 \
+                or t.numel() != count or not t.is_contiguous():
             raise TypeError(f"{name} must be a contiguous int32 tensor [{count}] on the cache's "
                             "device")
 
     def _sequences(self, table: torch.Tensor, lengths: torch.Tensor,
-                   starts: torch.Tensor | None, rows: int, most: int | None) -> abi.KvSequences:
+                   starts: torch.Tensor | None, rows: int, most: int | None) -> tuple:
+        """abi.KvSequences' fields."""
         if table.get_device() != self._index or table.dtype != torch.int32 or table.dim() != 2:
             raise TypeError("table must be an int32 tensor [batch, pages a sequence] on the "
                             "cache's device")
         batch, width = table.shape
-        if not table.is_contiguous() and (width > 1 and table.stride(1) != 1
-                                          or batch > 1 and table.stride(0) < width):
-            raise TypeError("table rows must be contiguous and must not overlap")
+        stride = width
+        if not table.is_contiguous():
+            stride = table.stride(0)
+            if width > 1 and table.stride(1) != 1 or batch > 1 and stride < width:
+                raise TypeError("table rows must be contiguous and must not overlap")
         self._int32(lengths, batch, "lengths")
         if batch > 65535:
             raise ValueError("at most 65535 sequences a call")
@@ -113,19 +124,23 @@ class Int8KVCache:
             most = rows if most is None else most
             if not 0 <= most <= 0x7fffffff:
                 raise ValueError("most out of range")
-        return abi.KvSequences(batch, table.data_ptr(), table.stride(0), width,
-                               lengths.data_ptr(), None if starts is None else starts.data_ptr(),
-                               rows, most)
+        return (batch, table.data_ptr(), stride, width, lengths.data_ptr(),
+                0 if starts is None else starts.data_ptr(), rows, most)
 
-    def _rows(self, t: torch.Tensor, heads: int, name: str) -> None:
-        if t.get_device() != self._index or t.dtype not in FLOAT_TYPES or t.dim() != 3:
+    def _rows(self, t: torch.Tensor, heads: int, name: str) -> tuple[int, int]:
+        """Checks packed rows; returns their and their heads' strides."""
+        if t.dtype not in FLOAT_TYPES or t.get_device() != self._index or t.dim() != 3:
             raise TypeError(f"{name} must be an f32, bf16 or f16 tensor [rows, heads, head_dim] "
                             "on the cache's device")
         _, has, dim = t.shape
         if has != heads or dim != self.head_dim:
             raise ValueError(f"{name} must have {heads} heads of {self.head_dim}")
-        if t.stride(2) != 1:
+        if t.is_contiguous():
+            return has * dim, dim
+        rows, of_heads, last = t.stride()
+        if last != 1:
             raise TypeError(f"{name}'s last axis must be contiguous")
+        return rows, of_heads
 
     # -------------------------------------------------------------------- calls
 
@@ -141,16 +156,16 @@ class Int8KVCache:
         scale grew. Two sequences of one call must not write the same page.
         NaN and infinities are stored as 0 and +-127 and reported through the
         status."""
-        self._rows(k, self.kv_heads, "k")
-        self._rows(v, self.kv_heads, "v")
-        if k.shape != v.shape or k.dtype != v.dtype:
+        k_rows, k_heads = self._rows(k, self.kv_heads, "k")
+        v_rows, v_heads = self._rows(v, self.kv_heads, "v")
+        rows = k.shape[0]
+        if v.shape[0] != rows or k.dtype != v.dtype:
             raise ValueError("k and v must have one shape and type")
-        seqs = self._sequences(table, lengths, starts, k.shape[0], most)
+        seqs = _SEQUENCES.pack(*self._sequences(table, lengths, starts, rows, most))
         own_status = status is None
         status = status or StatusWord(self.device)
-        launch("cim22_cuda_kv_write", self._index, lib().cim22_cuda_kv_write,
-               ctypes.byref(self._view), ctypes.byref(seqs), FLOAT_TYPES[k.dtype], k.data_ptr(),
-               k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        launch("cim22_cuda_kv_write", self._index, lib().cim22_cuda_kv_write, self._view, seqs,
+               FLOAT_TYPES[k.dtype], k.data_ptr(), k_rows, k_heads, v.data_ptr(), v_rows, v_heads,
                status.tensor.data_ptr())
         if own_status:
             status.raise_if_set()
@@ -177,14 +192,14 @@ class Int8KVCache:
             self._rows(t, self.kv_heads, name)
             if not t.is_contiguous():
                 raise TypeError(f"{name} must be contiguous")
-        if k.shape != v.shape or k.dtype != v.dtype:
+        rows = k.shape[0]
+        if v.shape[0] != rows or k.dtype != v.dtype:
             raise ValueError("k and v must have one shape and type")
-        seqs = self._sequences(table, lengths, starts, k.shape[0], most)
+        seqs = _SEQUENCES.pack(*self._sequences(table, lengths, starts, rows, most))
         own_status = status is None
         status = status or StatusWord(self.device)
-        launch("cim22_cuda_kv_read", self._index, lib().cim22_cuda_kv_read,
-               ctypes.byref(self._view), ctypes.byref(seqs), FLOAT_TYPES[k.dtype], k.data_ptr(),
-               v.data_ptr(), status.tensor.data_ptr())
+        launch("cim22_cuda_kv_read", self._index, lib().cim22_cuda_kv_read, self._view, seqs,
+               FLOAT_TYPES[k.dtype], k.data_ptr(), v.data_ptr(), status.tensor.data_ptr())
         if own_status:
             status.raise_if_set()
         return k, v
@@ -205,43 +220,53 @@ class Int8KVCache:
         longest: the longest of lengths (default: what the table can hold)."""
         if q.dim() != 3:
             raise TypeError("q must be [rows, q_heads, head_dim]")
-        heads = q.shape[1]
-        self._rows(q, heads, "q")
+        rows, heads, _ = q.shape
+        row_stride, head_stride = self._rows(q, heads, "q")
         if heads < 1 or heads % self.kv_heads:
             raise ValueError("q_heads must be a multiple of kv_heads")
-        seqs = self._sequences(table, lengths, starts, q.shape[0], most)
+        seqs = self._sequences(table, lengths, starts, rows, most)
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
         if not math.isfinite(scale):
             raise ValueError("scale must be finite")
         if not 0 <= window <= 0x7fffffff:
             raise ValueError("window out of range")
-        held = seqs.table_width * self.block
-        longest = held if longest is None else longest
-        if longest < 0:
-            raise ValueError("longest must not be negative")
+        if longest is None:
+            longest = table.shape[1] * self.block
+        elif not 0 <= longest <= 0x7fffffffffffffff:
+            raise ValueError("longest out of range")
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = torch.empty_like(q) if q.is_contiguous() else \
+                torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device \
                 or not out.is_contiguous():
             raise TypeError("out must be contiguous, of q's shape and type")
         elif out.data_ptr() == q.data_ptr() and q.numel():
             raise ValueError("out must not be q")
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) \
+        lse = torch.empty(rows, heads, dtype=torch.float32, device=self.device) \
             if return_lse else None
-        call = abi.KvAttention(FLOAT_TYPES[q.dtype], heads, q.data_ptr(), q.stride(0),
-                               q.stride(1), out.data_ptr(),
-                               None if lse is None else lse.data_ptr(), scale, int(causal),
-                               window, longest)
+        call = _ATTENTION.pack(FLOAT_TYPES[q.dtype], heads, q.data_ptr(), row_stride, head_stride,
+                               out.data_ptr(), 0 if lse is None else lse.data_ptr(), scale,
+                               bool(causal), window, longest)
+        seqs = _SEQUENCES.pack(*seqs)
         own_status = status is None
         status = status or StatusWord(self.device)
-        cache, seqs, call = ctypes.byref(self._view), ctypes.byref(seqs), ctypes.byref(call)
-        ws = None
-        nbytes = lib().cim22_cuda_kv_attend_workspace(cache, seqs, call)
-        if nbytes:
-            ws = (workspace or Workspace(self.device)).get(nbytes)
-        launch("cim22_cuda_kv_attend", self._index, lib().cim22_cuda_kv_attend, cache, seqs, call,
-               None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
-               status.tensor.data_ptr())
+        buffer = None if workspace is None else workspace.buffer
+        if buffer is not None and buffer.get_device() != self._index:
+            raise ValueError("workspace must be on the cache's device")
+
+        def attend(at: int, nbytes: int) -> None:
+            launch("cim22_cuda_kv_attend", self._index, lib().cim22_cuda_kv_attend, self._view,
+                   seqs, call, at, nbytes, status.tensor.data_ptr())
+
+        have = 0 if buffer is None else buffer.numel()
+        try:
+            attend(buffer.data_ptr() if have else 0, have)
+        except CudaError: # nothing was launched; most calls need no more than is there
+            need = lib().cim22_cuda_kv_attend_workspace(self._view, seqs, call)
+            if need <= have:
+                raise
+            buffer = (workspace or Workspace(self.device)).get(need)
+            attend(buffer.data_ptr(), buffer.numel())
         if own_status:
             status.raise_if_set()
         return (out, lse) if return_lse else out

@@ -562,6 +562,8 @@ def test_results_repeat_and_do_not_hang_on_streams():
     lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st, out=q.half()),
     lambda s, q, k, t, n, st: s.cache.attend(q.cpu(), t, n, st),
     lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st, out=q),
+    lambda s, q, k, t, n, st: s.cache.attend(q, t, n, st,
+                                             workspace=Workspace(torch.device("cpu"))),
     lambda s, q, k, t, n, st: s.cache.write(k, k.half(), t, n, st),
     lambda s, q, k, t, n, st: s.cache.write(k, k[:8], t, n, st),
     lambda s, q, k, t, n, st: s.cache.write(q, q, t, n, st),
