@@ -1,7 +1,9 @@
 // kv_attention.cu - attention of few query rows over the 8-bit cache, and the
 // dispatch between it and the tensor-memory kernel for prompts.
 //
-// Decode reads every cached code once: bound by HBM. The products are taken
+// Decode reads every cached code once: bound by HBM (64 sequences of 286,000
+// tokens in all, 8 kv heads of 128, bf16: 110 us, 5.3 TB/s; one of 200,000, 4 kv
+// heads, 47 us, 4.4 TB/s with its filling and joining). The products are taken
 // transposed, S^T = K Q^T and O^T = V^T P^T (m16n8k16), so that 16 tokens or
 // 16 elements of the head fill the 16 rows and a tile needs only 8 query rows
 // (query tokens x the heads that share a kv head). A work item is a 16-token
@@ -746,11 +748,11 @@ struct Plan {
 // (decode | prompt, head_dim 128, bf16, 8 kv heads, L2 flushed: 32 sequences of
 // 4,096 with 32 rows 145 | 197 us, 48 rows 195 | 199, 64 rows 244 | 197; one of
 // 32,768 46 | 63, 58 | 65, 75 | 65). So do more rows where all of its tiles of 16
-// have a place at once and come to kDecodeWork keys (one sequence of 2,000 with
-// 256 rows 32 | 54 us; 4 of 1,000 with 128 rows 33 | 39; twice the work, 4 of
-// 2,000 with 128 rows, 49 | 48; more tiles than places, 16 of 300 with 64 rows,
-// 37 | 27): the prompt kernel starts with some 25 us of filling and joining.
-constexpr int64_t kDecodeRows = 32, kDecodeWork = 1 << 18;
+// have a place at once and come to kDecodeWork keys: the prompt kernel takes some
+// 15 us to fill and empty (one sequence of 1,000 with 256 rows 25 | 33 us, 4 with
+// 64 rows 27 | 28; twice that work, one of 4,000 with 128 rows 36 | 30; more tiles
+// than places, 16 of 300 with 64 rows, 37 | 27).
+constexpr int64_t kDecodeRows = 32, kDecodeWork = 1 << 17;
 
 Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   Plan p{};

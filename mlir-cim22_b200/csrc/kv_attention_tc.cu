@@ -5,7 +5,9 @@
 // 128 rows x 128 keys (head_dim 128) take 2 x 512 cycles of f16 products, whose
 // operands fill shared memory's 128 bytes a cycle, and 1,024 of the
 // special-function units. A CTA therefore runs two streams of 128 query rows,
-// so that one's products cover the other's softmax:
+// so that one's products cover the other's softmax (a prompt of 8,192, 32 heads
+// of 128 on 8, bf16: 0.64 ms, 860 TFLOP/s; 3 chunks of 1,024 in a window of
+// 4,096, 24 heads of 64: 472):
 //   warps 0-7, 8-15 softmax of stream 0 and 1: two threads a row, one for each
 //                   64 keys of a tile, scores from TMEM, probabilities back over
 //                   them as the f16 A operand (one thread a row left too few
@@ -18,7 +20,8 @@
 // (Two buffers of 64 keys a stream, which let products run ahead, were slower:
 // a product of 64 keys still reads all of its query tile. So were all 128
 // scores of a row in registers, with or without more registers for these
-// warps.)
+// warps, and warps of their own for keys and for values: 0.66 ms. The queries
+// read by the softmax warps alone, while the converters start, took 0.71.)
 // Query rows are the tokens of a sequence times the heads that share a kv
 // head, so a tile of keys is converted once for up to 256 rows. The codes'
 // scales stay out of the products: a group of 16 tokens lies in one page, and
@@ -40,7 +43,9 @@ constexpr int kPanel = 128 * 128;    // bytes: 128 rows of 64 f16
 // The products' accumulation does not round to nearest: f32 outputs lost half
 // their accuracy to it over 1,500 keys (1.25e-6 relative; 4.8e-6 over 8,192). With
 // two parts a stream's sum is therefore taken out of the accumulators every
-// kFlush tiles and added to what it carries in memory, rounding to nearest.
+// kFlush tiles and added to what it carries in memory, rounding to nearest
+// (0.67e-6 over 1,800 keys; 5 prompts of up to 1,500, 16 heads of 80 on 4: 129 ->
+// 167 us).
 constexpr int kFlush = 2;
 constexpr uint64_t kWaitLimit = 2000000000ull; // ns
 
