@@ -15,7 +15,8 @@ attention of its queries. Lengths, starts and table live on the device, so a
 step can be captured into a CUDA graph and replayed with new contents.
 ``most`` bounds a sequence's rows in the call and ``longest`` its length; both
 are host numbers that size the launch (a graph's ``most`` has to cover every
-replay; any ``longest`` gives the right results). Under capture, and to avoid a
+replay; any ``longest`` gives the right results). By default they are all rows and
+what the table can hold, which starts many idle blocks for a batch of prompts. Under capture, and to avoid a
 synchronization in every call, pass ``status``: without it each call makes a
 status word of its own and reads it back. A ``workspace`` belongs to calls that
 run one after another, graphs among them.
@@ -45,7 +46,8 @@ assert _ATTENTION.size == ctypes.sizeof(abi.KvAttention)
 
 class Int8KVCache:
     """Keys and values of one layer in 8 bits, with a scale for each block of
-    tokens and head."""
+    tokens and head. ``codes`` and ``scales`` are its tensors, to copy pages from
+    and into; binding other tensors to the names has no effect on the calls."""
 
     def __init__(self, pages: int, kv_heads: int, head_dim: int, block: int = 64, *,
                  device: int | torch.device = 0) -> None:
@@ -215,9 +217,11 @@ class Int8KVCache:
         a sequence's n sits at position lengths[b] - n + i. causal: it sees
         positions up to its own; window > 0: only the last window of them. A
         query that sees nothing gives zeros. scale defaults to
-        head_dim ** -0.5; out must not overlap q. Returns out [rows, q_heads, head_dim] of q's type, or
-        (out, lse) with the f32 logarithm of each row's sum of exponentials.
-        longest: the longest of lengths (default: what the table can hold)."""
+        head_dim ** -0.5; out must not overlap q. Returns out [rows, q_heads,
+        head_dim] of q's type, or (out, lse) with the f32 logarithm of each row's
+        sum of exponentials. A query row that holds NaN or an infinity gives NaN
+        wherever it sees a key. longest: the longest of lengths (default: what the
+        table can hold)."""
         if q.dim() != 3:
             raise TypeError("q must be [rows, q_heads, head_dim]")
         rows, heads, _ = q.shape

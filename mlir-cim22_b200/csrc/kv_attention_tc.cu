@@ -44,8 +44,8 @@ constexpr int kPanel = 128 * 128;    // bytes: 128 rows of 64 f16
 // their accuracy to it over 1,500 keys (1.25e-6 relative; 4.8e-6 over 8,192). With
 // two parts a stream's sum is therefore taken out of the accumulators every
 // kFlush tiles and added to what it carries in memory, rounding to nearest
-// (0.67e-6 over 1,800 keys; 5 prompts of up to 1,500, 16 heads of 80 on 4: 129 ->
-// 167 us).
+// (0.7e-6 over 1,800 keys; 5 prompts of up to 1,500, 16 heads of 80 on 4: 129 ->
+// 161 us).
 constexpr int kFlush = 2;
 constexpr uint64_t kWaitLimit = 2000000000ull; // ns
 
@@ -523,22 +523,40 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       asm volatile("bar.sync %0, 64;" ::"r"(2 + st * 4 + (warp & 3)) : "memory");
       top = fmaxf(top, sm.tops[n & 1][st][half ^ 1][row]);
       if (kParts == 2 && carry && n > 0 && n % kFlush == 0) {
+        // What is carried is read kAhead steps of 8 elements before it is used (a
+        // prompt of 4,096, 32 heads of 128: 477 us; 544 read in place).
+        constexpr int kSteps = kD / 16, kAhead = 2;
+        const int d0 = half * (kD / 2), end = min(d0 + kD / 2, v.dim);
+        float old[kAhead][8];
+        auto fetch = [&](int step) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float &to = old[step % kAhead][i];
+            to = 0.0f;
+            if (live && n > kFlush && d0 + 8 * step < end)
+              to = carry[(d0 + 8 * step + i) * plane];
+          }
+        };
+#pragma unroll
+        for (int step = 0; step < kAhead; ++step)
+          fetch(step);
         ok = bar_wait(&sm.o_full[st], (n - 1) & 1, failed) && ok;
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-        for (int d = half * (kD / 2); d < (half + 1) * (kD / 2); d += 8) {
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+          const int d = d0 + 8 * step;
+          if (d >= end)
+            break;
           uint32_t y[8];
           tmem_load8(o_at + d, y);
           if (live) {
-            float old[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              old[i] = n > kFlush ? carry[(d + i) * plane] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              carry[(d + i) * plane] = fmaf(old[i], carried, __uint_as_float(y[i]));
+              carry[(d + i) * plane] = fmaf(old[step % kAhead][i], carried, __uint_as_float(y[i]));
           }
+          if (step + kAhead < kSteps)
+            fetch(step + kAhead);
         }
         carried = 1.0f;
       }
