@@ -7,10 +7,12 @@
 // the scale and stores the codes. The block's earlier codes are loaded only
 // when the scale grew.
 //
-// Bound by HBM for prompts (values in, one byte a value out: 57,560 tokens of 8
-// heads of 128 in bf16 81 us to write, 4.4 TB/s, and 70 to read back, 5.0) and by
-// latency for single tokens (length, page, scale and value loads in a row: 64
-// sequences, 2 us each way).
+// Bound for prompts by HBM (values in, one byte a value out) and as much by the
+// issue of instructions (88% and 84% of the slots): 57,560 tokens of 8 heads of
+// 128 in bf16 81 us to write, 4.4 TB/s, and 70 to read back, 5.1 (128 threads a
+// block, for fewer warps to set up, 136 and 74). Single tokens are bound by
+// latency (length, page, scale and value loads in a row: 64 sequences, 8 heads,
+// 3.4 us).
 #include "kv_util.cuh"
 
 #include <algorithm>
@@ -241,6 +243,9 @@ __global__ void __launch_bounds__(kThreads)
   const float scale = v.scales[(static_cast<int64_t>(page) * v.heads + head) * 2 + side];
   const int8_t *codes = kv_codes(v, page, head, side) + lo * v.dim;
   const int chunks = (hi - lo) * parts.d;
+  const int64_t stride = static_cast<int64_t>(v.heads) * v.dim;
+  T *to = out + (row + lo) * stride + head * v.dim;
+  const bool aligned = (reinterpret_cast<uintptr_t>(to) & 15) == 0; // rows are whole vectors
   constexpr int kUnroll = 4;
   for (int c0 = threadIdx.x; c0 < chunks; c0 += kUnroll * kThreads) {
     union {
@@ -265,7 +270,11 @@ __global__ void __launch_bounds__(kThreads)
           y[j] = __fmul_rn(y[j], scale);
         Pack<T> o;
         pack(y, o);
-        store_pack(out + ((row + lo + i) * v.heads + head) * v.dim, (c - i * parts.d) * V, v.dim, o);
+        T *at = to + i * stride + (c - i * parts.d) * V;
+        if (aligned)
+          *reinterpret_cast<uint4 *>(at) = o.raw;
+        else
+          store_pack(at, 0, V, o);
       }
     }
   }
