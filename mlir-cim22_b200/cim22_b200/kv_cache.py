@@ -47,7 +47,8 @@ assert _ATTENTION.size == ctypes.sizeof(abi.KvAttention)
 class Int8KVCache:
     """Keys and values of one layer in 8 bits, with a scale for each block of
     tokens and head. ``codes`` and ``scales`` are its tensors, to copy pages from
-    and into; binding other tensors to the names has no effect on the calls."""
+    and into; the names cannot be bound to others. A deep or unpickled copy is
+    a cache over tensors of its own, a shallow one over the same."""
 
     def __init__(self, pages: int, kv_heads: int, head_dim: int, block: int = 64, *,
                  device: int | torch.device = 0) -> None:
@@ -87,12 +88,26 @@ class Int8KVCache:
             raise ValueError("pages or kv_heads out of range")
 
     def _init(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
-        self.codes, self.scales = codes, scales
+        # The calls take addresses. These aliases, which nobody else sees, keep
+        # the memory there whatever is done to the tensors that are handed out.
+        self._memory = codes.detach(), scales.detach()
+        self._codes, self._scales = codes, scales
         self.pages, self.kv_heads, _, self.block, self.head_dim = codes.shape
         self.device, self._index = codes.device, codes.get_device()
         self._view = bytes(abi.KvCache(codes=codes.data_ptr(), scales=scales.data_ptr(),
                                        pages=self.pages, kv_heads=self.kv_heads,
                                        block=self.block, head_dim=self.head_dim))
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
+
+    def __reduce__(self):  # no addresses: they are taken of the copied tensors
+        return type(self).over, (self._codes, self._scales)
 
     # ------------------------------------------------------------- descriptions
 

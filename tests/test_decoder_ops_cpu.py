@@ -2,7 +2,9 @@
 that the C interface refuses before any launch (the pointers are never
 followed), and what the Python side refuses without a device."""
 
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -155,3 +157,32 @@ def test_cpu_tensors_and_shapes_are_refused():
 def test_status_messages():
     assert native.status_message(0x400) == "key/value cache page, length or start out of range"
     assert native.status_message(0x800) == "key/value cache does not support NaN or infinity"
+
+
+def host_cache():
+    """A cache whose tensors lie on the host, for what happens before a launch."""
+    c = Int8KVCache.__new__(Int8KVCache)
+    c._init(torch.zeros(2, 1, 2, 16, 16, dtype=torch.int8), torch.zeros(2, 1, 2))
+    return c
+
+
+def test_the_cache_keeps_the_memory_that_its_calls_use():
+    c = host_cache()
+    at = abi.KvCache.from_buffer_copy(c._view).codes, abi.KvCache.from_buffer_copy(c._view).scales
+    storages = c.codes.untyped_storage(), c.scales.untyped_storage()
+    for name in ("codes", "scales"):
+        # A rebound name would let the memory go that the calls still address.
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+        getattr(c, name).data = getattr(c, name).clone()
+    held = {t.data_ptr() for x in vars(c).values() for t in (x if isinstance(x, tuple) else (x,))
+            if isinstance(t, torch.Tensor)}
+    assert at == tuple(s.data_ptr() for s in storages) and held >= set(at)
+
+
+def test_copies_do_not_take_addresses_along():
+    """They are made anew over the copied tensors, which have to be on a device."""
+    c = host_cache()
+    for copied in (copy.copy, copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))):
+        with pytest.raises(TypeError, match="CUDA"):
+            copied(c)

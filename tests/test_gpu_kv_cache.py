@@ -1,7 +1,9 @@
 """The 8-bit key/value cache and attention over it against their definitions in
 64 bits (tests/decoder_reference.py)."""
 
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -631,3 +633,20 @@ def test_a_decoder_block_of_cim_layers():
         stream = x.double() + torch.sigmoid(gate.double()) * ref.norm(f.double(), "rms", post.weight)
         assert torch.allclose(h.double(), stream, **near)
         assert torch.allclose(y2.double(), ref.norm(stream, "rms", pre.weight), **near)
+
+
+def test_copies_of_a_cache_are_caches_of_their_own():
+    s = Setup([20, 9], 2, 16, 16)
+    s.fill()
+    table, at, first = s.device(s.lengths, [0, 20, 29])
+    want = s.cache.read(table, at, first, tokens=29)
+    for other in (copy.deepcopy(s.cache), pickle.loads(pickle.dumps(s.cache))):
+        codes, scales = s.cache.codes.clone(), s.cache.scales.clone()
+        got = other.read(table, at, first, tokens=29)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        k = s.rows(29, 2, torch.float32).cuda()
+        other.write(k, k, table, at, first)
+        assert torch.equal(s.cache.codes, codes) and torch.equal(s.cache.scales, scales)
+        assert not torch.equal(other.codes, codes)
+    same = copy.copy(s.cache)
+    assert same.codes is s.cache.codes and same.scales is s.cache.scales
