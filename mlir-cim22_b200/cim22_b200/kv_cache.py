@@ -54,6 +54,8 @@ class Int8KVCache:
                  device: int | torch.device = 0) -> None:
         dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
         self._shape_check(pages, kv_heads, head_dim, block)
+        if dev.type != "cuda":
+            raise TypeError("the cache must lie on a CUDA device")
         self._init(torch.zeros(pages, kv_heads, 2, block, head_dim, dtype=torch.int8, device=dev),
                    torch.zeros(pages, kv_heads, 2, dtype=torch.float32, device=dev))
 

@@ -186,3 +186,10 @@ def test_copies_do_not_take_addresses_along():
     for copied in (copy.copy, copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))):
         with pytest.raises(TypeError, match="CUDA"):
             copied(c)
+
+
+@pytest.mark.parametrize("device", ["cpu", "meta", torch.device("cpu")])
+def test_a_cache_off_the_gpu_is_refused(device):
+    """Its calls would hand a kernel addresses of the host."""
+    with pytest.raises(TypeError, match="CUDA"):
+        Int8KVCache(2, 1, 16, 16, device=device)
