@@ -161,6 +161,13 @@ class Int8KVCache:
             raise TypeError(f"{name}'s last axis must be contiguous")
         return rows, of_heads
 
+    def _status_word(self, status: StatusWord | None) -> StatusWord:
+        if status is None:
+            return StatusWord(self.device)
+        if status.tensor.get_device() != self._index:
+            raise ValueError("status must be on the cache's device")
+        return status
+
     # -------------------------------------------------------------------- calls
 
     def write(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
@@ -182,7 +189,7 @@ class Int8KVCache:
             raise ValueError("k and v must have one shape and type")
         seqs = _SEQUENCES.pack(*self._sequences(table, lengths, starts, rows, most))
         own_status = status is None
-        status = status or StatusWord(self.device)
+        status = self._status_word(status)
         launch("cim22_cuda_kv_write", self._index, lib().cim22_cuda_kv_write, self._view, seqs,
                FLOAT_TYPES[k.dtype], k.data_ptr(), k_rows, k_heads, v.data_ptr(), v_rows, v_heads,
                status.tensor.data_ptr())
@@ -216,7 +223,7 @@ class Int8KVCache:
             raise ValueError("k and v must have one shape and type")
         seqs = _SEQUENCES.pack(*self._sequences(table, lengths, starts, rows, most))
         own_status = status is None
-        status = status or StatusWord(self.device)
+        status = self._status_word(status)
         launch("cim22_cuda_kv_read", self._index, lib().cim22_cuda_kv_read, self._view, seqs,
                FLOAT_TYPES[k.dtype], k.data_ptr(), v.data_ptr(), status.tensor.data_ptr())
         if own_status:
@@ -270,7 +277,7 @@ class Int8KVCache:
                                bool(causal), window, longest)
         seqs = _SEQUENCES.pack(*seqs)
         own_status = status is None
-        status = status or StatusWord(self.device)
+        status = self._status_word(status)
         buffer = None if workspace is None else workspace.buffer
         if buffer is not None and buffer.get_device() != self._index:
             raise ValueError("workspace must be on the cache's device")

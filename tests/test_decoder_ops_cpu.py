@@ -9,7 +9,7 @@ import pickle
 import pytest
 import torch
 
-from cim22_b200 import abi, cim_ops, native
+from cim22_b200 import abi, cim_ops, kv_cache, native
 from cim22_b200.kv_cache import Int8KVCache
 
 HERE = 4096  # an address that is never read
@@ -193,3 +193,37 @@ def test_a_cache_off_the_gpu_is_refused(device):
     """Its calls would hand a kernel addresses of the host."""
     with pytest.raises(TypeError, match="CUDA"):
         Int8KVCache(2, 1, 16, 16, device=device)
+
+
+class Elsewhere:
+    """A tensor of another device, as far as the checks look."""
+
+    shape = (1,)
+    dtype = torch.int32
+
+    def get_device(self):
+        return 5
+
+    def data_ptr(self):
+        return HERE
+
+
+def test_a_status_word_of_another_device_is_refused(monkeypatch):
+    """The kernels write to it."""
+    launched = []
+    monkeypatch.setattr(kv_cache, "launch", lambda *a: launched.append(a))
+    c = host_cache()
+    status = cim_ops.StatusWord(torch.device("cpu"))
+    k, q = torch.zeros(2, 1, 16), torch.zeros(2, 2, 16)
+    table, lengths = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    calls = [lambda: c.write(k, k, table, lengths, status=status),
+             lambda: c.read(table, lengths, out=(k, k.clone()), status=status),
+             lambda: c.attend(q, table, lengths, status=status)]
+    for call in calls:
+        call()
+    assert len(launched) == 3
+    status.tensor = Elsewhere()
+    for call in calls:
+        with pytest.raises(ValueError, match="status"):
+            call()
+    assert len(launched) == 3

@@ -650,3 +650,15 @@ def test_copies_of_a_cache_are_caches_of_their_own():
         assert not torch.equal(other.codes, codes)
     same = copy.copy(s.cache)
     assert same.codes is s.cache.codes and same.scales is s.cache.scales
+
+
+def test_a_status_word_on_the_host_is_refused():
+    s = Setup([20, 9], 2, 16, 16)
+    q, k = s.rows(9, 4, torch.float32).cuda(), s.rows(9, 2, torch.float32).cuda()
+    table, at, first = s.device(s.lengths, [0, 6, 9])
+    host = StatusWord(torch.device("cpu"))
+    for call in (lambda: s.cache.attend(q, table, at, first, status=host),
+                 lambda: s.cache.read(table, at, first, tokens=9, status=host),
+                 lambda: s.cache.write(k, k, table, at, first, status=host)):
+        with pytest.raises(ValueError, match="status"):
+            call()
