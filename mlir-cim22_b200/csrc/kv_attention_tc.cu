@@ -31,6 +31,7 @@
 // their results are joined at the end. It serves few rows, and f32 queries,
 // whose rows are two f16 parts and need the second tile's shared memory.
 #include "kv_attention.h"
+#include "kv_convert.h"
 
 #include <algorithm>
 
@@ -745,42 +746,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       }
     };
     uint4 hold[2][kSteps];
-    const int parts = 2 * count;
-    auto used = [&](int j) { // this warp has read part j's places
-      __syncwarp();
-      if (lane == 0)
-        bar_arrive(&sm.index_empty[j % kIndex]);
+    // True for all of the warp or none.
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, bar_wait(bar, parity, failed));
     };
-    bool ok = parts == 0 || bar_wait(&sm.index_full[0], 0, failed);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok && parts > 0) {
-      load(0, 0, hold[0]);
-      load(0, 1, hold[1]);
-      used(0);
-    }
-    for (int j = 0; j < parts && ok; ++j) {
-      const bool more = j + 1 < parts;
-      // A tile's slot was emptied by the product of the tile before last.
-      if (j >= 4)
-        ok = bar_wait(&sm.kv_empty[0][(j >> 1) & 1], ((j >> 2) - 1) & 1, failed);
-      store(0, j, hold[0]);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(&sm.kv_full[0][j & 3]);
-      if (more) {
-        ok = bar_wait(&sm.index_full[(j + 1) % kIndex], ((j + 1) / kIndex) & 1, failed) && ok;
-        load(j + 1, 0, hold[0]);
-      }
-      if (j >= 4)
-        ok = bar_wait(&sm.kv_empty[1][(j >> 1) & 1], ((j >> 2) - 1) & 1, failed) && ok;
-      store(1, j, hold[1]);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(&sm.kv_full[1][j & 3]);
-      if (more) {
-        load(j + 1, 1, hold[1]);
-        used(j + 1);
-      }
-      ok = __all_sync(0xffffffffu, ok);
-    }
+    convert_parts(
+        2 * count,
+        [&](int j) { return wait(&sm.index_full[j % kIndex], (j / kIndex) & 1); },
+        [&](int side, int j) { return wait(&sm.kv_empty[side][(j >> 1) & 1], ((j >> 2) - 1) & 1); },
+        [&](int j, int side) { load(j, side, hold[side]); },
+        [&](int side, int j) {
+          store(side, j, hold[side]);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          bar_arrive(&sm.kv_full[side][j & 3]);
+        },
+        [&](int j) { // this warp has read part j's places
+          __syncwarp();
+          if (lane == 0)
+            bar_arrive(&sm.index_empty[j % kIndex]);
+        });
   } else {
     if (warp == 20) {
       // ----------------------------------------------------------- products
