@@ -602,7 +602,7 @@ extern "C" int cim22_cuda_block_norm(const cim22_block_norm *d, void *stream) {
   a.gate_stride = d->gate_stride;
   a.h_stride = d->h_stride;
   a.y_stride = d->y_stride;
-  a.gate_rows = d->gate_rows;
+  a.gate_rows = std::min(d->gate_rows, d->rows); // as much as any more; divided by in 32 bits
   a.type = d->type;
   a.gate_type = d->gate_type;
   a.gate_columns = static_cast<int>(d->gate_columns == d->dim ? 0 : 1);

@@ -1,10 +1,12 @@
 """Block norm against its definition in 64 bits."""
 
+import ctypes
+
 import pytest
 import torch
 
 import decoder_reference as ref
-from cim22_b200 import cim_ops
+from cim22_b200 import abi, cim_ops, native
 from cim22_b200.cim_ops import Norm, block_norm
 
 pytestmark = pytest.mark.gpu
@@ -214,3 +216,19 @@ def test_on_another_stream():
 def test_refusals(call, error):
     with pytest.raises(error):
         call(make(4, 32, torch.float32))
+
+
+@pytest.mark.parametrize("dim", [64, 61])
+@pytest.mark.parametrize("gate_rows", [7, 2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 62])
+def test_a_gate_row_for_more_rows_than_there_are(dim, gate_rows):
+    """The C entry takes any count of rows that share a gate row."""
+    x, gate = make(7, dim, torch.float32), make(1, dim, torch.float32, 4)
+    h = torch.empty_like(x)
+    call = abi.BlockNorm(type=abi.FLOAT32, rows=7, dim=dim, x=x.data_ptr(), x_stride=dim,
+                         residual=0, residual_stride=0, residual_scale=1.0,
+                         gate=gate.data_ptr(), gate_stride=dim, gate_rows=gate_rows,
+                         gate_columns=dim, gate_type=abi.FLOAT32, gate_activation=0,
+                         h=h.data_ptr(), h_stride=dim, y=0, y_stride=0)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert native.lib().cim22_cuda_block_norm(ctypes.byref(call), stream) == 0
+    assert torch.equal(h, x * gate)
