@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     const int key0 = (begin + j * (kG * kWarps)) << 4;
     bool whole = key0 + 16 * kG - 1 < s.length &&
                  (!a.causal || key0 + 16 * kG - 1 <= pos_first) &&
-                 (a.window <= 0 || key0 > pos_last - a.window);
+                 key0 >= window_start(a.window, pos_last);
 #pragma unroll
     for (int u = 0; u < kG; ++u)
       whole &= k[u].w != 0.0f;

@@ -79,17 +79,23 @@ __device__ __forceinline__ float nan_max(float a, float b) { // a NaN stays
   return b > a || b != b ? b : a;
 }
 
+// The first key within the window of a row at position p, which may lie far
+// before the sequence's start: p - window need not fit 32 bits.
+__device__ __forceinline__ int window_start(int window, int p) {
+  return window > 0 && p >= window ? p - window + 1 : 0;
+}
+
 // The range of keys [lo, hi) that rows at positions p0 .. p1 can see.
 __device__ __forceinline__ void key_range(const KvAttendArgs &a, int length, int p0, int p1,
                                           int &lo, int &hi) {
   hi = a.causal ? min(length, p1 + 1) : length;
-  lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+  lo = window_start(a.window, p0);
   if (hi < lo)
     hi = lo;
 }
 
 __device__ __forceinline__ bool sees(const KvAttendArgs &a, int length, int p, int key) {
-  return key < length && (!a.causal || key <= p) && (a.window <= 0 || key > p - a.window);
+  return key < length && (!a.causal || key <= p) && key >= window_start(a.window, p);
 }
 
 // Power-of-two factor 2^(141 - E) that brings a row whose largest magnitude

@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     const bool live = f < rows;
     const int pos = offset + (live ? f / a.group : 0);
     const int row_hi = !live ? 0 : a.causal ? min(s.length, pos + 1) : s.length;
-    const int row_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const int row_lo = window_start(a.window, pos);
     const float coef = sm.coef[kShare ? row : st * kM + row];
     float m = kNone, l = 0.0f;
     // What the stream carries: [split][stream][kv head][element][packed row],

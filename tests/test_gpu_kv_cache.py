@@ -662,3 +662,13 @@ def test_a_status_word_on_the_host_is_refused():
                  lambda: s.cache.write(k, k, table, at, first, status=host)):
         with pytest.raises(ValueError, match="status"):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 3, 2 ** 31 - 1])
+def test_windows_of_any_width_with_rows_before_the_start(dtype, causal, window):
+    """Positions down to -8 less the window do not fit 32 bits."""
+    s = Setup([2, 16, 0, 60], 2, 32, 16)
+    s.fill()
+    s.check_attend([5, 24, 4, 60], dtype, causal=causal, window=window)
