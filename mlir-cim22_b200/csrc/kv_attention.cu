@@ -275,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     for (int j = 0; j < kTiles; ++j)
       o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.0f;
   }
+  float widest = -INFINITY; // log2 of the largest value scale met
   // The pages of groups [64 i, 64 i + 32) are in batch_page, of the next 32 in
   // next_page; each is refilled when its last group has been taken.
   int round = 0, parity = 0, issued = min(count, kRounds - 1);
@@ -290,7 +291,13 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
             v.scales + (static_cast<int64_t>(page) * v.heads + head) * 2);
         const float sv = fmaxf(sc.y, kKvLeastScale);
         k = make_float4(sc.x, log2f(sv), 1.0f / sv, 1.0f);
+        widest = fmaxf(widest, k.y);
       }
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+        widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, o));
+      if (k.w != 0.0f && k.y < widest - kApart)
+        k.z = 0.0f;
       __syncwarp();
       constants[warp][lane] = k;
     }
@@ -361,6 +368,10 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
 #pragma unroll
     for (int u = 0; u < kG; ++u)
       whole &= k[u].w != 0.0f;
+    bool beside = false; // the same for the warp
+#pragma unroll
+    for (int u = 0; u < kG; ++u)
+      beside |= k[u].z == 0.0f;
     uint32_t pb[kG][kQ][kParts][2];
 #pragma unroll
     for (int t = 0; t < kQ; ++t) {
@@ -411,11 +422,11 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
 #pragma unroll
           for (int x = 4; x < 32; x *= 2)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          const float to = top - kTop<kParts>;
+          const float to = floorf(top - kTop<kParts>);
           if (to > m[t][r]) {
             const float shrink = exp2_approx(m[t][r] - to); // 0 for the first
+            l[t][r] = weigh(l[t][r], m[t][r] - to);
             m[t][r] = to;
-            l[t][r] *= shrink;
 #pragma unroll
             for (int j2 = 0; j2 < kTiles; ++j2) {
               o[t][j2][r] *= shrink;
@@ -424,6 +435,23 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
           }
         }
         arguments();
+      }
+      if (beside) { // weights of groups far below the largest value scale
+#pragma unroll
+        for (int u = 0; u < kG; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float slope = coef[t][r] * k[u].x;
+            const bool hide0 = hidden >> (4 * u + r) & 1, hide1 = hidden >> (4 * u + r + 2) & 1;
+            const float best = fmaxf(hide0 ? -INFINITY : sc[u][t][r] * slope,
+                                     hide1 ? -INFINITY : sc[u][t][r + 2] * slope);
+            if (k[u].z == 0.0f && best > -INFINITY) {
+              const float e = ceilf(best);
+              l[t][r] += weigh((hide0 ? 0.0f : exp2_approx(fmaf(sc[u][t][r], slope, -e))) +
+                                   (hide1 ? 0.0f : exp2_approx(fmaf(sc[u][t][r + 2], slope, -e))),
+                               e - m[t][r]);
+            }
+          }
       }
 #pragma unroll
       for (int u = 0; u < kG; ++u) {
@@ -541,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     for (int o = 16; o; o >>= 1)
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float share = exp2_approx(mine - top);
-    sum *= share;
+    sum = weigh(sum, mine - top);
 #pragma unroll
     for (int o = 16; o; o >>= 1)
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -627,15 +655,15 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
     for (int u = 0; u < kAhead; ++u)
       to = fmaxf(to, ml[u].x);
     const float shrink = exp2_approx(m - to);
+    sum = weigh(sum, m - to);
     m = to;
-    sum *= shrink;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       acc[e] *= shrink;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const float share = exp2_approx(ml[u].x - m);
-      sum = fmaf(ml[u].y, share, sum);
+      sum += weigh(ml[u].y, ml[u].x - m);
       acc[0] = fmaf(p[u].x, share, acc[0]);
       acc[1] = fmaf(p[u].y, share, acc[1]);
       acc[2] = fmaf(p[u].z, share, acc[2]);
@@ -660,7 +688,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
       const float2 ml = warp_ml[x];
       const float4 p = warp_o[x][lane];
       const float share = exp2_approx(ml.x - top);
-      sum = fmaf(ml.y, share, sum);
+      sum += weigh(ml.y, ml.x - top);
       acc[0] = fmaf(p.x, share, acc[0]);
       acc[1] = fmaf(p.y, share, acc[1]);
       acc[2] = fmaf(p.z, share, acc[2]);

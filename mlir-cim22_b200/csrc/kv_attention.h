@@ -58,10 +58,20 @@ namespace {
 //   out = sum_j p_j * code_j / l,   l = sum_j p_j / value_scale_j,
 // so the products take the codes alone (exact in f16), p needs no range
 // beyond its own maximum, and one multiply a block scales l.
+// l does need more. Value scales reach from 2^-87 (a block of zeros) to 2^121,
+// and where they lie far apart a key of much weight has a p below f32's range,
+// although its part of l, 2^(score - m), is within it. Blocks whose scale is
+// below 2^-kApart times the largest one met therefore carry 0 in place of 1 /
+// value_scale, and their weights are computed by themselves, relative to their
+// own largest. What p loses of the others weighs at most 2^(kApart - 126) of the
+// largest weight a key. m and the references of such sums are integers, so that
+// differences of far ones are exact. (A block of zeros beside values of up to
+// 16 is not that far apart.)
 // Value scales below kKvLeastScale count as it (the writer's least one).
+constexpr float kApart = 84.0f;
 constexpr float kKvLeastScale = 0x1p-87f;
-// p is kept at most 2^kTop when the reference is set and may grow to
-// 2^kGrowth before it is set again. f16 (largest 65504, steps of 2^-24) then
+// p is kept below 2^(kTop + 1), the row's largest at 2^kTop or more, when the
+// reference is set and may grow to 2^kGrowth before it is set again. f16 (largest 65504, steps of 2^-24) then
 // holds every p to within 2^-11 of itself or 2^-31 of the largest; with two
 // parts (f32 queries), which set it again sooner, to within 2^-22 or 2^-38.
 // kNone: the reference of a row that has seen no key.
@@ -73,6 +83,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// l * 2^d of a sum of weights, where 2^d alone may lie below f32's range.
+__device__ __forceinline__ float weigh(float l, float d) {
+  return d > -100.0f ? l * exp2_approx(d) : l * 0x1p-100f * exp2_approx(d + 100.0f);
 }
 
 __device__ __forceinline__ float nan_max(float a, float b) { // a NaN stays

@@ -34,6 +34,7 @@
 #include "kv_convert.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cim {
 namespace {
@@ -64,6 +65,7 @@ template <int kCh> struct alignas(1024) PromptSmem {
   uint64_t s_full[2], p_full[2], o_full[2], done;
   uint32_t tmem;
   int failed;
+  uint2 range[16]; // least and largest value scale (bits) that each softmax warp found
 };
 
 __device__ __forceinline__ uint32_t smem_at(const void *p) {
@@ -222,6 +224,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// Score to exponent: a positive slope (of nearly nothing where the row or the
+// scale is zero) leaves what is hidden at -infinity.
+__device__ __forceinline__ float score_slope(float coef, float key_scale) {
+  const float slope = coef * key_scale;
+  return slope < 1e-37f ? 1e-37f : slope;
+}
+
 // In the order written: all of a tile's at once would not leave registers for
 // its scores.
 __device__ __forceinline__ float4 load_scale(uint32_t at) {
@@ -270,6 +279,38 @@ __device__ __forceinline__ float2 exp2_pair(float2 x) {
 
 __device__ __forceinline__ void tmem_stored() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// The weights, relative to 2^m, of a row's keys in groups far below the largest
+// value scale, of 64 keys whose scores lie at `scores` in TMEM. The row sees keys
+// from .. to - 1 of them.
+__device__ __noinline__ float apart_weights(uint32_t scores, uint32_t scales, float far, int from,
+                                            int to, float coef, float m) {
+  float l = 0.0f;
+  for (int g = 0; g < kSub / 16; ++g) {
+    const float4 sc = load_scale(scales + 16 * g);
+    if (!(sc.y < far) || sc.y == -INFINITY) // the same for the warp
+      continue;
+    const float slope = score_slope(coef, sc.x);
+    for (int c = 16 * g; c < 16 * (g + 1); c += 8) {
+      uint32_t y[8];
+      tmem_load8(scores + c, y);
+      float best = -INFINITY, w = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i >= from && c + i < to)
+          best = fmaxf(best, __uint_as_float(y[i]));
+      if (best > -INFINITY) {
+        const float e = ceilf(best * slope);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i >= from && c + i < to)
+            w += exp2_approx(fmaf(__uint_as_float(y[i]), slope, -e));
+        l += weigh(w, e - m);
+      }
+    }
+  }
+  return l;
 }
 
 // kCount neighbouring elements of a query row as f32, zero from `dim` on.
@@ -364,7 +405,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   const int tile0 = min(all, split * each), count = min(all, tile0 + each) - tile0;
   const int key_base = (first16 << 4) + tile0 * kTile; // of this CTA's tile 0
 
-  // Queries: a warp takes every 16th row, a lane 2 * kCh neighbouring elements.
+  // The softmax warps look over the value scales: a page's table entry before
+  // the queries, its scale after them, so that neither is waited for.
+  const int first_page = key_base >> v.block_log2;
+  const int pages =
+      count > 0 ? ((min(key_base + count * kTile, s.length) - 1) >> v.block_log2) - first_page + 1 : 0;
+  auto value_scale = [&](int page) {
+    return page >= 0 ? fmaxf(v.scales[(static_cast<int64_t>(page) * v.heads + head) * 2 + 1], kKvLeastScale)
+                     : 0.0f;
+  };
+  const int thread = static_cast<int>(threadIdx.x);
+  const int page = thread < min(pages, 512) ? kv_page(v, b, first_page + thread) : -1;
+
+  // Queries: a warp takes every 24th row, a lane 2 * kCh neighbouring elements.
   const bool negative = a.scale_log2 < 0.0f; // the products then take -q
 #pragma unroll 4
   for (int r = warp; r < kRows; r += kThreads / 32) {
@@ -416,15 +469,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         *reinterpret_cast<uint32_t *>(to + kCh * kPanel) = l[0];
     }
   }
+  const float first_scale = value_scale(page);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0); // columns: scores [stream][128], outputs [stream][kD]
   int *failed = &sm.failed;
-
   if (warp < 16) {
     // ------------------------------------------------------------- softmax
+    // The range of the value scales decides how the weights are summed.
+    uint32_t least = 0x7f800000u, most = 0; // bits: they are positive
+    auto widen = [&](float scale) {
+      least = min(least, scale > 0.0f ? __float_as_uint(scale) : least);
+      most = max(most, __float_as_uint(scale));
+    };
+    widen(first_scale);
+    for (int i = thread + 512; i < pages; i += 512)
+      widen(value_scale(kv_page(v, b, first_page + i)));
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0)
+      sm.range[warp] = make_uint2(least, most);
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+    const uint2 range = sm.range[lane & 15];
+    least = __reduce_min_sync(0xffffffffu, range.x);
+    most = __reduce_max_sync(0xffffffffu, range.y);
+    const float far = log2f(__uint_as_float(most)) - kApart; // -infinity: no scales
+    const bool apart = log2f(__uint_as_float(least)) < far;
+
     const int st = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + st * kTile + lanes, o_at = tmem + 2 * kTile + st * kD + lanes;
@@ -445,8 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     float carried = 0.0f; // nothing yet
     const int mine = kShare ? (count - st + 1) / 2 : count;
     bool ok = true;
-#pragma unroll 1
-    for (int n = 0; n < mine; ++n) {
+    auto take = [&](auto with_apart, int n) { // the stream's n-th tile
       const int tile = kShare ? 2 * n + st : n;
       const int key0 = key_base + tile * kTile;
       const int from = min(max(row_lo - key0, 0), kTile), to = min(max(row_hi - key0, 0), kTile);
@@ -466,17 +538,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         for (int i = 0; i < 16; ++i)
           y[i] = key + i >= from && key + i < to ? y[i] : 0xff800000u; // -infinity
       };
-      // Score to exponent: a positive slope (of nearly nothing where the row or
-      // the scale is zero) leaves what is hidden at -infinity.
-      auto slope_of = [&](float key_scale) {
-        const float slope = coef * key_scale;
-        return slope < 1e-37f ? 1e-37f : slope;
-      };
       // A new reference for the rows that outgrew theirs (the first is kNone).
       auto refer = [&](bool grown, float to) {
         const float shrink = grown ? exp2_approx(m - to) : 1.0f; // 0 for the first
+        l = grown ? weigh(l, m - to) : l;
         m = grown ? to : m;
-        l *= shrink;
         carried *= shrink;
         if (n > 0 && !(carry && n % kFlush == 0)) {
           ok = bar_wait(&sm.o_full[st], (n - 1) & 1, failed) && ok;
@@ -516,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         }
         best = max3(best, __uint_as_float(y[14]), __uint_as_float(y[15]));
         const float4 sc = load_scale(scale_at + g * 16);
-        slopes[g] = slope_of(sc.x);
+        slopes[g] = score_slope(coef, sc.x);
         top = fmaxf(top, fmaf(fmaxf(best, next), slopes[g], sc.y));
       }
       // Both halves of a row have one reference.
@@ -563,7 +629,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       }
       const bool grown = top > (m == kNone ? -INFINITY : m + kGrowth<kParts>);
       if (__any_sync(0xffffffffu, grown))
-        refer(grown, top - kTop<kParts>);
+        refer(grown, floorf(top - kTop<kParts>));
+      if constexpr (decltype(with_apart)::value) {
+        tmem_loaded(x[0]);
+        l += apart_weights(from_at, scale_at, far, from - kSub * half, to - kSub * half, coef, m);
+        tmem_load_start(from_at, x[0]);
+      }
       const float origin = m == kNone ? 0.0f : m;
       // Probabilities over the scores: of every 32 columns 16 hold their f16,
       // the next 16 the small parts.
@@ -598,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
             low[i / 2] = pack_half(q.x - back.x, q.y - back.y);
           }
         }
-        l = fmaf(sum.x + sum.y, sc.z, l);
+        l = fmaf(sum.x + sum.y, decltype(with_apart)::value && sc.y < far ? 0.0f : sc.z, l);
         const uint32_t at = from_at + (g >> 1) * 32 + (g & 1) * 8;
         tmem_store8(at, high);
         if (kParts == 2 && (g & 1))
@@ -609,6 +680,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       bar_arrive(&sm.p_full[st]);
       if (lane == 0) // the warp is done with its part's scales
         bar_arrive(&sm.index_empty[part0]);
+    };
+    // Two loops, so that the ordinary one has nothing of far scales (in one, behind
+    // a test a tile, a prompt of 8,192 took 14 us more).
+    if (apart) {
+#pragma unroll 1
+      for (int n = 0; n < mine; ++n)
+        take(std::true_type{}, n);
+    } else {
+#pragma unroll 1
+      for (int n = 0; n < mine; ++n)
+        take(std::false_type{}, n);
     }
     if (mine > 0)
       ok = bar_wait(&sm.o_full[st], (mine - 1) & 1, failed) && ok;
@@ -649,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         const float most = fmaxf(m, m1);
         share = m == kNone ? 0.0f : exp2_approx(m - most);
         other = m1 == kNone ? 0.0f : exp2_approx(m1 - most);
-        l = l * share + sm.join[1][row] * other; // NaN stays
+        l = weigh(l, m - most) + weigh(sm.join[1][row], m1 - most); // NaN stays
         m = most;
       }
     }

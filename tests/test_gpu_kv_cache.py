@@ -672,3 +672,74 @@ def test_windows_of_any_width_with_rows_before_the_start(dtype, causal, window):
     s = Setup([2, 16, 0, 60], 2, 32, 16)
     s.fill()
     s.check_attend([5, 24, 4, 60], dtype, causal=causal, window=window)
+
+
+def check_far_scales(s, q, length, causal, paddings, bounds):
+    """As check_attend, but a block's log2 of its scale is below 128 and off by up
+    to an ulp, 2^-17, as is the exponent that it goes into; so is the logarithm
+    of the sum of weights over scales in lse."""
+    new, heads, dtype = q.shape[0], q.shape[1], q.dtype
+    table, at, first = s.device([length], [0, new])
+    held = [s.host.values(s.table[0], length, side) for side in range(2)]
+    want, want_lse, size, reach, peak = ref.attend(
+        q, *held, length - new, s.dim ** -0.5, causal, 0,
+        s.host.value_scales(s.table[0], length))
+    parts = 2 if dtype == torch.float32 else 1
+    step = 2.0 ** -22
+    p_err = torch.finfo(torch.float16).eps / 2 if parts == 1 else step
+    delta = (parts * (s.dim / 16) + 6) * step * reach + 2 * 2.0 ** -17
+    steps = (length / 16 + 70) * step
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + size * (
+        2 * p_err + 2 * delta + steps)[..., None] + (
+        127 * 2.0 ** (-31 if parts == 1 else -38)) * peak[..., None]
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -25
+    lse_tol = delta + steps + 2 * 2.0 ** -17
+    for rows in paddings:
+        more = torch.cat([q, torch.full((rows - new, heads, s.dim), math.nan, dtype=dtype)])
+        for longest in bounds:
+            out, lse = s.cache.attend(more.cuda(), table, at, first, causal=causal,
+                                      longest=longest, return_lse=True, status=s.status)
+            s.status.raise_if_set()
+            off = (out[:new].double().cpu() - want).abs()
+            assert bool((off <= tol).all()), (
+                rows, longest, float((off / tol.clamp(min=1e-300)).max()))
+            lse_off = (lse[:new].double().cpu() - want_lse).abs()
+            assert bool((lse_off <= lse_tol).all()), (rows, longest, float(lse_off.max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", ["small first", "large first", "mixed"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_value_scales_further_apart_than_exponents_reach(dtype, order, new):
+    """Blocks of zeros (the least scale, 2^-87) beside values near 1e30 (65,000
+    for f16): every key's weight counts, whatever its block's scale."""
+    n, large = 1120, 6e4 if dtype == torch.float16 else 1e30
+    s = Setup([n], 1, 32, 16)
+    k, v = s.rows(n, 1, torch.float32), s.rows(n, 1, torch.float32).clamp(-1, 1)
+    sizes = torch.tensor({"small first": [0, 0, 1e-20, 1, 0, large, 0],
+                          "large first": [large, 0, 0, 1, 1e-20, 0, 0],
+                          "mixed": [0, large, 0, 0, large, 1e-20, 0]}[order])
+    if order == "mixed":
+        sizes = sizes.repeat(10)  # every block of another size
+    v *= sizes.repeat_interleave(n // len(sizes))[:, None, None]
+    s.host.write(k, v, s.table, [n], [0, n])
+    table, at, first = s.device([n], [0, n])
+    s.cache.write(k.cuda(), v.cuda(), table, at, first, status=s.status)
+    q = s.rows(new, 2, dtype)
+    for causal, length in ((True, n), (False, n), (True, n // 7 * 2)):
+        check_far_scales(s, q, length, causal, (new, 7200, 38000), (64, n))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("where", [3, 580])
+def test_one_block_of_large_values_in_a_long_context(dtype, where):
+    """More pages than a CTA of the prompt kernel has threads to look at them."""
+    n = 600 * 16
+    s = Setup([n], 1, 16, 16)
+    k, v = s.rows(n, 1, torch.float32) * 0.5, torch.zeros(n, 1, 16)
+    v[16 * where:16 * where + 16] = 1e30
+    s.host.write(k, v, s.table, [n], [0, n])
+    table, at, first = s.device([n], [0, n])
+    s.cache.write(k.cuda(), v.cuda(), table, at, first, status=s.status)
+    check_far_scales(s, s.rows(40, 1, dtype), n, True, (40, 38000), (64, n))
