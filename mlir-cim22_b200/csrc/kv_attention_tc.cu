@@ -506,7 +506,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     const int pos = offset + (live ? f / a.group : 0);
     const int row_hi = !live ? 0 : a.causal ? min(s.length, pos + 1) : s.length;
     const int row_lo = window_start(a.window, pos);
-    const float coef = sm.coef[kShare ? row : st * kM + row];
+    // A row that sees nothing takes no NaN from its query: what is hidden stays so.
+    const float coef = row_lo < row_hi ? sm.coef[kShare ? row : st * kM + row] : 0.0f;
     float m = kNone, l = 0.0f;
     // What the stream carries: [split][stream][kv head][element][packed row],
     // to be multiplied by `carried`.

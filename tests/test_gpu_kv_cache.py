@@ -743,3 +743,28 @@ def test_one_block_of_large_values_in_a_long_context(dtype, where):
     table, at, first = s.device([n], [0, n])
     s.cache.write(k.cuda(), v.cuda(), table, at, first, status=s.status)
     check_far_scales(s, s.rows(40, 1, dtype), n, True, (40, 38000), (64, n))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 4000, 38000])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_not_finite_query_that_sees_nothing_gives_zeros(dtype, rows, causal):
+    """Rows before the start, in one tile with rows that see keys."""
+    s = Setup([3], 2, 32, 16)
+    s.fill()
+    table, at, first = s.device([3], [0, 5])
+    q = torch.zeros(rows, 4, 32, dtype=dtype)
+    q[:5] = s.rows(5, 4, dtype)
+    clean = q.clone()
+    q[0], q[1, :, 3], q[3, 1, 2] = math.nan, math.inf, -math.inf
+    kw = dict(return_lse=True, causal=causal, window=0 if causal else 2, status=s.status)
+    out, lse = s.cache.attend(q.cuda(), table, at, first, **kw)
+    want, want_lse = s.cache.attend(clean.cuda(), table, at, first, **kw)
+    s.status.raise_if_set()
+    blind = 2 if causal else 0  # without a causal mask every row sees what follows it
+    assert bool((out[:blind] == 0).all()) and bool((lse[:blind] == -math.inf).all())
+    assert bool(torch.isnan(out[3, 1]).all()) and bool(torch.isnan(lse[3, 1]))
+    assert torch.equal(out[2], want[2]) and torch.equal(out[4], want[4])
+    assert torch.equal(lse[2], want_lse[2]) and torch.equal(lse[4], want_lse[4])
+    if not causal:
+        assert bool(torch.isnan(out[:2]).all())
