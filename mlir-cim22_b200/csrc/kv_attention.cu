@@ -782,10 +782,14 @@ struct Plan {
 // than places, 16 of 300 with 64 rows, 37 | 27).
 constexpr int64_t kDecodeRows = 32, kDecodeWork = 1 << 17;
 
+// Rows that a launch is sized for: one at least, since a sequence with more rows
+// than the bound is reported by the kernels.
+int64_t most_rows(const KvView &v) { return std::max<int64_t>(1, std::min<int64_t>(v.most, v.rows)); }
+
 Plan attend_plan(const KvView &v, const cim22_kv_attention &t) {
   Plan p{};
   const int64_t group = t.q_heads / v.heads;
-  const int64_t rows = std::min<int64_t>(v.most, v.rows) * group;
+  const int64_t rows = most_rows(v) * group;
   const int64_t held = static_cast<int64_t>(v.table_width) << v.block_log2;
   const int64_t longest = std::max<int64_t>(1, std::min(t.longest, held));
   const int64_t tiles16 = (rows + 15) / 16 * v.heads * v.batch;
@@ -880,7 +884,7 @@ cudaError_t launch_attend(const KvAttendArgs &a, int type, const Plan &plan, cud
       : plan.few  ? launch_decode<T, kParts, 1>(a, plan.tiles, stream)
                   : launch_decode<T, kParts, 2>(a, plan.tiles, stream);
   if (e == cudaSuccess && a.splits > a.cluster) {
-    const int64_t rows = std::min<int64_t>(a.v.most, a.v.rows) * a.q_heads;
+    const int64_t rows = most_rows(a.v) * a.q_heads;
     e = a.splits / a.cluster <= 8
             ? launch_pdl(kv_join_kernel<T, 1>, dim3(static_cast<unsigned>((rows + 3) / 4), 1, a.v.batch),
                          dim3(128), 0, stream, a)

@@ -768,3 +768,31 @@ def test_a_not_finite_query_that_sees_nothing_gives_zeros(dtype, rows, causal):
     assert torch.equal(lse[2], want_lse[2]) and torch.equal(lse[4], want_lse[4])
     if not causal:
         assert bool(torch.isnan(out[:2]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("rows,longest", [(9, 20), (3000, 20), (3000, 100000)])
+def test_no_rows_to_a_sequence(dtype, rows, longest):
+    """A bound of no rows: nothing to do where there are none, an index error
+    where there are some."""
+    s = Setup([20, 9], 1, 16, 16, width=7000)
+    s.fill()
+    q = s.rows(rows, 2, dtype).cuda()
+    k = s.rows(rows, 1, dtype).cuda()
+    out = torch.full_like(q, 5.0)
+    pair = torch.full_like(k, 5.0), torch.full_like(k, 5.0)
+    for starts, error in (([0, 0, 0], False), ([0, 6, 9], True)):
+        table, at, first = s.device(s.lengths, starts)
+        codes = s.cache.codes.clone()
+        for call in (lambda: s.cache.attend(q, table, at, first, most=0, longest=longest, out=out,
+                                            status=s.status),
+                     lambda: s.cache.read(table, at, first, most=0, out=pair, status=s.status),
+                     lambda: s.cache.write(k, k, table, at, first, most=0, status=s.status)):
+            call()
+            if error:
+                with pytest.raises(RuntimeError, match="page, length or start out of range"):
+                    s.status.raise_if_set()
+                s.status.reset()
+            s.status.raise_if_set()
+        assert all(bool((t == 5).all()) for t in (out, *pair))
+        assert torch.equal(s.cache.codes, codes)
