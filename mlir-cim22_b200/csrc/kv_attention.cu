@@ -838,7 +838,7 @@ bool attend_args(const char *what, const KvView &v, const cim22_kv_attention *t)
     return refuse("strides must not be negative");
   if (!(t->scale == t->scale) || t->scale - t->scale != 0.0f)
     return refuse("scale must be finite");
-  if (static_cast<int64_t>(v.most) * (t->q_heads / v.heads) > 0x3fffffff)
+  if (most_rows(v) * (t->q_heads / v.heads) > 0x3fffffff)
     return refuse("too many query rows");
   return true;
 }

@@ -796,3 +796,18 @@ def test_no_rows_to_a_sequence(dtype, rows, longest):
             s.status.raise_if_set()
         assert all(bool((t == 5).all()) for t in (out, *pair))
         assert torch.equal(s.cache.codes, codes)
+
+
+@pytest.mark.parametrize("most", [31, 1000, 2 ** 31 - 1])
+def test_a_bound_of_rows_past_those_there_are(most):
+    s = Setup([20, 31], 1, 16, 16)
+    s.fill()
+    table, at, first = s.device(s.lengths, [0, 20, 51])
+    q, k = s.rows(51, 4, torch.float32).cuda(), s.rows(51, 1, torch.float32).cuda()
+    want = s.cache.attend(q, table, at, first, most=31, status=s.status)
+    assert torch.allclose(s.cache.attend(q, table, at, first, most=most, status=s.status), want,
+                          rtol=2.0 ** -18, atol=2.0 ** -18)
+    s.cache.write(k, k, table, at, first, most=most, status=s.status)
+    got = s.cache.read(table, at, first, tokens=51, most=most, status=s.status)
+    assert torch.equal(got[0], got[1])
+    s.status.raise_if_set()
