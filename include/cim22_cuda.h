@@ -822,8 +822,8 @@ int cim22_cuda_block_norm(const cim22_block_norm *description, void *stream);
  * lengths[b] counts the tokens that sequence b holds with this call's tokens,
  * which are its last n_b; their rows are packed, sequence b's from starts[b]
  * to starts[b + 1] - 1 (starts NULL: one row for every sequence). A token at
- * a negative position (lengths[b] < n_b, such as an empty slot's) is neither
- * written nor read. Rows from starts[batch] on are left alone. Offsets,
+ * a negative position (lengths[b] < n_b, such as an empty slot's) is not
+ * written, and reads as zeros. Rows from starts[batch] on are left alone. Offsets,
  * lengths or page numbers out of range are not followed: they set
  * CIM22_STATUS_CACHE_INDEX and the tokens in question are skipped. */
 typedef struct cim22_kv_cache {

@@ -202,8 +202,10 @@ class Int8KVCache:
              out: tuple[torch.Tensor, torch.Tensor] | None = None,
              status: StatusWord | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The values of each sequence's last starts[b + 1] - starts[b] tokens,
-        packed: (k, v), contiguous [tokens, kv_heads, head_dim]. tokens is the
-        number of packed rows (starts' last entry; the batch without starts)."""
+        packed: (k, v), contiguous [tokens, kv_heads, head_dim]; zeros for rows
+        that a sequence has no tokens for (an empty slot's). tokens is the number
+        of packed rows (starts' last entry; the batch without starts); rows behind
+        the last sequence's are left as they are."""
         if out is None:
             if dtype not in FLOAT_TYPES:
                 raise TypeError("dtype must be f32, bf16 or f16")

@@ -206,6 +206,19 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// Rows of one plane, dim elements each, shared by `ctas` CTAs. Out of line: few
+// calls have such rows, and within the kernel it took 10 registers more.
+template <typename T>
+__device__ __noinline__ void zero_rows(T *rows, int count, int dim, int64_t stride, int cta, int ctas) {
+  const Pack<T> none;
+  const int parts = dim / kVec<T>;
+  for (int64_t c = static_cast<int64_t>(cta) * kThreads + threadIdx.x;
+       c < static_cast<int64_t>(count) * parts; c += static_cast<int64_t>(ctas) * kThreads) {
+    const int64_t i = c / parts;
+    store_pack(rows + i * stride, (c - i * parts) * kVec<T>, dim, none);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     kv_read_kernel(const KvView v, T *__restrict__ k, T *__restrict__ values, const FastDiv parts,
@@ -225,10 +238,17 @@ __global__ void __launch_bounds__(kThreads)
       atomicOr(status, CIM22_STATUS_CACHE_INDEX);
     return;
   }
+  if (!out)
+    return;
+  const int64_t stride = static_cast<int64_t>(v.heads) * v.dim;
+  const int before = s.n - s.length; // rows before the sequence's start
+  if (before > 0)                    // are zeros; the plane's CTAs share them
+    zero_rows(out + s.row0 * stride + head * v.dim, before, v.dim, stride, touch,
+              gridDim.x / planes);
   const int begin = max(0, s.length - s.n);
   const int ordinal = (begin >> v.block_log2) + touch;
   const int64_t base = static_cast<int64_t>(ordinal) << v.block_log2;
-  if (!out || begin >= s.length || base >= s.length)
+  if (begin >= s.length || base >= s.length)
     return;
   const int page = kv_page(v, b, ordinal);
   if (page < 0) {
@@ -243,7 +263,6 @@ __global__ void __launch_bounds__(kThreads)
   const float scale = v.scales[(static_cast<int64_t>(page) * v.heads + head) * 2 + side];
   const int8_t *codes = kv_codes(v, page, head, side) + lo * v.dim;
   const int chunks = (hi - lo) * parts.d;
-  const int64_t stride = static_cast<int64_t>(v.heads) * v.dim;
   T *to = out + (row + lo) * stride + head * v.dim;
   const bool aligned = (reinterpret_cast<uintptr_t>(to) & 15) == 0; // rows are whole vectors
   constexpr int kUnroll = 4;

@@ -811,3 +811,30 @@ def test_a_bound_of_rows_past_those_there_are(most):
     got = s.cache.read(table, at, first, tokens=51, most=most, status=s.status)
     assert torch.equal(got[0], got[1])
     s.status.raise_if_set()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,dim,block", [(1, 16, 16), (3, 80, 32)])
+def test_rows_before_the_start_read_as_zeros(dtype, heads, dim, block):
+    s = Setup([5, 0, 70, 3, 2 * block], heads, dim, block)
+    s.fill()
+    new = [9, 40, 70, 1, 3 * block + 1]
+    first = [0]
+    for n in new:
+        first.append(first[-1] + n)
+    table, at, starts = s.device(s.lengths, first)
+    k, v = (torch.full((first[-1] + 6, heads, dim), 5.0, dtype=dtype, device="cuda")
+            for _ in range(2))
+    s.cache.read(table, at, starts, out=(k, v), status=s.status)
+    s.status.raise_if_set()
+    for side, got in enumerate((k, v)):
+        for b, n in enumerate(new):
+            want = torch.zeros(max(0, n - s.lengths[b]), heads, dim, dtype=dtype)
+            held = s.host.values(s.table[b], s.lengths[b], side)[-n:].float().to(dtype)
+            assert torch.equal(got[first[b]:first[b + 1]].cpu(), torch.cat([want, held]))
+        assert bool((got[first[-1]:] == 5).all())
+    # An empty slot of a fixed batch.
+    k, v = (torch.full((5, heads, dim), 5.0, dtype=dtype, device="cuda") for _ in range(2))
+    s.cache.read(table, at, out=(k, v), status=s.status)
+    assert bool((k[1] == 0).all()) and bool((v[1] == 0).all())
+    assert not bool((k == 5).all(-1).any())
