@@ -503,10 +503,16 @@ def _gate_rows(gate: torch.Tensor, x: torch.Tensor, rows: int, dim: int) -> tupl
     if gate.dim() >= 2 and gate.shape[-1] in (1, dim):
         columns = gate.shape[-1]
         lead = gate.numel() // columns
-        if rows == 0 or lead and rows % lead == 0:
+        fits = gate.dim() == 2
+        if gate.dim() > 2 and gate.dim() <= x.dim():
+            axes = list(gate.shape[:-1])
+            while axes and axes[-1] == 1:
+                axes.pop()
+            fits = axes == list(x.shape[:len(axes)])
+        if fits and (rows == 0 or lead and rows % lead == 0):
             return rows // lead if lead > 1 else 0, columns
-    raise ValueError("gate must be [dim], or [groups, dim] or [groups, 1] with groups dividing "
-                     "the rows")
+    raise ValueError("gate must be [dim]; [groups, dim] or [groups, 1] with groups dividing the "
+                     "rows; or have x's first axes, then axes of 1, then dim or 1")
 
 
 def _empty_rows(x: torch.Tensor) -> torch.Tensor:
@@ -529,8 +535,9 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     None when there is nothing to combine (no residual, post or gate) and y
     None without pre. gate is [dim]; [rows, dim] or [rows, 1]; or, for a batch
     of equally long sequences, [groups, dim] or [groups, 1] with groups
-    dividing the rows (consecutive rows share a gate row); f32 or x's type;
-    gate_activation None, "sigmoid" or "tanh". Arithmetic is f32, and y is
+    dividing the rows (consecutive rows share a gate row). With more axes it
+    has x's first ones, then any of 1, then dim or 1 ([batch, 1, dim], not [1,
+    length, dim]). It is f32 or x's type; gate_activation None, "sigmoid" or "tanh". Arithmetic is f32, and y is
     computed from h before h is rounded. out and normed receive h and y; they
     may be x or residual themselves (the same view), but not overlap them in
     any other way."""

@@ -227,3 +227,26 @@ def test_a_status_word_of_another_device_is_refused(monkeypatch):
         with pytest.raises(ValueError, match="status"):
             call()
     assert len(launched) == 3
+
+
+@pytest.mark.parametrize("x,gate,rows", [
+    ((12, 8), (8,), (0, 8)), ((12, 8), (1, 8), (0, 8)), ((12, 8), (3, 8), (4, 8)),
+    ((12, 8), (12, 1), (1, 1)), ((3, 4, 8), (3, 8), (4, 8)), ((3, 4, 8), (12, 8), (1, 8)),
+    ((3, 4, 8), (3, 4, 8), (1, 8)), ((3, 4, 8), (3, 4, 1), (1, 1)), ((3, 4, 8), (3, 1, 8), (4, 8)),
+    ((3, 4, 8), (1, 1, 8), (0, 8)), ((1, 4, 8), (1, 4, 8), (1, 8)),
+    ((2, 3, 4, 8), (2, 3, 8), (4, 8)), ((2, 3, 4, 8), (2, 1, 1, 1), (12, 1)),
+    ((0, 4, 8), (0, 4, 8), None)])
+def test_gate_shapes(x, gate, rows):
+    got = cim_ops._gate_rows(torch.zeros(gate), torch.zeros(x), torch.zeros(x).numel() // 8, 8)
+    assert rows is None or got == rows
+
+
+@pytest.mark.parametrize("x,gate", [
+    ((3, 4, 8), (1, 4, 8)), ((4, 4, 8), (1, 4, 8)), ((3, 4, 8), (1, 4, 1)), ((2, 3, 4, 8), (1, 3, 8)),
+    ((2, 3, 4, 8), (2, 1, 4, 8)), ((2, 3, 4, 8), (1, 3, 1, 8)), ((6, 2, 8), (2, 3, 8)),
+    ((12, 8), (3, 1, 8)), ((12, 8), (3, 4, 8)), ((3, 4, 8), (3, 4, 1, 8)), ((3, 4, 8), (4, 3, 8))])
+def test_gates_of_more_axes_that_are_no_prefix_of_the_rows_are_refused(x, gate):
+    """[1, T, dim] would broadcast over the batch anywhere else; its values must
+    not go to consecutive rows instead."""
+    with pytest.raises(ValueError, match="gate must be"):
+        cim_ops._gate_rows(torch.zeros(gate), torch.zeros(x), torch.zeros(x).numel() // 8, 8)

@@ -1,6 +1,7 @@
 """Block norm against its definition in 64 bits."""
 
 import ctypes
+import math
 
 import pytest
 import torch
@@ -232,3 +233,19 @@ def test_a_gate_row_for_more_rows_than_there_are(dim, gate_rows):
     stream = torch.cuda.current_stream().cuda_stream
     assert native.lib().cim22_cuda_block_norm(ctypes.byref(call), stream) == 0
     assert torch.equal(h, x * gate)
+
+
+@pytest.mark.parametrize("shape", [(3, 4, 64), (3, 4, 1), (3, 1, 64), (3, 1, 1), (1, 1, 64),
+                                   (3, 64)])
+def test_gates_of_more_axes(shape):
+    x, gate = make(12, 64, torch.float32).view(3, 4, 64), make(12, 64, torch.float32, 4)
+    gate = gate.flatten()[:math.prod(shape)].view(shape)
+    h, _ = block_norm(x, gate=gate)
+    assert torch.equal(h, x * (gate[:, None] if len(shape) == 2 else gate))
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 64), (1, 4, 1), (4, 3, 64), (3, 4, 1, 64), (2, 6, 64)])
+def test_gates_that_are_no_prefix_are_refused(shape):
+    x = make(12, 64, torch.float32).view(3, 4, 64)
+    with pytest.raises(ValueError, match="gate must be"):
+        block_norm(x, gate=torch.ones(shape, device="cuda"))
