@@ -838,3 +838,21 @@ def test_rows_before_the_start_read_as_zeros(dtype, heads, dim, block):
     s.cache.read(table, at, out=(k, v), status=s.status)
     assert bool((k[1] == 0).all()) and bool((v[1] == 0).all())
     assert not bool((k == 5).all(-1).any())
+
+
+@pytest.mark.parametrize("dim", [48, 128])
+def test_a_low_bound_of_lengths_costs_no_accuracy(dim):
+    """f32 prompts take their sums out of the accumulators by what the table can
+    hold: with one part of the key axis either way, the bits are the same."""
+    s = Setup([2900], 1, dim, 32)
+    s.fill()
+    table, at, first = s.device([2900], [0, 40])
+    q = torch.zeros(38000, 2, dim)
+    q[:40] = s.rows(40, 2, torch.float32)
+    q = q.cuda()
+    want, want_lse = s.cache.attend(q, table, at, first, return_lse=True, status=s.status)
+    for longest in (0, 64, 512, 2900, 10 ** 6):
+        out, lse = s.cache.attend(q, table, at, first, return_lse=True, longest=longest,
+                                  status=s.status)
+        assert torch.equal(out[:40], want[:40]) and torch.equal(lse[:40], want_lse[:40])
+    s.status.raise_if_set()
