@@ -57,8 +57,8 @@ class Workspace:
     may still use them (each is at least twice the one before)."""
 
     def __init__(self, device: torch.device) -> None:
-        self.device = device
         self.buffer = torch.empty(0, dtype=torch.uint8, device=device)
+        self.device = self.buffer.device  # with its index: it grows where it is
         self.outgrown: list[torch.Tensor] = []
 
     def get(self, nbytes: int) -> torch.Tensor:

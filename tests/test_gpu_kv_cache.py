@@ -856,3 +856,10 @@ def test_a_low_bound_of_lengths_costs_no_accuracy(dim):
                                   status=s.status)
         assert torch.equal(out[:40], want[:40]) and torch.equal(lse[:40], want_lse[:40])
     s.status.raise_if_set()
+
+
+def test_a_workspace_stays_on_its_device():
+    """A device without an index is the one that was current at the start."""
+    workspace = Workspace(torch.device("cuda"))
+    assert workspace.device == torch.device("cuda", torch.cuda.current_device())
+    assert workspace.get(1 << 20).device == workspace.device
