@@ -422,10 +422,10 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
 #pragma unroll
           for (int x = 4; x < 32; x *= 2)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          const float to = floorf(top - kTop<kParts>);
+          const float to = top - kTop<kParts>;
           if (to > m[t][r]) {
             const float shrink = exp2_approx(m[t][r] - to); // 0 for the first
-            l[t][r] = weigh(l[t][r], m[t][r] - to);
+            l[t][r] = weigh(l[t][r], m[t][r], to);
             m[t][r] = to;
 #pragma unroll
             for (int j2 = 0; j2 < kTiles; ++j2) {
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
               const float e = ceilf(best);
               l[t][r] += weigh((hide0 ? 0.0f : exp2_approx(fmaf(sc[u][t][r], slope, -e))) +
                                    (hide1 ? 0.0f : exp2_approx(fmaf(sc[u][t][r + 2], slope, -e))),
-                               e - m[t][r]);
+                               e, m[t][r]);
             }
           }
       }
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kParts, kQ>)
     for (int o = 16; o; o >>= 1)
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float share = exp2_approx(mine - top);
-    sum = weigh(sum, mine - top);
+    sum = weigh(sum, mine, top);
 #pragma unroll
     for (int o = 16; o; o >>= 1)
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
     for (int u = 0; u < kAhead; ++u)
       to = fmaxf(to, ml[u].x);
     const float shrink = exp2_approx(m - to);
-    sum = weigh(sum, m - to);
+    sum = weigh(sum, m, to);
     m = to;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const float share = exp2_approx(ml[u].x - m);
-      sum += weigh(ml[u].y, ml[u].x - m);
+      sum += weigh(ml[u].y, ml[u].x, m);
       acc[0] = fmaf(p[u].x, share, acc[0]);
       acc[1] = fmaf(p[u].y, share, acc[1]);
       acc[2] = fmaf(p[u].z, share, acc[2]);
@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendArgs a) {
       const float2 ml = warp_ml[x];
       const float4 p = warp_o[x][lane];
       const float share = exp2_approx(ml.x - top);
-      sum += weigh(ml.y, ml.x - top);
+      sum += weigh(ml.y, ml.x, top);
       acc[0] = fmaf(p.x, share, acc[0]);
       acc[1] = fmaf(p.y, share, acc[1]);
       acc[2] = fmaf(p.z, share, acc[2]);

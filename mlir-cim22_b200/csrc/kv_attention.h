@@ -64,14 +64,15 @@ namespace {
 // below 2^-kApart times the largest one met therefore carry 0 in place of 1 /
 // value_scale, and their weights are computed by themselves, relative to their
 // own largest. What p loses of the others weighs at most 2^(kApart - 126) of the
-// largest weight a key. m and the references of such sums are integers, so that
-// differences of far ones are exact. (A block of zeros beside values of up to
-// 16 is not that far apart.)
+// largest weight a key. (A block of zeros beside values of up to 16 is not that
+// far apart.)
 // Value scales below kKvLeastScale count as it (the writer's least one).
 constexpr float kApart = 84.0f;
 constexpr float kKvLeastScale = 0x1p-87f;
-// p is kept below 2^(kTop + 1), the row's largest at 2^kTop or more, when the
-// reference is set and may grow to 2^kGrowth before it is set again. f16 (largest 65504, steps of 2^-24) then
+// p is kept at most 2^kTop when the reference is set and may grow to 2^kGrowth
+// before it is set again: the largest is then a power of two, which f16 does not
+// round (with whole references one key of much weight in 200,000 was, and
+// outputs were off by 3.8e-4, not 2.0e-4, of which 2.0e-4 are their own). f16 (largest 65504, steps of 2^-24) then
 // holds every p to within 2^-11 of itself or 2^-31 of the largest; with two
 // parts (f32 queries), which set it again sooner, to within 2^-22 or 2^-38.
 // kNone: the reference of a row that has seen no key.
@@ -85,8 +86,14 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// l * 2^d of a sum of weights, where 2^d alone may lie below f32's range.
-__device__ __forceinline__ float weigh(float l, float d) {
+// l * 2^(a - b) of a sum of weights. Between far references 2^(a - b) alone may
+// lie below f32's range, and a - b rounds: their whole and broken parts are
+// then subtracted apart. Near ones take the factor that the outputs take.
+__device__ __forceinline__ float weigh(float l, float a, float b) {
+  if (fabsf(a - b) < 16.0f)
+    return l * exp2_approx(a - b);
+  const float d = rintf(a) - rintf(b);
+  l *= exp2_approx((a - rintf(a)) - (b - rintf(b)));
   return d > -100.0f ? l * exp2_approx(d) : l * 0x1p-100f * exp2_approx(d + 100.0f);
 }
 

@@ -306,7 +306,7 @@ __device__ __noinline__ float apart_weights(uint32_t scores, uint32_t scales, fl
         for (int i = 0; i < 8; ++i)
           if (c + i >= from && c + i < to)
             w += exp2_approx(fmaf(__uint_as_float(y[i]), slope, -e));
-        l += weigh(w, e - m);
+        l += weigh(w, e, m);
       }
     }
   }
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       // A new reference for the rows that outgrew theirs (the first is kNone).
       auto refer = [&](bool grown, float to) {
         const float shrink = grown ? exp2_approx(m - to) : 1.0f; // 0 for the first
-        l = grown ? weigh(l, m - to) : l;
+        l = grown ? weigh(l, m, to) : l;
         m = grown ? to : m;
         carried *= shrink;
         if (n > 0 && !(carry && n % kFlush == 0)) {
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       }
       const bool grown = top > (m == kNone ? -INFINITY : m + kGrowth<kParts>);
       if (__any_sync(0xffffffffu, grown))
-        refer(grown, floorf(top - kTop<kParts>));
+        refer(grown, top - kTop<kParts>);
       if constexpr (decltype(with_apart)::value) {
         tmem_loaded(x[0]);
         l += apart_weights(from_at, scale_at, far, from - kSub * half, to - kSub * half, coef, m);
@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         const float most = fmaxf(m, m1);
         share = m == kNone ? 0.0f : exp2_approx(m - most);
         other = m1 == kNone ? 0.0f : exp2_approx(m1 - most);
-        l = weigh(l, m - most) + weigh(sm.join[1][row], m1 - most); // NaN stays
+        l = weigh(l, m, most) + weigh(sm.join[1][row], m1, most); // NaN stays
         m = most;
       }
     }

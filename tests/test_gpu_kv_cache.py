@@ -863,3 +863,25 @@ def test_a_workspace_stays_on_its_device():
     workspace = Workspace(torch.device("cuda"))
     assert workspace.device == torch.device("cuda", torch.cuda.current_device())
     assert workspace.get(1 << 20).device == workspace.device
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new", [1, 64])
+def test_a_key_of_all_the_weight_loses_nothing(dtype, new):
+    """Its probability is a power of two when the reference is set by it, so that
+    rounding it to f16 costs nothing: the output is the value, rounded once
+    (2^-16 for its exponent, below 512 and so off by up to 2^-16, twice)."""
+    s = Setup([64], 1, 64, 16)
+    k, v = s.rows(64, 1, torch.float32), s.rows(64, 1, torch.float32)
+    s.host.write(k, v, s.table, [64], [0, 64])
+    table, at, first = s.device([64], [0, new])
+    s.cache.write(k.cuda(), v.cuda(), *s.device([64], [0, 64]), status=s.status)
+    want = s.host.values(s.table[0], 64, 1)[-new:]
+    for padding in (new, 15000, 40000):
+        q = torch.zeros(padding, 1, 64, dtype=dtype)
+        q[:new] = (20 * k[-new:]).to(dtype)  # 100 or more above every other key
+        out = s.cache.attend(q.cuda(), table, at, first, causal=False, status=s.status)
+        off = (out[:new].cpu().double() - want).abs()
+        tol = (torch.finfo(dtype).eps / 2 + 2 * 2.0 ** -16) * want.abs() + 2.0 ** -25
+        assert bool((off <= tol).all()), (padding, float((off / tol).max()))
+    s.status.raise_if_set()
