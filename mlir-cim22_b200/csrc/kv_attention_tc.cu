@@ -410,12 +410,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
   const int first_page = key_base >> v.block_log2;
   const int pages =
       count > 0 ? ((min(key_base + count * kTile, s.length) - 1) >> v.block_log2) - first_page + 1 : 0;
-  auto value_scale = [&](int page) {
-    return page >= 0 ? fmaxf(v.scales[(static_cast<int64_t>(page) * v.heads + head) * 2 + 1], kKvLeastScale)
-                     : 0.0f;
+  auto entry = [&](int i) { return v.table[b * v.table_stride + first_page + i]; };
+  auto value_scale = [&](int page) { // 0: no such page
+    return page >= 0 && page < v.pages
+               ? fmaxf(v.scales[(static_cast<int64_t>(page) * v.heads + head) * 2 + 1], kKvLeastScale)
+               : 0.0f;
   };
   const int thread = static_cast<int>(threadIdx.x);
-  const int page = thread < min(pages, 512) ? kv_page(v, b, first_page + thread) : -1;
+  int page = -1; // not looked at until the queries are done
+  if (thread < min(pages, 512))
+    page = entry(thread);
 
   // Queries: a warp takes every 24th row, a lane 2 * kCh neighbouring elements.
   const bool negative = a.scale_log2 < 0.0f; // the products then take -q
@@ -486,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     };
     widen(first_scale);
     for (int i = thread + 512; i < pages; i += 512)
-      widen(value_scale(kv_page(v, b, first_page + i)));
+      widen(value_scale(entry(i)));
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0)
