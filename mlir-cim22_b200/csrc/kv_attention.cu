@@ -2,7 +2,7 @@
 // dispatch between it and the tensor-memory kernel for prompts.
 //
 // Decode reads every cached code once: bound by HBM (64 sequences of 286,000
-// tokens in all, 8 kv heads of 128, bf16: 110 us, 5.3 TB/s; one of 200,000, 4 kv
+// tokens in all, 8 kv heads of 128, bf16: 112 us, 5.2 TB/s; one of 200,000, 4 kv
 // heads, 47 us, 4.4 TB/s with its filling and joining). The products are taken
 // transposed, S^T = K Q^T and O^T = V^T P^T (m16n8k16), so that 16 tokens or
 // 16 elements of the head fill the 16 rows and a tile needs only 8 query rows

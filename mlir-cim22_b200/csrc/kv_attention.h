@@ -77,6 +77,10 @@ constexpr float kKvLeastScale = 0x1p-87f;
 // parts (f32 queries), which set it again sooner, to within 2^-22 or 2^-38.
 // kNone: the reference of a row that has seen no key.
 constexpr float kNone = -1e30f;
+// One part costs f16 outputs some accuracy, since l takes the probabilities
+// unrounded: 2.7e-4 against 64 bits, not 2.1e-4, where many keys share the weight
+// (chunks of 1,024, window 4,096); bf16 outputs none (1.7e-3 both). Two parts
+// would double the second product.
 template <int kParts> constexpr float kTop = kParts == 2 ? 13.0f : 6.0f;
 template <int kParts> constexpr float kGrowth = kParts == 2 ? 15.0f : 14.0f;
 

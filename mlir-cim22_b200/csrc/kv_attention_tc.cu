@@ -6,8 +6,9 @@
 // operands fill shared memory's 128 bytes a cycle, and 1,024 of the
 // special-function units. A CTA therefore runs two streams of 128 query rows,
 // so that one's products cover the other's softmax (a prompt of 8,192, 32 heads
-// of 128 on 8, bf16: 0.64 ms, 860 TFLOP/s; 3 chunks of 1,024 in a window of
-// 4,096, 24 heads of 64: 472):
+// of 128 on 8, bf16: 0.65 ms, 844 TFLOP/s, in ten calls, 0.69 ms, 797, once the
+// clock falls at the power limit; 3 chunks of 1,024 each in a window of 4,096, 24
+// heads of 64: 171 us, 451, and of 1,024 and less 194 us, 240):
 //   warps 0-7, 8-15 softmax of stream 0 and 1: two threads a row, one for each
 //                   64 keys of a tile, scores from TMEM, probabilities back over
 //                   them as the f16 A operand (one thread a row left too few
@@ -47,7 +48,7 @@ constexpr int kPanel = 128 * 128;    // bytes: 128 rows of 64 f16
 // two parts a stream's sum is therefore taken out of the accumulators every
 // kFlush tiles and added to what it carries in memory, rounding to nearest
 // (0.7e-6 over 1,800 keys; 5 prompts of up to 1,500, 16 heads of 80 on 4: 129 ->
-// 161 us).
+// 161 us, now 166).
 constexpr int kFlush = 2;
 constexpr uint64_t kWaitLimit = 2000000000ull; // ns
 
@@ -261,7 +262,8 @@ __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&r)[8])
 // units work at their limit: n = rint(x) by adding 1.5 * 2^23, a polynomial in
 // f = x - n of [-0.5, 0.5] (least largest relative error, fitted by reweighted
 // least squares: 2.7e-6), n added to the exponent bits. Below 2^-120 it stays
-// there.
+// there, hidden keys included: in f16 that is 0, and to l it adds at most
+// 2^(kApart - 126) of the row's largest weight a key.
 __device__ __forceinline__ float2 exp2_pair(float2 x) {
   x.x = fmaxf(x.x, -120.0f);
   x.y = fmaxf(x.y, -120.0f);
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
       top = fmaxf(top, sm.tops[n & 1][st][half ^ 1][row]);
       if (kParts == 2 && carry && n > 0 && n % kFlush == 0) {
         // What is carried is read kAhead steps of 8 elements before it is used (a
-        // prompt of 4,096, 32 heads of 128: 477 us; 544 read in place).
+        // prompt of 4,096, 32 heads of 128: 544 us read in place, 477 so, now 488).
         constexpr int kSteps = kD / 16, kAhead = 2;
         const int d0 = half * (kD / 2), end = min(d0 + kD / 2, v.dim);
         float old[kAhead][8];
@@ -687,7 +689,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         bar_arrive(&sm.index_empty[part0]);
     };
     // Two loops, so that the ordinary one has nothing of far scales (in one, behind
-    // a test a tile, a prompt of 8,192 took 14 us more).
+    // a test a tile, a prompt of 8,192 took 14 us more). The other takes 732 us for
+    // that prompt with a block of zeros among 64, 993 with every second one.
     if (apart) {
 #pragma unroll 1
       for (int n = 0; n < mine; ++n)

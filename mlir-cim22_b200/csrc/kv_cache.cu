@@ -8,8 +8,8 @@
 // when the scale grew.
 //
 // Bound for prompts by HBM (values in, one byte a value out) and as much by the
-// issue of instructions (88% and 84% of the slots): 57,560 tokens of 8 heads of
-// 128 in bf16 81 us to write, 4.4 TB/s, and 70 to read back, 5.1 (128 threads a
+// issue of instructions (88% and 81% of the slots): 57,560 tokens of 8 heads of
+// 128 in bf16 81 us to write, 4.4 TB/s, and 71 to read back, 5.0 (128 threads a
 // block, for fewer warps to set up, 136 and 74). Single tokens are bound by
 // latency (length, page, scale and value loads in a row: 64 sequences, 8 heads,
 // 3.4 us).
